@@ -762,6 +762,87 @@ int hreg_debug_fps_cluster(int b, int n, int m, const float *points, float *temp
 int hreg_debug_gemm_tn_s(const float *A, int lda, const float *B, int ldb, int R, int N, int K,
                          float beta, void *ws, float *out, void *stream, int S);
 
+/* ------------------------------------------------------------------ token operators --
+ * Attention over token sequences with its backward pass and a bucketed relative position
+ * bias, dropout without a stored mask, and the gated residual with the norms around it
+ * (tok_attn.hip, tok_elem.hip).  All shapes are checked here; lengths and masks are read on
+ * the device and clamped there.  Row data is f32 or bf16, all of one call alike. */
+#define HREG_TOK_F32 0
+#define HREG_TOK_BF16 1
+#define HREG_TOK_MAX_BUCKETS 128
+#define HREG_TOK_MAX_THRESH 64
+
+/* o_i = sum_j softmax_j(scale q_i . k_j + bias[bucket(j - i - start)][h]) v_j for each batch
+ * entry and head; H query heads share Hk key heads in groups of H / Hk.  Strides are in
+ * elements, (batch, token, head); rows of D elements are contiguous, 16-byte aligned, D % 8 == 0,
+ * D <= 128.  k_len / q_len [B] (or NULL): valid keys / rows, clamped to [0, Nk] / [0, Nq];
+ * key_mask [B][Nk] bytes (batch stride mask_sb; or NULL): 0 = not seen.  Keys beyond their length
+ * or masked are never read into a result; rows beyond their length, and rows that see no key,
+ * are 0 and take no gradient.  start = (valid keys - valid rows) with align_end, else 0; causal:
+ * query i sees keys j <= i + start. */
+typedef struct {
+    int dtype, B, Nq, Nk, H, Hk, D, causal, align_end;
+    float scale;
+    const void *q, *k, *v;
+    void *out; /* read by the backward pass */
+    int64_t qs[3], ks[3], vs[3], os[3];
+    float *lse; /* [B][H][Nq] log2 of the rows' sums: written by fwd (or NULL), read by bwd */
+    const int32_t *q_len, *k_len;
+    const uint8_t *key_mask;
+    int64_t mask_sb;
+    /* bias[num_buckets][H] (or NULL) of bias_dtype.  An offset o = j - i - start has bucket n up to
+     * n < exact, then exact + #{t: n >= thresh[t]}; n = |o|, plus num_buckets / 2 where o > 0, with
+     * `both`, else max(-o, 0).  exact = half of a side's buckets, nthresh = side - exact - 1,
+     * ascending thresholds <= max_distance <= 1024. */
+    const void *bias;
+    int bias_dtype, num_buckets, max_distance, both, nthresh;
+    int32_t thresh[HREG_TOK_MAX_THRESH];
+    /* backward: dout (strides dos); dq [B][Nq][H][D], dk / dv [B][Nk][Hk][D] contiguous; dbias
+     * [num_buckets][H] of bias_dtype; dq, dbias and dk with dv may be NULL: not wanted */
+    const void *dout;
+    int64_t dos[3];
+    void *dq, *dk, *dv, *dbias;
+    void *ws; /* 256-byte aligned, hreg_tok_attn_ws_bytes(p, backward) bytes */
+    size_t ws_bytes;
+} hreg_tok_attn_t;
+
+size_t hreg_tok_attn_ws_bytes(const hreg_tok_attn_t *p, int backward);
+int hreg_tok_attn_fwd(const hreg_tok_attn_t *p, void *stream);
+int hreg_tok_attn_bwd(const hreg_tok_attn_t *p, void *stream);
+
+/* y = x kept ? x / (1 - p) : 0 over n elements, p = step / 65536 (step < 65536).  Element e is kept
+ * where its 16 bits of Philox4x32-10 are >= step: key = the 64-bit seed, counter = (e / 8 low, high,
+ * site, 0), halfword e % 8 of the four output words.  seed_dev: read the seed there (a captured
+ * graph replays with new ones), else `seed`.  The backward pass is the same call on the gradient. */
+int hreg_tok_dropout(const void *x, void *y, int64_t n, int dtype, uint32_t step, uint64_t seed,
+                     const uint64_t *seed_dev, uint32_t site, void *stream);
+
+/* y = x + scale gate dropout(post(f)), h = pre(y) over R rows of C <= 8192 elements, all
+ * contiguous.  post / pre: 0 none, 1 RMS norm, 2 layer norm (statistics and arithmetic in f32, h
+ * from y before its rounding); weights and biases [C] of param_dtype, NULL = 1 / 0.  gate row r /
+ * gate_rows (NULL gate = 1).  f NULL: y = x, not written.  pre 0: no h.  stats [R][4]: mean and
+ * 1 / deviation of post and pre.  Backward: dy, dh (NULL = 0) -> dx, df, dgate, and the parameters'
+ * gradients (each NULL where not wanted); y (x where f is NULL) and stats as the forward pass left
+ * them. */
+typedef struct {
+    int dtype, param_dtype, R, C, gate_rows, post, pre;
+    float scale, eps;
+    uint32_t step, site;
+    uint64_t seed;
+    const uint64_t *seed_dev;
+    const void *x, *f, *gate, *post_w, *post_b, *pre_w, *pre_b;
+    void *y, *h;
+    float *stats;
+    const void *dy, *dh;
+    void *dx, *df, *dgate, *dpost_w, *dpost_b, *dpre_w, *dpre_b;
+    void *ws; /* 256-byte aligned, hreg_tok_block_ws_bytes(p) bytes, backward only */
+    size_t ws_bytes;
+} hreg_tok_block_t;
+
+size_t hreg_tok_block_ws_bytes(const hreg_tok_block_t *p);
+int hreg_tok_block_fwd(const hreg_tok_block_t *p, void *stream);
+int hreg_tok_block_bwd(const hreg_tok_block_t *p, void *stream);
+
 /* library build id (for the loaded-.so audit) */
 const char *hreg_version(void);
 

@@ -54,7 +54,40 @@ class Gemm(ctypes.Structure):
                 ("add", Seg * 2), ("nadd", _i)]
 
 
+_u32 = ctypes.c_uint32
+_u64 = ctypes.c_uint64
+TOK_F32, TOK_BF16 = 0, 1
+TOK_MAX_BUCKETS, TOK_MAX_THRESH, TOK_MAX_DISTANCE = 128, 64, 1024
+
+
+class TokAttn(ctypes.Structure):
+    _fields_ = [("dtype", _i), ("B", _i), ("Nq", _i), ("Nk", _i), ("H", _i), ("Hk", _i), ("D", _i),
+                ("causal", _i), ("align_end", _i), ("scale", ctypes.c_float), ("q", _vp), ("k", _vp),
+                ("v", _vp), ("out", _vp), ("qs", _i64 * 3), ("ks", _i64 * 3), ("vs", _i64 * 3),
+                ("os", _i64 * 3), ("lse", _vp), ("q_len", _vp), ("k_len", _vp), ("key_mask", _vp),
+                ("mask_sb", _i64), ("bias", _vp), ("bias_dtype", _i), ("num_buckets", _i),
+                ("max_distance", _i), ("both", _i), ("nthresh", _i),
+                ("thresh", ctypes.c_int32 * TOK_MAX_THRESH), ("dout", _vp), ("dos", _i64 * 3),
+                ("dq", _vp), ("dk", _vp), ("dv", _vp), ("dbias", _vp), ("ws", _vp),
+                ("ws_bytes", ctypes.c_size_t)]
+
+
+class TokBlock(ctypes.Structure):
+    _fields_ = [("dtype", _i), ("param_dtype", _i), ("R", _i), ("C", _i), ("gate_rows", _i),
+                ("post", _i), ("pre", _i), ("scale", ctypes.c_float), ("eps", ctypes.c_float),
+                ("step", _u32), ("site", _u32), ("seed", _u64), ("seed_dev", _vp), ("x", _vp),
+                ("f", _vp), ("gate", _vp), ("post_w", _vp), ("post_b", _vp), ("pre_w", _vp),
+                ("pre_b", _vp), ("y", _vp), ("h", _vp), ("stats", _vp), ("dy", _vp), ("dh", _vp),
+                ("dx", _vp), ("df", _vp), ("dgate", _vp), ("dpost_w", _vp), ("dpost_b", _vp),
+                ("dpre_w", _vp), ("dpre_b", _vp), ("ws", _vp), ("ws_bytes", ctypes.c_size_t)]
+
+
 _SIGS = {
+    "hreg_tok_attn_fwd": [ctypes.POINTER(TokAttn), _vp],
+    "hreg_tok_attn_bwd": [ctypes.POINTER(TokAttn), _vp],
+    "hreg_tok_dropout": [_vp, _vp, _i64, _i, _u32, _u64, _vp, _u32, _vp],
+    "hreg_tok_block_fwd": [ctypes.POINTER(TokBlock), _vp],
+    "hreg_tok_block_bwd": [ctypes.POINTER(TokBlock), _vp],
     "hreg_furthest_point_sampling": [_i, _i, _i, _vp, _vp, _vp, _vp, _vp],
     "hreg_fps_bounded": [_i, _i, _i, _vp, _vp, _vp, _vp, _i, _vp],
     "hreg_weighted_furthest_point_sampling": [_i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp],
@@ -207,7 +240,8 @@ EXPORTS = tuple(_SIGS) + ("hreg_version", "hreg_spatial_index_bytes", "hreg_col_
                           "hreg_nbr_head_table_floats", "hreg_group6_l2_table_floats",
                           "hreg_group6_l3_table_floats", "hreg_group_l1_6_table_floats",
                           "hreg_group_split6_l2_table_floats", "hreg_group_split6_l3_table_floats",
-                          "hreg_coarse_head6_table_floats", "hreg_icp_ws_bytes")
+                          "hreg_coarse_head6_table_floats", "hreg_icp_ws_bytes",
+                          "hreg_tok_attn_ws_bytes", "hreg_tok_block_ws_bytes")
 
 _lib = None
 _checkers = None
@@ -266,6 +300,10 @@ def load(require_gpu: bool = True):
         L.hreg_icp_ws_bytes.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_int]
         L.hreg_ts_gemm_bn_ws_bytes.restype = ctypes.c_size_t
         L.hreg_ts_gemm_bn_ws_bytes.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_int]
+        L.hreg_tok_attn_ws_bytes.restype = ctypes.c_size_t
+        L.hreg_tok_attn_ws_bytes.argtypes = [ctypes.POINTER(TokAttn), ctypes.c_int]
+        L.hreg_tok_block_ws_bytes.restype = ctypes.c_size_t
+        L.hreg_tok_block_ws_bytes.argtypes = [ctypes.POINTER(TokBlock)]
         for name in ("hreg_nbr_head_table_floats", "hreg_group6_l2_table_floats", "hreg_group6_l3_table_floats",
                      "hreg_group_l1_6_table_floats", "hreg_group_split6_l2_table_floats",
                      "hreg_group_split6_l3_table_floats", "hreg_coarse_head6_table_floats"):

@@ -40,7 +40,7 @@ CFLAGS = [
 # gets it, and tests/test_isa.py fails if any built kernel still mixes the two.  The
 # host-side compile ignores the feature (a warning).
 NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-B6_MARKERS = ("mfma_chain.h", "split_chain.h", "mfma_jt.h", "mfma_f32_32x32x16_bf16")
+B6_MARKERS = ("mfma_chain.h", "split_chain.h", "mfma_jt.h", "mfma_f32_32x32x16_bf16", "tokens.h")
 
 
 def uses_bf16_mfma(path: str) -> bool:

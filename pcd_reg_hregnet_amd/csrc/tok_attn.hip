@@ -1,0 +1,719 @@
+// tok_attn.hip -- attention over token sequences: forward, and the backward pass that
+// recomputes the probabilities from the stored logarithm of their sums; a learned relative
+// position bias by buckets and its gradient are part of both.
+//
+//   s_ij = scale q_i . k_j + bias[bucket(j - i - start)]     (masked: -inf)
+//   p_ij = exp(s_ij - lse_i),  o_i = sum_j p_ij v_j
+//   D_i  = do_i . o_i,  ds_ij = p_ij (do_i . v_j - D_i)
+//   dv_j = sum_i p_ij do_i,  dk_j = scale sum_i ds_ij q_i,  dq_i = scale sum_j ds_ij k_j
+//   dbias[b] = sum of ds_ij over all pairs in bucket b
+//
+// All products run on v_mfma_f32_32x32x16_bf16: bf16 operands as they are, f32 operands as
+// three exact bf16 pieces (six products).  Scores are made transposed (keys x queries) where
+// the next product sums over keys, and straight (queries x keys) where it sums over queries:
+// the result registers are then already the next product's operand.  Scores, sums and
+// accumulators are f32; p and ds are rounded to bf16 for bf16 tensors (off by at most 2^-8 of
+// each, as the tensors themselves are), and cut into three exact pieces for f32 tensors.
+
+#include "tokens.h"
+
+namespace {
+
+using namespace hreg_tok;
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int NT = 256;          // threads a workgroup
+constexpr int ROWS = 128;        // rows a workgroup owns: 32 a wave
+constexpr int MAX_BINS = 2049;   // offsets -max_distance .. max_distance with max_distance <= 1024
+
+struct Buckets {
+    int n, far, both, exact, nthresh;
+    int thresh[HREG_TOK_MAX_THRESH];
+};
+
+struct Args {
+    const void *q, *k, *v, *out_r, *dout;
+    void *out, *dq, *dk, *dv, *dbias;
+    float *lse, *delta, *bins;
+    const int *q_len, *k_len;
+    const uint8_t *key_mask;
+    const void *bias;
+    int64_t qs[3], ks[3], vs[3], os[3], dos[3], mask_sb;
+    int B, Nq, Nk, H, Hk, D, causal, align_end, bias_f32;
+    float scale;
+    Buckets bk;
+};
+
+// the bucket of offset o = key position - query position: one for each offset up to `exact`,
+// then steps of the logarithm, whose first offsets are bk.thresh
+__device__ __forceinline__ int bucket_of(const Buckets &bk, int o) {
+    const int n = bk.both ? (o < 0 ? -o : o) : (o < 0 ? -o : 0);
+    int b = n;
+    if (n >= bk.exact) {
+        b = bk.exact;
+        for (int t = 0; t < bk.nthresh; ++t) b += n >= bk.thresh[t];
+    }
+    return b + (bk.both && o > 0 ? bk.n / 2 : 0);
+}
+
+__device__ __forceinline__ float bias_at(const Args &a, int b, int h) {
+    const size_t at = (size_t)b * a.H + h;
+    return a.bias_f32 ? static_cast<const float *>(a.bias)[at] : (float)static_cast<const __bf16 *>(a.bias)[at];
+}
+
+// this workgroup's batch entry, head and tile: neighbours share keys, and so an L2
+struct Where { int b, h, tile; };
+__device__ __forceinline__ Where where(int heads, int tiles) {
+    const int n = xcd_block(blockIdx.x, gridDim.x);
+    return {n / (tiles * heads), n / tiles % heads, n % tiles};
+}
+
+struct Span { int nq, nk, start; };  // valid rows, valid keys, position of query 0
+__device__ __forceinline__ Span span_of(const Args &a, int b) {
+    Span s;
+    s.nq = a.q_len ? min(max(a.q_len[b], 0), a.Nq) : a.Nq;
+    s.nk = a.k_len ? min(max(a.k_len[b], 0), a.Nk) : a.Nk;
+    s.start = a.align_end ? s.nk - s.nq : 0;
+    return s;
+}
+
+// One [R][DP] tile between global memory, registers and LDS pieces.  Rows at or beyond `valid`,
+// rows whose mask is 0 and columns at or beyond D are zero, whatever memory holds there.
+template <class T, int DP, int R>
+struct Stage {
+    static constexpr int CPR = DP / 8, N = R * CPR / NT, NP = Elem<T>::NP, PLANE = R * DP;
+    static_assert(R * CPR % NT == 0, "tile");
+    Chunk<T> c[N];
+    __device__ __forceinline__ void load(const T *base, int64_t ld, int row0, int valid, int D, const uint8_t *mask) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const int id = threadIdx.x + u * NT, r = row0 + id / CPR, d = id % CPR * 8;
+            if (r < valid && d < D && (!mask || mask[r])) c[u].load(base + (int64_t)r * ld + d);
+            else c[u].zero();
+        }
+    }
+    __device__ __forceinline__ void store(uint16_t *t) const {
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const int id = threadIdx.x + u * NT;
+            bf16x8 p[NP];
+            c[u].pieces(p);
+#pragma unroll
+            for (int s = 0; s < NP; ++s)
+                *reinterpret_cast<u32x4_m *>(t + s * PLANE + tile_at<DP>(id / CPR, id % CPR)) = __builtin_bit_cast(u32x4, p[s]);
+        }
+    }
+};
+
+// one row's pieces as an operand with the row in lane & 31, straight from global memory
+template <class T, int DP>
+__device__ __forceinline__ void load_row(const T *row, bool ok, int D, int lane,
+                                         bf16x8 (&f)[DP / 16][Elem<T>::NP]) {
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+        const int d = 16 * c + 8 * (lane >> 5);
+        Chunk<T> x;
+        if (ok && d < D) x.load(row + d);
+        else x.zero();
+        x.pieces(f[c]);
+    }
+}
+
+// ---------------------------------------------------------------------- forward --
+
+// Scores of 32 keys (rows) against the wave's 32 queries (columns) in units of log2, masked.
+// kpos = key index of row 0 - position of this lane's query, krow = key index of row 0.
+template <bool BIAS>
+__device__ __forceinline__ void finish_scores(const Args &a, f32x16 &s, float scale2, const float *tab, int far,
+                                              int krow, int kpos, int nk, bool edge, const uint8_t *mask, int half) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int kr = 8 * (r >> 2) + 4 * half + (r & 3);
+        float x = s[r] * scale2;
+        if constexpr (BIAS) x += tab[min(max(kpos + kr, -far), far) + far];
+        if (edge) {
+            const bool keep = krow + kr < nk && (!a.causal || kpos + kr <= 0) && (!mask || mask[min(krow + kr, nk - 1)]);
+            x = keep ? x : -INFINITY;
+        }
+        s[r] = x;
+    }
+}
+
+// the bias of one head over all clamped offsets, in units of log2
+__device__ __forceinline__ void fill_table(const Args &a, float *tab, int h) {
+    for (int o = threadIdx.x; o <= 2 * a.bk.far; o += NT) tab[o] = bias_at(a, bucket_of(a.bk, o - a.bk.far), h) * LOG2E;
+}
+
+template <class T, int DP, int KT, bool BIAS>
+__global__ __launch_bounds__(NT) void attn_fwd(Args a) {
+    constexpr int NP = Elem<T>::NP, MT = KT / 32, PLANE = KT * DP;
+    extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
+    uint16_t *kt = lds, *vt = lds + NP * PLANE;
+    float *tab = reinterpret_cast<float *>(lds + 2 * NP * PLANE);
+    const int tiles = (a.Nq + ROWS - 1) / ROWS;
+    const Where w = where(a.H, tiles);
+    const Span sp = span_of(a, w.b);
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
+    const int q0 = (tiles - 1 - w.tile) * ROWS, i = q0 + 32 * wave + (lane & 31);
+    const int hk = w.h / (a.H / a.Hk);
+    const T *K = static_cast<const T *>(a.k) + w.b * a.ks[0] + hk * a.ks[2];
+    const T *V = static_cast<const T *>(a.v) + w.b * a.vs[0] + hk * a.vs[2];
+    const uint8_t *mask = a.key_mask ? a.key_mask + w.b * a.mask_sb : nullptr;
+    if constexpr (BIAS) fill_table(a, tab, w.h);
+
+    bf16x8 qf[DP / 16][NP];
+    load_row<T, DP>(static_cast<const T *>(a.q) + w.b * a.qs[0] + (int64_t)i * a.qs[1] + w.h * a.qs[2], i < sp.nq, a.D,
+                    lane, qf);
+    const float scale2 = a.scale * LOG2E;
+    f32x16 acc[DP / 32];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) acc[d] = zero16();
+    float m = -INFINITY, l = 0.f;
+
+    // keys that some row of the workgroup sees
+    const int last = min(q0 + ROWS, sp.nq) - 1;
+    const int kend = last < q0 ? 0 : a.causal ? min(sp.nk, max(last + sp.start + 1, 0)) : sp.nk;
+    Stage<T, DP, KT> sk, sv;
+    if (kend > 0) {
+        sk.load(K, a.ks[1], 0, sp.nk, a.D, mask);
+        sv.load(V, a.vs[1], 0, sp.nk, a.D, mask);
+    }
+    for (int j0 = 0; j0 < kend; j0 += KT) {
+        __syncthreads();
+        sk.store(kt);
+        sv.store(vt);
+        __syncthreads();
+        if (j0 + KT < kend) {
+            sk.load(K, a.ks[1], j0 + KT, sp.nk, a.D, mask);
+            sv.load(V, a.vs[1], j0 + KT, sp.nk, a.D, mask);
+        }
+        const int qw = q0 + 32 * wave + sp.start;  // position of the wave's first query
+        if (a.causal && j0 > qw + 31) continue;
+        const bool edge = mask || j0 + KT > sp.nk || (a.causal && j0 + KT - 1 > qw);
+        f32x16 s[MT];
+        float top = m;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            s[t] = zero16();
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) {
+                bf16x8 kf[NP];
+                row_frag<DP>(kt, PLANE, 32 * t, c, lane, kf);
+                mma<NP>(s[t], kf, qf[c]);
+            }
+            finish_scores<BIAS>(a, s[t], scale2, tab, a.bk.far, j0 + 32 * t, j0 + 32 * t - (i + sp.start), sp.nk, edge,
+                                mask, half);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
+        }
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float ref = top == -INFINITY ? 0.f : top;  // a row without a key so far keeps sums of 0
+        if (__any(top != m)) {
+            const float shrink = __builtin_amdgcn_exp2f(m - ref);
+            l *= shrink;
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[d][r] *= shrink;
+            m = top;
+        }
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float p[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    p[r] = __builtin_amdgcn_exp2f(s[t][8 * c + r] - ref);
+                    l += p[r];
+                }
+                bf16x8 pf[NP];
+                to_pieces<NP>(p, pf);
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) {
+                    bf16x8 vf[NP];
+                    col_frag<DP>(vt, PLANE, 32 * t + 16 * c, 32 * d, lane, vf);
+                    mma<NP>(acc[d], vf, pf);
+                }
+            }
+        }
+    }
+    l += __shfl_xor(l, 32);
+    const bool any = i < sp.nq && l != 0.f;  // (a NaN sum stays NaN)
+    const float inv = any ? 1.f / l : 0.f;
+    if (i < a.Nq) {
+        T *o = static_cast<T *>(a.out) + w.b * a.os[0] + (int64_t)i * a.os[1] + w.h * a.os[2];
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int col = 32 * d + 2 * r + 4 * half;
+                if (col < a.D)
+                    store4(o + col, any ? acc[d][r] * inv : 0.f, any ? acc[d][r + 1] * inv : 0.f,
+                           any ? acc[d][r + 2] * inv : 0.f, any ? acc[d][r + 3] * inv : 0.f);
+            }
+        // a row without keys: p = exp2(s - inf) = 0 in the backward pass
+        if (a.lse && half == 0)
+            a.lse[((size_t)w.b * a.H + w.h) * a.Nq + i] = any ? m + __builtin_amdgcn_logf(l) : INFINITY;
+    }
+}
+
+// ---------------------------------------------------------------------- backward --
+
+// delta[b][h][i] = do_i . o_i: 16 lanes a row.  Bound by its reads.
+template <class T>
+__global__ __launch_bounds__(NT) void attn_delta(Args a) {
+    const int64_t rows = (int64_t)a.B * a.H * a.Nq, row = (int64_t)blockIdx.x * (NT / 16) + threadIdx.x / 16;
+    if (row >= rows) return;
+    const int i = row % a.Nq, h = row / a.Nq % a.H, b = row / a.Nq / a.H, d = threadIdx.x % 16 * 8;
+    float s = 0.f;
+    if (d < a.D && i < span_of(a, b).nq) {
+        Chunk<T> x, y;
+        x.load(static_cast<const T *>(a.dout) + b * a.dos[0] + (int64_t)i * a.dos[1] + h * a.dos[2] + d);
+        y.load(static_cast<const T *>(a.out_r) + b * a.os[0] + (int64_t)i * a.os[1] + h * a.os[2] + d);
+        s = x.dot(y);
+    }
+    s = row_sum16(s);
+    if (threadIdx.x % 16 == 0) a.delta[row] = s;
+}
+
+// dk, dv of 128 keys: every wave keeps 32 keys and walks all rows of all heads that share them,
+// so the sums over a group need no second pass and have one order.
+template <class T, int DP, int QT, bool BIAS>
+__global__ __launch_bounds__(NT) void attn_bwd_kv(Args a) {
+    constexpr int NP = Elem<T>::NP, PLANE = QT * DP;
+    extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
+    uint16_t *qt = lds, *dt = lds + NP * PLANE;
+    float *lt = reinterpret_cast<float *>(lds + 2 * NP * PLANE), *et = lt + QT, *tab = et + QT;
+    const Where w = where(a.Hk, (a.Nk + ROWS - 1) / ROWS);
+    const Span sp = span_of(a, w.b);
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
+    const int k0 = w.tile * ROWS, j = k0 + 32 * wave + (lane & 31);
+    const uint8_t *mask = a.key_mask ? a.key_mask + w.b * a.mask_sb : nullptr;
+    const bool ok = j < sp.nk && (!mask || mask[j]);
+    bf16x8 kf[DP / 16][NP], vf[DP / 16][NP];
+    load_row<T, DP>(static_cast<const T *>(a.k) + w.b * a.ks[0] + (int64_t)j * a.ks[1] + w.h * a.ks[2], ok, a.D, lane, kf);
+    load_row<T, DP>(static_cast<const T *>(a.v) + w.b * a.vs[0] + (int64_t)j * a.vs[1] + w.h * a.vs[2], ok, a.D, lane, vf);
+    f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) dk[d] = dv[d] = zero16();
+    const float scale2 = a.scale * LOG2E;
+    const int first = a.causal ? max(k0 - sp.start, 0) / QT * QT : 0;  // rows before see no key of the tile
+    const int G = a.H / a.Hk;
+    if (k0 < sp.nk)
+        for (int g = 0; g < G; ++g) {
+            const int h = w.h * G + g;
+            const T *Q = static_cast<const T *>(a.q) + w.b * a.qs[0] + h * a.qs[2];
+            const T *dO = static_cast<const T *>(a.dout) + w.b * a.dos[0] + h * a.dos[2];
+            const float *lse = a.lse + ((size_t)w.b * a.H + h) * a.Nq, *delta = a.delta + ((size_t)w.b * a.H + h) * a.Nq;
+            if constexpr (BIAS) {
+                __syncthreads();
+                fill_table(a, tab, h);
+            }
+            Stage<T, DP, QT> sq, sd;
+            if (first < sp.nq) {
+                sq.load(Q, a.qs[1], first, sp.nq, a.D, nullptr);
+                sd.load(dO, a.dos[1], first, sp.nq, a.D, nullptr);
+            }
+            for (int i0 = first; i0 < sp.nq; i0 += QT) {
+                __syncthreads();
+                sq.store(qt);
+                sd.store(dt);
+                if (threadIdx.x < QT) {
+                    const int i = i0 + threadIdx.x;
+                    lt[threadIdx.x] = i < sp.nq ? lse[i] : INFINITY;
+                    et[threadIdx.x] = i < sp.nq ? delta[i] : 0.f;
+                }
+                __syncthreads();
+                if (i0 + QT < sp.nq) {
+                    sq.load(Q, a.qs[1], i0 + QT, sp.nq, a.D, nullptr);
+                    sd.load(dO, a.dos[1], i0 + QT, sp.nq, a.D, nullptr);
+                }
+#pragma unroll
+                for (int t = 0; t < QT / 32; ++t) {
+                    const int p0 = i0 + 32 * t + sp.start;  // position of the first query
+                    if (a.causal && p0 + 31 < k0 + 32 * wave) continue;
+                    const bool edge = a.causal && p0 < k0 + 32 * wave + 31;
+                    f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+                    for (int c = 0; c < DP / 16; ++c) {
+                        bf16x8 f[NP];
+                        row_frag<DP>(qt, PLANE, 32 * t, c, lane, f);
+                        mma<NP>(s, f, kf[c]);
+                        row_frag<DP>(dt, PLANE, 32 * t, c, lane, f);
+                        mma<NP>(dp, f, vf[c]);
+                    }
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        float p[8], ds[8];
+#pragma unroll
+                        for (int r = 0; r < 8; ++r) {
+                            const int ir = 8 * (2 * c + (r >> 2)) + 4 * half + (r & 3);
+                            float x = s[8 * c + r] * scale2;
+                            const int o = j - (p0 + ir);
+                            if constexpr (BIAS) x += tab[min(max(o, -a.bk.far), a.bk.far) + a.bk.far];
+                            const bool keep = !edge || o <= 0;
+                            p[r] = keep ? __builtin_amdgcn_exp2f(x - lt[32 * t + ir]) : 0.f;
+                            ds[r] = keep ? p[r] * (dp[8 * c + r] - et[32 * t + ir]) : 0.f;
+                        }
+                        bf16x8 pf[NP], sf[NP];
+                        to_pieces<NP>(p, pf);
+                        to_pieces<NP>(ds, sf);
+#pragma unroll
+                        for (int d = 0; d < DP / 32; ++d) {
+                            bf16x8 f[NP];
+                            col_frag<DP>(dt, PLANE, 32 * t + 16 * c, 32 * d, lane, f);
+                            mma<NP>(dv[d], f, pf);
+                            col_frag<DP>(qt, PLANE, 32 * t + 16 * c, 32 * d, lane, f);
+                            mma<NP>(dk[d], f, sf);
+                        }
+                    }
+                }
+            }
+        }
+    if (j < a.Nk) {
+        const int64_t at = (((int64_t)w.b * a.Nk + j) * a.Hk + w.h) * a.D;
+        T *ok_ = static_cast<T *>(a.dk) + at, *ov = static_cast<T *>(a.dv) + at;
+        const float f = a.scale;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int col = 32 * d + 2 * r + 4 * half;
+                if (col >= a.D) continue;
+                store4(ok_ + col, ok ? dk[d][r] * f : 0.f, ok ? dk[d][r + 1] * f : 0.f, ok ? dk[d][r + 2] * f : 0.f,
+                       ok ? dk[d][r + 3] * f : 0.f);
+                store4(ov + col, ok ? dv[d][r] : 0.f, ok ? dv[d][r + 1] : 0.f, ok ? dv[d][r + 2] : 0.f,
+                       ok ? dv[d][r + 3] : 0.f);
+            }
+    }
+}
+
+// The bias gradient of one wave: sums of ds over the diagonals of its 32 x 32 tiles.  Offset
+// o = base - t with t = (query - key) mod 32 (add) or that + 32 (carry): every value moves to
+// lane t of its half, two sums a lane.  The carry of a tile is the add of the next one, so each
+// diagonal goes once to the wave's bins; beyond the far offsets one sum a lane is kept.  No
+// atomics: every sum has one order.
+struct Diagonals {
+    float carry = 0.f, left = 0.f, right = 0.f;
+    int base = 0;
+    __device__ __forceinline__ void flush(float v, int at, float *bins, int far, int lane) {
+        v += __shfl_xor(v, 32);
+        const int o = at - (lane & 31);
+        if (lane < 32) {
+            if (o <= -far) left += v;
+            else if (o >= far) right += v;
+            else bins[o + far] += v;
+        }
+    }
+    // ds of keys base_key .. +31 (rows) and the wave's queries; b = first key - first query position
+    __device__ __forceinline__ void tile(const f32x16 &ds, int b, float *bins, int far, int lane) {
+        const int t = lane & 31, half = lane >> 5;
+        float a = carry;
+        carry = 0.f;
+        if (b - 31 >= far || b + 31 <= -far) {
+            flush(a, b, bins, far, lane);
+            float s = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s += ds[r];
+            if (b < 0) left += s;
+            else right += s;
+        } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int kr = 8 * (r >> 2) + 4 * half + (r & 3);
+                const float x = __shfl(ds[r], ((t + kr) & 31) | (lane & 32));
+                if (t + kr < 32) a += x;
+                else carry += x;
+            }
+            flush(a, b, bins, far, lane);
+        }
+        base = b + 32;
+    }
+    __device__ __forceinline__ void end(float *bins, int far, int lane) {
+        flush(carry, base, bins, far, lane);
+        left = wave_sum_f32(left);
+        right = wave_sum_f32(right);
+        if (lane == 0) {
+            bins[0] += left;
+            bins[2 * far] += right;
+        }
+    }
+};
+
+// dq of 128 rows, and the bias gradient's sums over their diagonals
+template <class T, int DP, int KT, bool BIAS>
+__global__ __launch_bounds__(NT) void attn_bwd_q(Args a) {
+    constexpr int NP = Elem<T>::NP, PLANE = KT * DP;
+    extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
+    uint16_t *kt = lds, *vt = lds + NP * PLANE;
+    const int W = 2 * a.bk.far + 1;
+    float *tab = reinterpret_cast<float *>(lds + 2 * NP * PLANE);
+    const int tiles = (a.Nq + ROWS - 1) / ROWS;
+    const Where w = where(a.H, tiles);
+    const Span sp = span_of(a, w.b);
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
+    const int tile = tiles - 1 - w.tile, q0 = tile * ROWS, i = q0 + 32 * wave + (lane & 31);
+    const int hk = w.h / (a.H / a.Hk);
+    const T *K = static_cast<const T *>(a.k) + w.b * a.ks[0] + hk * a.ks[2];
+    const T *V = static_cast<const T *>(a.v) + w.b * a.vs[0] + hk * a.vs[2];
+    const uint8_t *mask = a.key_mask ? a.key_mask + w.b * a.mask_sb : nullptr;
+    float *bins = tab + W + wave * W;
+    if constexpr (BIAS) {
+        fill_table(a, tab, w.h);
+        for (int o = threadIdx.x; o < 4 * W; o += NT) tab[W + o] = 0.f;
+    }
+    bf16x8 qf[DP / 16][NP], df[DP / 16][NP];
+    load_row<T, DP>(static_cast<const T *>(a.q) + w.b * a.qs[0] + (int64_t)i * a.qs[1] + w.h * a.qs[2], i < sp.nq, a.D,
+                    lane, qf);
+    load_row<T, DP>(static_cast<const T *>(a.dout) + w.b * a.dos[0] + (int64_t)i * a.dos[1] + w.h * a.dos[2], i < sp.nq,
+                    a.D, lane, df);
+    const size_t row = ((size_t)w.b * a.H + w.h) * a.Nq + i;
+    const float lse = i < sp.nq ? a.lse[row] : INFINITY, delta = i < sp.nq ? a.delta[row] : 0.f;
+    const float scale2 = a.scale * LOG2E;
+    f32x16 acc[DP / 32];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) acc[d] = zero16();
+    Diagonals dg;
+    const int last = min(q0 + ROWS, sp.nq) - 1;
+    const int kend = last < q0 ? 0 : a.causal ? min(sp.nk, max(last + sp.start + 1, 0)) : sp.nk;
+    Stage<T, DP, KT> sk, sv;
+    if (kend > 0) {
+        sk.load(K, a.ks[1], 0, sp.nk, a.D, mask);
+        sv.load(V, a.vs[1], 0, sp.nk, a.D, mask);
+    }
+    for (int j0 = 0; j0 < kend; j0 += KT) {
+        __syncthreads();
+        sk.store(kt);
+        sv.store(vt);
+        __syncthreads();
+        if (j0 + KT < kend) {
+            sk.load(K, a.ks[1], j0 + KT, sp.nk, a.D, mask);
+            sv.load(V, a.vs[1], j0 + KT, sp.nk, a.D, mask);
+        }
+        const int qw = q0 + 32 * wave + sp.start;
+#pragma unroll
+        for (int t = 0; t < KT / 32; ++t) {
+            const int j = j0 + 32 * t;
+            if (j >= kend || (a.causal && j > qw + 31)) continue;
+            const bool edge = mask || j + 32 > sp.nk || (a.causal && j + 31 > qw);
+            f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) {
+                bf16x8 f[NP];
+                row_frag<DP>(kt, PLANE, 32 * t, c, lane, f);
+                mma<NP>(s, f, qf[c]);
+                row_frag<DP>(vt, PLANE, 32 * t, c, lane, f);
+                mma<NP>(dp, f, df[c]);
+            }
+            finish_scores<BIAS>(a, s, scale2, tab, a.bk.far, j, j - (i + sp.start), sp.nk, edge, mask, half);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float p = __builtin_amdgcn_exp2f(s[r] - lse);
+                s[r] = s[r] == -INFINITY ? 0.f : p * (dp[r] - delta);
+            }
+            if (BIAS && a.dbias) dg.tile(s, j - qw, bins, a.bk.far, lane);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float x[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) x[r] = s[8 * c + r];
+                bf16x8 sf[NP];
+                to_pieces<NP>(x, sf);
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) {
+                    bf16x8 f[NP];
+                    col_frag<DP>(kt, PLANE, 32 * t + 16 * c, 32 * d, lane, f);
+                    mma<NP>(acc[d], f, sf);
+                }
+            }
+        }
+    }
+    if (i < a.Nq && a.dq) {
+        T *o = static_cast<T *>(a.dq) + (((int64_t)w.b * a.Nq + i) * a.H + w.h) * a.D;
+        const float f = a.scale;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int col = 32 * d + 2 * r + 4 * half;
+                if (col < a.D) store4(o + col, acc[d][r] * f, acc[d][r + 1] * f, acc[d][r + 2] * f, acc[d][r + 3] * f);
+            }
+    }
+    if (BIAS && a.dbias) {
+        if (kend == 0) __syncthreads();  // the bins were cleared by other waves
+        dg.end(bins, a.bk.far, lane);
+        __syncthreads();
+        float *to = a.bins + (((size_t)w.b * a.H + w.h) * tiles + tile) * W;
+        for (int o = threadIdx.x; o < W; o += NT)
+            to[o] = ((tab[W + o] + tab[2 * W + o]) + tab[3 * W + o]) + tab[4 * W + o];
+    }
+}
+
+// dbias[bucket][h] from the workgroups' diagonal sums: per offset over batch and tiles, then per
+// bucket over its offsets, in 64 bits and in one order
+template <class T>
+__global__ __launch_bounds__(NT) void bias_reduce(Args a) {
+    __shared__ double sum[MAX_BINS];
+    const int h = blockIdx.x, W = 2 * a.bk.far + 1, tiles = (a.Nq + ROWS - 1) / ROWS;
+    for (int o = threadIdx.x; o < W; o += NT) {
+        double s = 0.;
+        for (int b = 0; b < a.B; ++b)
+            for (int t = 0; t < tiles; ++t) s += a.bins[(((size_t)b * a.H + h) * tiles + t) * W + o];
+        sum[o] = s;
+    }
+    __syncthreads();
+    for (int n = threadIdx.x; n < a.bk.n; n += NT) {
+        double s = 0.;
+        for (int o = 0; o < W; ++o)
+            if (bucket_of(a.bk, o - a.bk.far) == n) s += sum[o];
+        static_cast<T *>(a.dbias)[(size_t)n * a.H + h] = (T)(float)s;
+    }
+}
+
+// ------------------------------------------------------------------- C interface --
+
+int row_tiles(int n) { return (n + ROWS - 1) / ROWS; }
+
+bool vec_ok(const void *p, const int64_t s[3], int esize) {
+    const int64_t n = 16 / esize;
+    return p && reinterpret_cast<uintptr_t>(p) % 16 == 0 && s[0] % n == 0 && s[1] % n == 0 && s[2] % n == 0;
+}
+
+// the argument checks shared by both directions; fills the kernels' arguments
+int take(const hreg_tok_attn_t *p, Args &a) {
+    if (!p || (p->dtype != HREG_TOK_F32 && p->dtype != HREG_TOK_BF16)) return HREG_ERR_INVALID;
+    if (p->B < 0 || p->Nq < 0 || p->Nk < 0 || p->H < 1 || p->Hk < 1 || p->H % p->Hk) return HREG_ERR_INVALID;
+    if (p->D < 8 || p->D > 128 || p->D % 8) return HREG_ERR_UNSUPPORTED;
+    if ((int64_t)p->B * p->H * (row_tiles(p->Nq) + 1) > INT32_MAX || (int64_t)p->B * p->H * (row_tiles(p->Nk) + 1) > INT32_MAX ||
+        p->Nq > (1 << 30) || p->Nk > (1 << 30))
+        return HREG_ERR_UNSUPPORTED;
+    const int es = p->dtype == HREG_TOK_F32 ? 4 : 2;
+    const bool empty = p->B == 0 || p->Nq == 0;
+    if (!empty && (!vec_ok(p->q, p->qs, es) || !vec_ok(p->out, p->os, es))) return HREG_ERR_INVALID;
+    if (p->B > 0 && p->Nk > 0 && (!vec_ok(p->k, p->ks, es) || !vec_ok(p->v, p->vs, es))) return HREG_ERR_INVALID;
+    a = Args{};
+    a.q = p->q; a.k = p->k; a.v = p->v; a.out = p->out; a.out_r = p->out; a.dout = p->dout;
+    a.dq = p->dq; a.dk = p->dk; a.dv = p->dv; a.dbias = p->dbias;
+    a.lse = p->lse; a.q_len = p->q_len; a.k_len = p->k_len; a.key_mask = p->key_mask; a.bias = p->bias;
+    for (int i = 0; i < 3; ++i) {
+        a.qs[i] = p->qs[i]; a.ks[i] = p->ks[i]; a.vs[i] = p->vs[i]; a.os[i] = p->os[i]; a.dos[i] = p->dos[i];
+    }
+    a.mask_sb = p->mask_sb;
+    a.B = p->B; a.Nq = p->Nq; a.Nk = p->Nk; a.H = p->H; a.Hk = p->Hk; a.D = p->D;
+    a.causal = p->causal != 0; a.align_end = p->align_end != 0; a.scale = p->scale;
+    if (p->bias) {
+        if (p->bias_dtype != HREG_TOK_F32 && p->bias_dtype != HREG_TOK_BF16) return HREG_ERR_INVALID;
+        const int side = p->both ? p->num_buckets / 2 : p->num_buckets, exact = side / 2;
+        if (p->num_buckets < 2 || (p->both && (p->num_buckets % 2 || side < 2)) || p->max_distance <= exact)
+            return HREG_ERR_INVALID;
+        if (p->num_buckets > HREG_TOK_MAX_BUCKETS || p->max_distance > (MAX_BINS - 1) / 2) return HREG_ERR_UNSUPPORTED;
+        if (p->nthresh != side - exact - 1 || p->nthresh > HREG_TOK_MAX_THRESH) return HREG_ERR_INVALID;
+        a.bias_f32 = p->bias_dtype == HREG_TOK_F32;
+        a.bk.n = p->num_buckets; a.bk.far = p->max_distance; a.bk.both = p->both != 0; a.bk.exact = exact;
+        a.bk.nthresh = p->nthresh;
+        for (int t = 0; t < p->nthresh; ++t) a.bk.thresh[t] = p->thresh[t];
+    }
+    return HREG_OK;
+}
+
+// launches F<T, DP, tile, BIAS> with its dynamic LDS (above the 64 KB default where needed)
+template <class K>
+int launch(K *kernel, int grid, size_t lds, void *stream, const Args &a) {
+    if (lds > 65536 &&
+        hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
+        return HREG_ERR_LAUNCH;
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(NT), lds, as_stream(stream), a);
+    HREG_CHECK_LAUNCH();
+    return HREG_OK;
+}
+
+template <class T, int DP, bool BIAS>
+int fwd(const Args &a, void *stream) {
+    constexpr int KT = sizeof(T) == 2 || DP == 32 ? 64 : 32;
+    const size_t lds = (size_t)2 * Elem<T>::NP * KT * DP * 2 + (BIAS ? (2 * a.bk.far + 1) * 4 : 0);
+    return launch(attn_fwd<T, DP, KT, BIAS>, a.B * a.H * row_tiles(a.Nq), lds, stream, a);
+}
+
+template <class T, int DP, bool BIAS>
+int bwd(const Args &a, void *stream) {
+    constexpr int NP = Elem<T>::NP, QT = sizeof(T) == 2 || DP == 32 ? 64 : 32;
+    const size_t W = BIAS ? 2 * a.bk.far + 1 : 0, tile = (size_t)2 * NP * QT * DP * 2;
+    int rc = HREG_OK;
+    if (a.Nq > 0) {
+        const int64_t rows = (int64_t)a.B * a.H * a.Nq;
+        hipLaunchKernelGGL(attn_delta<T>, dim3((rows + NT / 16 - 1) / (NT / 16)), dim3(NT), 0, as_stream(stream), a);
+        HREG_CHECK_LAUNCH();
+    }
+    if (a.Nk > 0 && a.dk) rc = launch(attn_bwd_kv<T, DP, QT, BIAS>, a.B * a.Hk * row_tiles(a.Nk), tile + (2 * QT + W) * 4, stream, a);
+    if (rc == HREG_OK && a.Nq > 0 && (a.dq || a.dbias))
+        rc = launch(attn_bwd_q<T, DP, QT, BIAS>, a.B * a.H * row_tiles(a.Nq), tile + 5 * W * 4, stream, a);
+    return rc;
+}
+
+template <class T, bool BIAS, bool BACK>
+int by_width(const Args &a, void *stream) {
+    if constexpr (BACK) {
+        if (a.D <= 32) return bwd<T, 32, BIAS>(a, stream);
+        if (a.D <= 64) return bwd<T, 64, BIAS>(a, stream);
+        return bwd<T, 128, BIAS>(a, stream);
+    } else {
+        if (a.D <= 32) return fwd<T, 32, BIAS>(a, stream);
+        if (a.D <= 64) return fwd<T, 64, BIAS>(a, stream);
+        return fwd<T, 128, BIAS>(a, stream);
+    }
+}
+
+template <bool BACK>
+int by_type(const hreg_tok_attn_t *p, const Args &a, void *stream) {
+    if (p->dtype == HREG_TOK_F32)
+        return a.bias ? by_width<float, true, BACK>(a, stream) : by_width<float, false, BACK>(a, stream);
+    return a.bias ? by_width<__bf16, true, BACK>(a, stream) : by_width<__bf16, false, BACK>(a, stream);
+}
+
+size_t delta_bytes(const hreg_tok_attn_t *p) { return ((size_t)p->B * p->H * p->Nq * 4 + 255) / 256 * 256; }
+
+}  // namespace
+
+extern "C" {
+
+size_t hreg_tok_attn_ws_bytes(const hreg_tok_attn_t *p, int backward) {
+    if (!p || p->B < 0 || p->Nq < 0 || p->H < 1 || !backward) return 0;
+    return delta_bytes(p) + (p->bias ? (size_t)p->B * p->H * row_tiles(p->Nq) * (2 * (size_t)p->max_distance + 1) * 4 : 0);
+}
+
+int hreg_tok_attn_fwd(const hreg_tok_attn_t *p, void *stream) {
+    Args a;
+    const int rc = take(p, a);
+    if (rc != HREG_OK) return rc;
+    if (p->ws_bytes < hreg_tok_attn_ws_bytes(p, 0)) return HREG_ERR_INVALID;
+    if (a.B == 0 || a.Nq == 0) return HREG_OK;
+    return by_type<false>(p, a, stream);
+}
+
+int hreg_tok_attn_bwd(const hreg_tok_attn_t *p, void *stream) {
+    Args a;
+    const int rc = take(p, a);
+    if (rc != HREG_OK) return rc;
+    if (!a.bias) a.dbias = nullptr;
+    if (a.B > 0 && a.Nq > 0 && (!vec_ok(p->dout, p->dos, p->dtype == HREG_TOK_F32 ? 4 : 2) || !p->lse)) return HREG_ERR_INVALID;
+    for (const void *g : {p->dq, p->dk, p->dv})
+        if (reinterpret_cast<uintptr_t>(g) % 16) return HREG_ERR_INVALID;
+    if (!p->dk != !p->dv) return HREG_ERR_INVALID;
+    const size_t need = hreg_tok_attn_ws_bytes(p, 1);
+    if (p->ws_bytes < need || (need && (!p->ws || reinterpret_cast<uintptr_t>(p->ws) % 256))) return HREG_ERR_INVALID;
+    a.delta = static_cast<float *>(p->ws);
+    a.bins = reinterpret_cast<float *>(static_cast<char *>(p->ws) + delta_bytes(p));
+    if (a.B > 0) {
+        const int rc2 = by_type<true>(p, a, stream);
+        if (rc2 != HREG_OK) return rc2;
+    }
+    if (a.dbias) {  // an empty batch too: the gradient is zero
+        if (a.bias_f32) hipLaunchKernelGGL(bias_reduce<float>, dim3(a.H), dim3(NT), 0, as_stream(stream), a);
+        else hipLaunchKernelGGL(bias_reduce<__bf16>, dim3(a.H), dim3(NT), 0, as_stream(stream), a);
+        HREG_CHECK_LAUNCH();
+    }
+    return HREG_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,458 @@
+"""Operators over token sequences on the HIP library: what a model needs to let its keypoint
+descriptors attend to each other, in training and when it answers one token at a time.
+
+* ``attention``: softmax(scale q k^T + bias) v with grouped key heads, lengths, a key mask and
+  causal order; its backward pass recomputes the probabilities (nothing of size Nq x Nk is
+  stored).  ``Buckets`` and a learned table give it a relative position bias by buckets, with
+  the table's gradient.  One call serves training and single tokens.
+* ``dropout``: from a counter-based generator, the mask made again where it is needed.
+* ``gated_residual_norm``: the norm behind one block, dropout, gate and scaled residual, and the
+  norm before the next block in one pass, forward and backward.
+
+They stand beside ``train_graph``'s operators: autograd functions whose arithmetic is one or a
+few C-ABI launches (csrc/tok_attn.hip, csrc/tok_elem.hip) on the current stream of the tensors'
+device; no CPU fallback.  Row data is float32 or bfloat16.  Float32 products keep float32
+accuracy (three exact bf16 pieces a value); sums, statistics and accumulators are float32.
+Results do not depend on the order in which workgroups run.  A call can be captured in a HIP
+graph: nothing is read on the host, and a seed tensor is read when the graph replays.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+import functools
+import math
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.float32: _lib.TOK_F32, torch.bfloat16: _lib.TOK_BF16}
+_NORMS = {None: 0, "rms": 1, "layer": 2}
+
+
+def _check(cond: bool, text: str) -> None:
+    if not cond:
+        raise ValueError(text)
+
+
+def _check_tensor(fn: str, name: str, t, device=None, dtype=None) -> None:
+    _check(isinstance(t, torch.Tensor) and t.is_cuda, f"{fn}: {name} must be a GPU tensor (no CPU fallback)")
+    _check(device is None or t.device == device, f"{fn}: {name} is on {t.device}, expected {device}")
+    _check(dtype is None or t.dtype == dtype, f"{fn}: {name} has type {t.dtype}, expected {dtype}")
+
+
+@contextlib.contextmanager
+def _on(device):
+    """the tensors' device is current inside; yields its current stream"""
+    if device.index == torch.cuda.current_device():
+        yield _lib.stream_handle()
+    else:
+        with torch.cuda.device(device):
+            yield _lib.stream_handle()
+
+
+def _launch(name: str, args, stream) -> None:
+    _lib.call(name, ctypes.byref(args), stream)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+# --------------------------------------------------------------------- relative positions
+
+@functools.lru_cache(maxsize=None)
+def _thresholds(exact: int, side: int, far: int) -> tuple:
+    """First offsets of the logarithmic buckets: the least n with (n / exact)^L >= (far /
+    exact)^t for t = 1 .. L - 1, L = side - exact, in whole numbers (a float logarithm would
+    decide borders by its rounding)."""
+    L = side - exact
+    out = []
+    for t in range(1, L):
+        n = max(exact, int(exact * (far / exact) ** (t / L)) - 1)
+        while n ** L * exact ** t < far ** t * exact ** L:
+            n += 1
+        while n > exact and (n - 1) ** L * exact ** t >= far ** t * exact ** L:
+            n -= 1
+        out.append(n)
+    return tuple(out)
+
+
+@dataclass(frozen=True)
+class Buckets:
+    """Buckets of the offset o = key position - query position.
+
+    ``bidirectional``: half of the buckets for o <= 0, half for o > 0; otherwise all of them for
+    o <= 0, and every o > 0 is in bucket 0.  On a side with S buckets distances below S // 2 have
+    one each; the others are equal steps of the logarithm up to ``max_distance``, the last one
+    for everything from there on.  A plain value: a program makes it once or for each call."""
+    num_buckets: int = 32
+    max_distance: int = 128
+    bidirectional: bool = True
+
+    def __post_init__(self):
+        n, far = self.num_buckets, self.max_distance
+        _check(isinstance(n, int) and isinstance(far, int), "Buckets: num_buckets and max_distance must be int")
+        _check(2 <= n <= _lib.TOK_MAX_BUCKETS, f"Buckets: num_buckets {n} not in 2 .. {_lib.TOK_MAX_BUCKETS}")
+        _check(not self.bidirectional or (n % 2 == 0 and n >= 4),
+               f"Buckets: num_buckets {n} must be even and at least 4 for both directions")
+        _check(self._side // 2 < far <= _lib.TOK_MAX_DISTANCE,
+               f"Buckets: max_distance {far} not in {self._side // 2 + 1} .. {_lib.TOK_MAX_DISTANCE}")
+
+    @property
+    def _side(self) -> int:
+        return self.num_buckets // 2 if self.bidirectional else self.num_buckets
+
+    @property
+    def thresholds(self) -> tuple:
+        """first distances of the logarithmic buckets after the first"""
+        return _thresholds(self._side // 2, self._side, self.max_distance)
+
+    def index(self, offset: int) -> int:
+        """the bucket of one offset"""
+        n = abs(offset) if self.bidirectional else max(-offset, 0)
+        exact = self._side // 2
+        b = n if n < exact else exact + sum(n >= t for t in self.thresholds)
+        return b + (self._side if self.bidirectional and offset > 0 else 0)
+
+
+# ------------------------------------------------------------------------------ attention
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy of it whose rows the kernels can read: contiguous rows in 16-byte steps"""
+    n = 16 // t.element_size()
+    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
+        s % n == 0 for s, m in zip(t.stride()[:-1], t.shape[:-1]) if m > 1)
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _strides(t: torch.Tensor):
+    """(batch, token, head) strides; a dimension of one element is never stepped over"""
+    return (ctypes.c_int64 * 3)(*(s if m > 1 else 0 for s, m in zip(t.stride()[:3], t.shape[:3])))
+
+
+@dataclass(frozen=True)
+class _AttnOptions:
+    scale: float
+    causal: bool
+    align_end: bool
+    buckets: Buckets | None
+
+
+def _attn_args(o: _AttnOptions, q, k, v, out, lse, q_len, k_len, key_mask, bias) -> _lib.TokAttn:
+    p = _lib.TokAttn()
+    p.dtype = _DTYPES[q.dtype]
+    p.B, p.Nq, p.H, p.D = q.shape
+    p.Nk, p.Hk = k.shape[1], k.shape[2]
+    p.causal, p.align_end, p.scale = int(o.causal), int(o.align_end), o.scale
+    p.q, p.k, p.v, p.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    p.qs, p.ks, p.vs, p.os = _strides(q), _strides(k), _strides(v), _strides(out)
+    p.lse, p.q_len, p.k_len, p.key_mask = _ptr(lse), _ptr(q_len), _ptr(k_len), _ptr(key_mask)
+    p.mask_sb = 0 if key_mask is None or key_mask.shape[0] == 1 else key_mask.stride(0)
+    if bias is not None:
+        b = o.buckets
+        p.bias, p.bias_dtype = bias.data_ptr(), _DTYPES[bias.dtype]
+        p.num_buckets, p.max_distance, p.both = b.num_buckets, b.max_distance, int(b.bidirectional)
+        p.nthresh = len(b.thresholds)
+        p.thresh[:p.nthresh] = b.thresholds
+    return p
+
+
+def _attn_ws(p: _lib.TokAttn, backward: int, device):
+    n = _lib.load().hreg_tok_attn_ws_bytes(ctypes.byref(p), backward)
+    ws = torch.empty(max(n, 16), dtype=torch.uint8, device=device)
+    p.ws, p.ws_bytes = ws.data_ptr(), n
+    return ws
+
+
+def _attn_forward(o, q, k, v, bias, q_len, k_len, key_mask, want_lse: bool):
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    B, Nq, H, _ = q.shape
+    lse = torch.empty(B, H, Nq, device=q.device) if want_lse else None
+    with _on(q.device) as stream:
+        p = _attn_args(o, q, k, v, out, lse, q_len, k_len, key_mask, bias)
+        ws = _attn_ws(p, 0, q.device)  # noqa: F841 (held until the launch is queued)
+        _launch("hreg_tok_attn_fwd", p, stream)
+    return q, k, v, out, lse
+
+
+class _TokAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, bias, o, q_len, k_len, key_mask):
+        q, k, v, out, lse = _attn_forward(o, q, k, v, bias, q_len, k_len, key_mask, True)
+        ctx.save_for_backward(q, k, v, bias, out, lse, q_len, k_len, key_mask)
+        ctx.o = o
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, bias, out, lse, q_len, k_len, key_mask = ctx.saved_tensors
+        need_q, need_k, need_v, need_b = ctx.needs_input_grad[:4]
+        dout = _rows(dout)
+        dev = q.device
+        dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if need_q else None
+        dk = torch.empty(k.shape, dtype=k.dtype, device=dev) if need_k or need_v else None
+        dv = torch.empty(v.shape, dtype=v.dtype, device=dev) if need_k or need_v else None
+        db = torch.empty(bias.shape, dtype=bias.dtype, device=dev) if need_b else None
+        with _on(dev) as stream:
+            p = _attn_args(ctx.o, q, k, v, out, lse, q_len, k_len, key_mask, bias)
+            p.dout, p.dos = dout.data_ptr(), _strides(dout)
+            p.dq, p.dk, p.dv, p.dbias = _ptr(dq), _ptr(dk), _ptr(dv), _ptr(db)
+            ws = _attn_ws(p, 1, dev)  # noqa: F841
+            _launch("hreg_tok_attn_bwd", p, stream)
+        return dq, dk if need_k else None, dv if need_v else None, db, None, None, None, None
+
+
+def _lengths(name: str, t, B: int, device):
+    if t is None:
+        return None
+    _check_tensor("attention", name, t, device)
+    _check(t.dtype in (torch.int32, torch.int64) and tuple(t.shape) == (B,),
+           f"attention: {name} must be int32 or int64 of shape ({B},), got {t.dtype} {tuple(t.shape)}")
+    if t.dtype == torch.int64:
+        t = t.clamp(0, 2 ** 31 - 1).to(torch.int32)
+    return t.contiguous()
+
+
+def attention(q, k, v, *, scale=None, causal=False, align_end=None, q_lengths=None, k_lengths=None,
+              key_mask=None, bias=None, buckets=None):
+    """softmax_j(scale q_i . k_j + bias[bucket, h]) v_j -> [B, Nq, H, D].
+
+    q [B, Nq, H, D]; k, v [B, Nk, Hk, D] with H a multiple of Hk (each key head serves H // Hk
+    consecutive query heads); float32 or bfloat16, D a multiple of 8 up to 128.  Any strides:
+    rows that are not contiguous 16-byte aligned steps are copied first.  scale: D ** -0.5 by
+    default.  Differentiable (once) in q, k, v and bias.
+
+    k_lengths, q_lengths [B] int32 / int64 on the GPU (clamped to the tensors): keys and queries
+    from there on do not exist.  key_mask [B or 1, Nk] bool: False keys are not seen.  Their
+    values, NaN among them, have no influence.  Queries that do not exist or see no key give 0
+    and take no gradient.  A key that is not finite and that any query sees may reach every query
+    of its batch entry.
+
+    Positions: key j stands at j; query i at i, or with align_end (the default where causal) at
+    i + keys - queries, so that the last query stands at the last key.  causal: a query sees keys
+    up to its own position.
+
+    bias [num_buckets, H] (float32 or q's type) and ``Buckets`` add a learned bias by the offset of
+    key and query.  With bfloat16 rows its gradient has their accuracy (about 2^-8 of it)."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _check_tensor("attention", name, t, None if name == "q" else q.device, None if name == "q" else q.dtype)
+        _check(t.dim() == 4, f"attention: {name} must be [batch, tokens, heads, width], got {tuple(t.shape)}")
+    _check(q.dtype in _DTYPES, f"attention: type {q.dtype} not supported (float32, bfloat16)")
+    B, Nq, H, D = q.shape
+    Nk, Hk = k.shape[1], k.shape[2]
+    _check(tuple(k.shape) == (B, Nk, Hk, D) and k.shape == v.shape,
+           f"attention: k {tuple(k.shape)} and v {tuple(v.shape)} do not fit q {tuple(q.shape)}")
+    _check(H >= 1 and Hk >= 1 and H % Hk == 0, f"attention: {H} heads are not a multiple of {Hk} key heads")
+    _check(8 <= D <= 128 and D % 8 == 0, f"attention: width {D} is not a multiple of 8 up to 128")
+    scale = D ** -0.5 if scale is None else float(scale)
+    _check(math.isfinite(scale), f"attention: scale {scale} is not finite")
+    q_len, k_len = _lengths("q_lengths", q_lengths, B, q.device), _lengths("k_lengths", k_lengths, B, q.device)
+    if key_mask is not None:
+        _check_tensor("attention", "key_mask", key_mask, q.device, torch.bool)
+        _check(key_mask.dim() == 2 and key_mask.shape[0] in (1, B) and key_mask.shape[1] == Nk,
+               f"attention: key_mask must be [{B} or 1, {Nk}], got {tuple(key_mask.shape)}")
+        key_mask = key_mask if key_mask.stride(1) == 1 else key_mask.contiguous()
+    _check((bias is None) == (buckets is None), "attention: bias and buckets come together")
+    if bias is not None:
+        _check(isinstance(buckets, Buckets), "attention: buckets must be a Buckets")
+        _check_tensor("attention", "bias", bias, q.device)
+        _check(bias.dtype in (torch.float32, q.dtype), f"attention: bias has type {bias.dtype}, expected float32 or {q.dtype}")
+        _check(tuple(bias.shape) == (buckets.num_buckets, H),
+               f"attention: bias must be [{buckets.num_buckets}, {H}], got {tuple(bias.shape)}")
+        bias = bias.contiguous()
+    o = _AttnOptions(scale, bool(causal), bool(causal if align_end is None else align_end), buckets)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias)):
+        return _TokAttention.apply(q, k, v, bias, o, q_len, k_len, key_mask)
+    return _attn_forward(o, q, k, v, bias, q_len, k_len, key_mask, False)[3]
+
+
+# -------------------------------------------------------------------------------- dropout
+
+def _draws(fn: str, p, seed, site, device):
+    """(step, seed value, seed tensor): p counts in steps of 2^-16"""
+    p = float(p)
+    _check(0.0 <= p < 1.0, f"{fn}: p {p} not in [0, 1)")
+    step = min(int(p * 65536 + 0.5), 65535)
+    _check(isinstance(site, int) and 0 <= site < 2 ** 32, f"{fn}: site must be an int of 32 bits")
+    if isinstance(seed, torch.Tensor):
+        _check_tensor(fn, "seed", seed, device, torch.int64)
+        _check(seed.numel() == 1, f"{fn}: seed must hold one value, got {tuple(seed.shape)}")
+        return step, 0, seed
+    _check(step == 0 or (isinstance(seed, int) and not isinstance(seed, bool)),
+           f"{fn}: p > 0 needs a seed (int or int64 GPU tensor)")
+    return step, (seed or 0) & (2 ** 64 - 1), None
+
+
+def _dropout(x, step, value, seed, site):
+    x = x.contiguous()
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    with _on(x.device) as stream:
+        _lib.call("hreg_tok_dropout", x, y, x.numel(), _DTYPES[x.dtype], step, value, _ptr(seed), site, stream)
+    return y
+
+
+class _TokDropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, step, value, seed, site):
+        ctx.save_for_backward(seed)
+        ctx.draws = step, value, site
+        return _dropout(x, step, value, seed, site)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        step, value, site = ctx.draws
+        return _dropout(dy, step, value, ctx.saved_tensors[0], site), None, None, None, None
+
+
+def dropout(x, p, seed, *, site=0, training=True):
+    """x with each element kept with probability 1 - p and divided by it, else 0.
+
+    p is taken in steps of 2^-16, and the kept values are scaled by that step, so the expectation
+    is x.  The choice depends on (seed, site, element number in x's logical order) alone:
+    Philox4x32-10, so the backward pass, or another call, makes the same mask.  seed: an int, or an
+    int64 GPU tensor of one value that is read on the device (it must keep its value until the
+    backward pass).  site (32 bits) tells the places of one model apart that share a seed.
+    float32 or bfloat16, any shape; training False returns x."""
+    _check_tensor("dropout", "x", x)
+    _check(x.dtype in _DTYPES, f"dropout: type {x.dtype} not supported (float32, bfloat16)")
+    step, value, seed = _draws("dropout", p, seed, site, x.device)
+    if not training or step == 0:
+        return x
+    return _TokDropout.apply(x, step, value, seed, site)
+
+
+# ------------------------------------------------------------------ residual, gate and norms
+
+@dataclass(frozen=True)
+class _BlockOptions:
+    scale: float
+    eps: float
+    post: int
+    pre: int
+    step: int
+    value: int
+    site: int
+    gate_rows: int
+
+
+def _block_args(o: _BlockOptions, like, param_dtype, seed, **tensors) -> _lib.TokBlock:
+    p = _lib.TokBlock()
+    C = like.shape[-1]
+    p.dtype, p.param_dtype = _DTYPES[like.dtype], _DTYPES[param_dtype]
+    p.R, p.C, p.gate_rows = like.numel() // C, C, o.gate_rows
+    p.post, p.pre, p.scale, p.eps = o.post, o.pre, o.scale, o.eps
+    p.step, p.site, p.seed, p.seed_dev = o.step, o.site, o.value, _ptr(seed)
+    for name, t in tensors.items():
+        setattr(p, name, _ptr(t))
+    return p
+
+
+class _GatedResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, f, gate, post_w, post_b, pre_w, pre_b, o, seed, param_dtype):
+        dev = x.device
+        y = torch.empty_like(x) if f is not None else None
+        h = torch.empty_like(x) if o.pre else None
+        stats = torch.empty(x.numel() // x.shape[-1], 4, device=dev)
+        with _on(dev) as stream:
+            p = _block_args(o, x, param_dtype, seed, x=x, f=f, gate=gate, post_w=post_w, post_b=post_b, pre_w=pre_w,
+                            pre_b=pre_b, y=y, h=h, stats=stats)
+            _launch("hreg_tok_block_fwd", p, stream)
+        ctx.save_for_backward(f, gate, post_w, post_b, pre_w, pre_b, stats, seed, x if y is None else y)
+        ctx.o, ctx.param_dtype = o, param_dtype
+        ctx.set_materialize_grads(False)
+        return y, h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh):
+        f, gate, post_w, post_b, pre_w, pre_b, stats, seed, y = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        like = [y, f, gate, post_w, post_b, pre_w, pre_b]
+        if dy is None and dh is None:
+            return (None,) * 10
+        make = torch.empty_like if y.numel() else torch.zeros_like  # (no rows: the sums are zero)
+        grads = [make(t) if n and t is not None else None for t, n in zip(like, need)]
+        dy, dh = (None if g is None else g.contiguous() for g in (dy, dh))
+        dev = y.device
+        with _on(dev) as stream:
+            p = _block_args(ctx.o, y, ctx.param_dtype, seed, y=y, f=f, gate=gate, post_w=post_w, post_b=post_b,
+                            pre_w=pre_w, pre_b=pre_b, stats=stats, dy=dy, dh=dh,
+                            **dict(zip(("dx", "df", "dgate", "dpost_w", "dpost_b", "dpre_w", "dpre_b"), grads)))
+            n = _lib.load().hreg_tok_block_ws_bytes(ctypes.byref(p))
+            ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
+            p.ws, p.ws_bytes = ws.data_ptr(), n
+            _launch("hreg_tok_block_bwd", p, stream)
+        return (*grads, None, None, None)
+
+
+def _gate_of(gate, x):
+    """(gate rows [n, C], rows of x a gate row serves): a gate that is constant over trailing token
+    dimensions is read in place; any other broadcast is written out"""
+    shape = (1,) * (x.dim() - gate.dim()) + tuple(gate.shape)
+    lead = 0
+    while lead < x.dim() - 1 and shape[lead] == x.shape[lead]:
+        lead += 1
+    if shape[-1] != x.shape[-1] or any(n != 1 for n in shape[lead:-1]):
+        return gate.expand(x.shape).contiguous(), 1
+    return gate.contiguous(), max(math.prod(x.shape[lead:-1]), 1)
+
+
+def gated_residual_norm(x, f, *, gate=None, scale=1.0, post_norm=None, post_weight=None, post_bias=None,
+                        pre_norm="rms", pre_weight=None, pre_bias=None, eps=1e-6, p=0.0, seed=None, site=0):
+    """y = x + scale * gate * dropout(post_norm(f)), h = pre_norm(y) -> (y, h).
+
+    The boundary between two blocks: f is the output of the last one, x the residual stream, h
+    the input of the next one.  x, f [..., C] float32 or bfloat16, C <= 8192.  Norms: None, "rms"
+    (x / sqrt(mean x^2 + eps)) or "layer" (mean taken off first), each with an optional weight and
+    bias [C] of float32 or x's type.  gate broadcasts against x ([C], [B, 1, C], [B, N, C], ...) and
+    has its type.  p, seed, site: as in ``dropout``.  f None: y is x, h its norm.  pre_norm None:
+    h is None.  h is made from y before y is rounded; the backward pass reads y as returned.
+    Differentiable (once) in x, f, gate, weights and biases."""
+    fn = "gated_residual_norm"
+    _check_tensor(fn, "x", x)
+    _check(x.dtype in _DTYPES, f"{fn}: type {x.dtype} not supported (float32, bfloat16)")
+    _check(x.dim() >= 1 and 1 <= x.shape[-1] <= 8192, f"{fn}: x {tuple(x.shape)} must have 1 .. 8192 channels")
+    C, dev = x.shape[-1], x.device
+    _check(x.numel() // C <= 2 ** 30, f"{fn}: more than 2^30 rows")
+    for name, norm, w, b in (("post", post_norm, post_weight, post_bias), ("pre", pre_norm, pre_weight, pre_bias)):
+        _check(norm in _NORMS, f"{fn}: {name}_norm {norm!r} is not one of None, 'rms', 'layer'")
+        _check(norm is not None or (w is None and b is None), f"{fn}: {name}_weight / {name}_bias without a norm")
+    params = {"post_weight": post_weight, "post_bias": post_bias, "pre_weight": pre_weight, "pre_bias": pre_bias}
+    for name, t in params.items():
+        if t is not None:
+            _check_tensor(fn, name, t, dev)
+            _check(tuple(t.shape) == (C,), f"{fn}: {name} must be [{C}], got {tuple(t.shape)}")
+            _check(t.dtype in (torch.float32, x.dtype), f"{fn}: {name} has type {t.dtype}, expected float32 or {x.dtype}")
+    step, value, seed = _draws(fn, p, seed, site, dev)
+    if f is None:
+        _check(gate is None and post_norm is None and step == 0, f"{fn}: gate, post_norm and p need f")
+        _check(pre_norm is not None, f"{fn}: neither f nor pre_norm: nothing to do")
+    else:
+        _check_tensor(fn, "f", f, dev, x.dtype)
+        _check(f.shape == x.shape, f"{fn}: f {tuple(f.shape)} does not fit x {tuple(x.shape)}")
+        f = f.contiguous()
+    _check(math.isfinite(float(scale)), f"{fn}: scale {scale} is not finite")
+    _check(float(eps) >= 0.0, f"{fn}: eps {eps} is negative")
+    rows = 1
+    if gate is not None:
+        _check_tensor(fn, "gate", gate, dev, x.dtype)
+        _check(1 <= gate.dim() <= x.dim() and all(
+            n in (1, m) for n, m in zip(reversed(gate.shape), reversed(x.shape))),
+            f"{fn}: gate {tuple(gate.shape)} does not broadcast to {tuple(x.shape)}")
+        gate, rows = _gate_of(gate, x)
+    types = {t.dtype for t in params.values() if t is not None} or {torch.float32}
+    if len(types) > 1:
+        params = {n: None if t is None else t.float() for n, t in params.items()}
+        types = {torch.float32}
+    params = [None if t is None else t.contiguous() for t in params.values()]
+    o = _BlockOptions(float(scale), float(eps), _NORMS[post_norm], _NORMS[pre_norm], step, value, site, rows)
+    x = x.contiguous()
+    y, h = _GatedResidualNorm.apply(x, f, gate, *params, o, seed if step else None, types.pop())
+    return x if y is None else y, h
