@@ -786,7 +786,11 @@ typedef struct {
     const void *q, *k, *v;
     void *out; /* read by the backward pass */
     int64_t qs[3], ks[3], vs[3], os[3];
-    float *lse; /* [B][H][Nq] log2 of the rows' sums: written by fwd (or NULL), read by bwd */
+    /* written by fwd (or NULL), read by bwd: lse [2][B][H][Nq], for f32 rows the rows' largest score
+     * (in units of log2) and 1 / sum, for bf16 rows log2 of their sums and nothing; out_rest, like
+     * out but contiguous, bf16 only: what out lost in rounding */
+    float *lse;
+    void *out_rest;
     const int32_t *q_len, *k_len;
     const uint8_t *key_mask;
     int64_t mask_sb;

@@ -64,7 +64,7 @@ class TokAttn(ctypes.Structure):
     _fields_ = [("dtype", _i), ("B", _i), ("Nq", _i), ("Nk", _i), ("H", _i), ("Hk", _i), ("D", _i),
                 ("causal", _i), ("align_end", _i), ("scale", ctypes.c_float), ("q", _vp), ("k", _vp),
                 ("v", _vp), ("out", _vp), ("qs", _i64 * 3), ("ks", _i64 * 3), ("vs", _i64 * 3),
-                ("os", _i64 * 3), ("lse", _vp), ("q_len", _vp), ("k_len", _vp), ("key_mask", _vp),
+                ("os", _i64 * 3), ("lse", _vp), ("out_rest", _vp), ("q_len", _vp), ("k_len", _vp), ("key_mask", _vp),
                 ("mask_sb", _i64), ("bias", _vp), ("bias_dtype", _i), ("num_buckets", _i),
                 ("max_distance", _i), ("both", _i), ("nthresh", _i),
                 ("thresh", ctypes.c_int32 * TOK_MAX_THRESH), ("dout", _vp), ("dos", _i64 * 3),

@@ -33,7 +33,7 @@ struct Buckets {
 
 struct Args {
     const void *q, *k, *v, *out_r, *dout;
-    void *out, *dq, *dk, *dv, *dbias;
+    void *out, *rest, *dq, *dk, *dv, *dbias;
     float *lse, *delta, *bins;
     const int *q_len, *k_len;
     const uint8_t *key_mask;
@@ -117,6 +117,34 @@ __device__ __forceinline__ void load_row(const T *row, bool ok, int D, int lane,
         else x.zero();
         x.pieces(f[c]);
     }
+}
+
+// What the backward pass makes a row's probabilities from.  bf16: p = exp2(s - log2 of the sum).
+// f32: p = exp2(s - m) / sum with the forward pass's own m and 1 / sum, because the logarithm of a
+// sum near 2^10 is rounded by 2^-21 and that error would be common to a row: it does not cancel in
+// the bias gradient's sums (6 times their error).  A row without keys: p = exp2(s - inf) = 0.
+struct RowSum { float ref, inv; };
+template <class T>
+__device__ __forceinline__ void save_sum(const Args &a, size_t row, bool any, float m, float l, float inv) {
+    if constexpr (Elem<T>::NP == 1) {
+        a.lse[row] = any ? m + __builtin_amdgcn_logf(l) : INFINITY;
+    } else {
+        a.lse[row] = any ? m : INFINITY;
+        a.lse[(size_t)a.B * a.H * a.Nq + row] = inv;
+    }
+}
+template <class T>
+__device__ __forceinline__ RowSum row_sum_of(const Args &a, size_t row, bool ok) {
+    RowSum r{INFINITY, 0.f};
+    if (!ok) return r;
+    r.ref = a.lse[row];
+    if constexpr (Elem<T>::NP > 1) r.inv = a.lse[(size_t)a.B * a.H * a.Nq + row];
+    return r;
+}
+template <class T>
+__device__ __forceinline__ float prob(float s, float ref, float inv) {
+    const float p = __builtin_amdgcn_exp2f(s - ref);
+    return Elem<T>::NP == 1 ? p : p * inv;
 }
 
 // ---------------------------------------------------------------------- forward --
@@ -243,18 +271,24 @@ __global__ __launch_bounds__(NT) void attn_fwd(Args a) {
     const float inv = any ? 1.f / l : 0.f;
     if (i < a.Nq) {
         T *o = static_cast<T *>(a.out) + w.b * a.os[0] + (int64_t)i * a.os[1] + w.h * a.os[2];
+        T *rest = a.rest ? static_cast<T *>(a.rest) + (((int64_t)w.b * a.Nq + i) * a.H + w.h) * a.D : nullptr;
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
                 const int col = 32 * d + 2 * r + 4 * half;
-                if (col < a.D)
-                    store4(o + col, any ? acc[d][r] * inv : 0.f, any ? acc[d][r + 1] * inv : 0.f,
-                           any ? acc[d][r + 2] * inv : 0.f, any ? acc[d][r + 3] * inv : 0.f);
+                if (col >= a.D) continue;
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = any ? acc[d][r + e] * inv : 0.f;
+                store4(o + col, x[0], x[1], x[2], x[3]);
+                if constexpr (NP == 1) {
+                    if (rest)
+                        store4(rest + col, x[0] - (float)(T)x[0], x[1] - (float)(T)x[1], x[2] - (float)(T)x[2],
+                               x[3] - (float)(T)x[3]);
+                }
             }
-        // a row without keys: p = exp2(s - inf) = 0 in the backward pass
-        if (a.lse && half == 0)
-            a.lse[((size_t)w.b * a.H + w.h) * a.Nq + i] = any ? m + __builtin_amdgcn_logf(l) : INFINITY;
+        if (a.lse && half == 0) save_sum<T>(a, ((size_t)w.b * a.H + w.h) * a.Nq + i, any, m, l, inv);
     }
 }
 
@@ -272,6 +306,10 @@ __global__ __launch_bounds__(NT) void attn_delta(Args a) {
         x.load(static_cast<const T *>(a.dout) + b * a.dos[0] + (int64_t)i * a.dos[1] + h * a.dos[2] + d);
         y.load(static_cast<const T *>(a.out_r) + b * a.os[0] + (int64_t)i * a.os[1] + h * a.os[2] + d);
         s = x.dot(y);
+        if (a.rest) {  // what out lost in rounding: it would be common to a row's ds
+            y.load(static_cast<const T *>(a.rest) + (((int64_t)b * a.Nq + i) * a.H + h) * a.D + d);
+            s += x.dot(y);
+        }
     }
     s = row_sum16(s);
     if (threadIdx.x % 16 == 0) a.delta[row] = s;
@@ -284,7 +322,7 @@ __global__ __launch_bounds__(NT) void attn_bwd_kv(Args a) {
     constexpr int NP = Elem<T>::NP, PLANE = QT * DP;
     extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
     uint16_t *qt = lds, *dt = lds + NP * PLANE;
-    float *lt = reinterpret_cast<float *>(lds + 2 * NP * PLANE), *et = lt + QT, *tab = et + QT;
+    float *lt = reinterpret_cast<float *>(lds + 2 * NP * PLANE), *et = lt + QT, *it = et + QT, *tab = it + QT;
     const Where w = where(a.Hk, (a.Nk + ROWS - 1) / ROWS);
     const Span sp = span_of(a, w.b);
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
@@ -305,7 +343,7 @@ __global__ __launch_bounds__(NT) void attn_bwd_kv(Args a) {
             const int h = w.h * G + g;
             const T *Q = static_cast<const T *>(a.q) + w.b * a.qs[0] + h * a.qs[2];
             const T *dO = static_cast<const T *>(a.dout) + w.b * a.dos[0] + h * a.dos[2];
-            const float *lse = a.lse + ((size_t)w.b * a.H + h) * a.Nq, *delta = a.delta + ((size_t)w.b * a.H + h) * a.Nq;
+            const size_t row0 = ((size_t)w.b * a.H + h) * a.Nq;
             if constexpr (BIAS) {
                 __syncthreads();
                 fill_table(a, tab, h);
@@ -321,8 +359,10 @@ __global__ __launch_bounds__(NT) void attn_bwd_kv(Args a) {
                 sd.store(dt);
                 if (threadIdx.x < QT) {
                     const int i = i0 + threadIdx.x;
-                    lt[threadIdx.x] = i < sp.nq ? lse[i] : INFINITY;
-                    et[threadIdx.x] = i < sp.nq ? delta[i] : 0.f;
+                    const RowSum rs = row_sum_of<T>(a, row0 + i, i < sp.nq);
+                    lt[threadIdx.x] = rs.ref;
+                    it[threadIdx.x] = rs.inv;
+                    et[threadIdx.x] = i < sp.nq ? a.delta[row0 + i] : 0.f;
                 }
                 __syncthreads();
                 if (i0 + QT < sp.nq) {
@@ -353,7 +393,7 @@ __global__ __launch_bounds__(NT) void attn_bwd_kv(Args a) {
                             const int o = j - (p0 + ir);
                             if constexpr (BIAS) x += tab[min(max(o, -a.bk.far), a.bk.far) + a.bk.far];
                             const bool keep = !edge || o <= 0;
-                            p[r] = keep ? __builtin_amdgcn_exp2f(x - lt[32 * t + ir]) : 0.f;
+                            p[r] = keep ? prob<T>(x, lt[32 * t + ir], it[32 * t + ir]) : 0.f;
                             ds[r] = keep ? p[r] * (dp[8 * c + r] - et[32 * t + ir]) : 0.f;
                         }
                         bf16x8 pf[NP], sf[NP];
@@ -469,7 +509,8 @@ __global__ __launch_bounds__(NT) void attn_bwd_q(Args a) {
     load_row<T, DP>(static_cast<const T *>(a.dout) + w.b * a.dos[0] + (int64_t)i * a.dos[1] + w.h * a.dos[2], i < sp.nq,
                     a.D, lane, df);
     const size_t row = ((size_t)w.b * a.H + w.h) * a.Nq + i;
-    const float lse = i < sp.nq ? a.lse[row] : INFINITY, delta = i < sp.nq ? a.delta[row] : 0.f;
+    const RowSum rs = row_sum_of<T>(a, row, i < sp.nq);
+    const float delta = i < sp.nq ? a.delta[row] : 0.f;
     const float scale2 = a.scale * LOG2E;
     f32x16 acc[DP / 32];
 #pragma unroll
@@ -509,7 +550,7 @@ __global__ __launch_bounds__(NT) void attn_bwd_q(Args a) {
             finish_scores<BIAS>(a, s, scale2, tab, a.bk.far, j, j - (i + sp.start), sp.nk, edge, mask, half);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const float p = __builtin_amdgcn_exp2f(s[r] - lse);
+                const float p = prob<T>(s[r], rs.ref, rs.inv);
                 s[r] = s[r] == -INFINITY ? 0.f : p * (dp[r] - delta);
             }
             if (BIAS && a.dbias) dg.tile(s, j - qw, bins, a.bk.far, lane);
@@ -575,9 +616,11 @@ __global__ __launch_bounds__(NT) void bias_reduce(Args a) {
 
 int row_tiles(int n) { return (n + ROWS - 1) / ROWS; }
 
-bool vec_ok(const void *p, const int64_t s[3], int esize) {
-    const int64_t n = 16 / esize;
-    return p && reinterpret_cast<uintptr_t>(p) % 16 == 0 && s[0] % n == 0 && s[1] % n == 0 && s[2] % n == 0;
+// rows of (batch, tokens, heads) in 16-byte steps; a dimension of one is never stepped over
+bool rows_ok(const void *p, const int64_t s[3], int esize, int b, int n, int h) {
+    const int64_t e = 16 / esize;
+    return p && reinterpret_cast<uintptr_t>(p) % 16 == 0 && (b == 1 || s[0] % e == 0) && (n == 1 || s[1] % e == 0) &&
+           (h == 1 || s[2] % e == 0);
 }
 
 // the argument checks shared by both directions; fills the kernels' arguments
@@ -590,10 +633,12 @@ int take(const hreg_tok_attn_t *p, Args &a) {
         return HREG_ERR_UNSUPPORTED;
     const int es = p->dtype == HREG_TOK_F32 ? 4 : 2;
     const bool empty = p->B == 0 || p->Nq == 0;
-    if (!empty && (!vec_ok(p->q, p->qs, es) || !vec_ok(p->out, p->os, es))) return HREG_ERR_INVALID;
-    if (p->B > 0 && p->Nk > 0 && (!vec_ok(p->k, p->ks, es) || !vec_ok(p->v, p->vs, es))) return HREG_ERR_INVALID;
+    if (!empty && (!rows_ok(p->q, p->qs, es, p->B, p->Nq, p->H) || !rows_ok(p->out, p->os, es, p->B, p->Nq, p->H) ||
+                   reinterpret_cast<uintptr_t>(p->out_rest) % 16)) return HREG_ERR_INVALID;
+    if (p->B > 0 && p->Nk > 0 && (!rows_ok(p->k, p->ks, es, p->B, p->Nk, p->Hk) || !rows_ok(p->v, p->vs, es, p->B, p->Nk, p->Hk))) return HREG_ERR_INVALID;
     a = Args{};
     a.q = p->q; a.k = p->k; a.v = p->v; a.out = p->out; a.out_r = p->out; a.dout = p->dout;
+    a.rest = p->dtype == HREG_TOK_BF16 ? p->out_rest : nullptr;
     a.dq = p->dq; a.dk = p->dk; a.dv = p->dv; a.dbias = p->dbias;
     a.lse = p->lse; a.q_len = p->q_len; a.k_len = p->k_len; a.key_mask = p->key_mask; a.bias = p->bias;
     for (int i = 0; i < 3; ++i) {
@@ -645,7 +690,7 @@ int bwd(const Args &a, void *stream) {
         hipLaunchKernelGGL(attn_delta<T>, dim3((rows + NT / 16 - 1) / (NT / 16)), dim3(NT), 0, as_stream(stream), a);
         HREG_CHECK_LAUNCH();
     }
-    if (a.Nk > 0 && a.dk) rc = launch(attn_bwd_kv<T, DP, QT, BIAS>, a.B * a.Hk * row_tiles(a.Nk), tile + (2 * QT + W) * 4, stream, a);
+    if (a.Nk > 0 && a.dk) rc = launch(attn_bwd_kv<T, DP, QT, BIAS>, a.B * a.Hk * row_tiles(a.Nk), tile + (3 * QT + W) * 4, stream, a);
     if (rc == HREG_OK && a.Nq > 0 && (a.dq || a.dbias))
         rc = launch(attn_bwd_q<T, DP, QT, BIAS>, a.B * a.H * row_tiles(a.Nq), tile + 5 * W * 4, stream, a);
     return rc;
@@ -696,7 +741,7 @@ int hreg_tok_attn_bwd(const hreg_tok_attn_t *p, void *stream) {
     const int rc = take(p, a);
     if (rc != HREG_OK) return rc;
     if (!a.bias) a.dbias = nullptr;
-    if (a.B > 0 && a.Nq > 0 && (!vec_ok(p->dout, p->dos, p->dtype == HREG_TOK_F32 ? 4 : 2) || !p->lse)) return HREG_ERR_INVALID;
+    if (a.B > 0 && a.Nq > 0 && (!rows_ok(p->dout, p->dos, p->dtype == HREG_TOK_F32 ? 4 : 2, p->B, p->Nq, p->H) || !p->lse)) return HREG_ERR_INVALID;
     for (const void *g : {p->dq, p->dk, p->dv})
         if (reinterpret_cast<uintptr_t>(g) % 16) return HREG_ERR_INVALID;
     if (!p->dk != !p->dv) return HREG_ERR_INVALID;

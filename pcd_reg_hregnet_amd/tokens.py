@@ -18,7 +18,6 @@ graph: nothing is read on the host, and a seed tensor is read when the graph rep
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 import math
@@ -32,29 +31,43 @@ _DTYPES = {torch.float32: _lib.TOK_F32, torch.bfloat16: _lib.TOK_BF16}
 _NORMS = {None: 0, "rms": 1, "layer": 2}
 
 
-def _check(cond: bool, text: str) -> None:
-    if not cond:
-        raise ValueError(text)
+_ENTRIES = {}
 
 
-def _check_tensor(fn: str, name: str, t, device=None, dtype=None) -> None:
-    _check(isinstance(t, torch.Tensor) and t.is_cuda, f"{fn}: {name} must be a GPU tensor (no CPU fallback)")
-    _check(device is None or t.device == device, f"{fn}: {name} is on {t.device}, expected {device}")
-    _check(dtype is None or t.dtype == dtype, f"{fn}: {name} has type {t.dtype}, expected {dtype}")
+def _call(name: str, *args) -> None:
+    """the C entry, bound at its first call (``_lib.load`` checks the library and the GPU then)"""
+    f = _ENTRIES.get(name)
+    if f is None:
+        f = _ENTRIES[name] = getattr(_lib.load(), name)
+    rc = f(*args)
+    if rc != _lib.HREG_OK:
+        raise RuntimeError(f"{name} failed: {_lib._ERRORS.get(rc, rc)} (code {rc})")
 
 
-@contextlib.contextmanager
-def _on(device):
-    """the tensors' device is current inside; yields its current stream"""
+def _launch(device, name: str, *args) -> None:
+    """the entry on the current stream of the tensors' device, which is current meanwhile"""
     if device.index == torch.cuda.current_device():
-        yield _lib.stream_handle()
+        _call(name, *args, _raw_stream(device.index))
     else:
         with torch.cuda.device(device):
-            yield _lib.stream_handle()
+            _call(name, *args, _raw_stream(device.index))
 
 
-def _launch(name: str, args, stream) -> None:
-    _lib.call(name, ctypes.byref(args), stream)
+# the handle of a device's current stream without the Stream object around it (torch's own
+# compiled code takes it from here): 0.3 us instead of 2.7
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+# (checks build their messages only when they fail: a call's host time is what a single token
+# waits for)
+def _check_tensor(fn: str, name: str, t, device=None, dtype=None) -> None:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{fn}: {name} must be a GPU tensor (no CPU fallback)")
+    if device is not None and t.device != device:
+        raise ValueError(f"{fn}: {name} is on {t.device}, expected {device}")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{fn}: {name} has type {t.dtype}, expected {dtype}")
 
 
 def _ptr(t):
@@ -94,12 +107,14 @@ class Buckets:
 
     def __post_init__(self):
         n, far = self.num_buckets, self.max_distance
-        _check(isinstance(n, int) and isinstance(far, int), "Buckets: num_buckets and max_distance must be int")
-        _check(2 <= n <= _lib.TOK_MAX_BUCKETS, f"Buckets: num_buckets {n} not in 2 .. {_lib.TOK_MAX_BUCKETS}")
-        _check(not self.bidirectional or (n % 2 == 0 and n >= 4),
-               f"Buckets: num_buckets {n} must be even and at least 4 for both directions")
-        _check(self._side // 2 < far <= _lib.TOK_MAX_DISTANCE,
-               f"Buckets: max_distance {far} not in {self._side // 2 + 1} .. {_lib.TOK_MAX_DISTANCE}")
+        if not (isinstance(n, int) and isinstance(far, int)):
+            raise ValueError("Buckets: num_buckets and max_distance must be int")
+        if not 2 <= n <= _lib.TOK_MAX_BUCKETS:
+            raise ValueError(f"Buckets: num_buckets {n} not in 2 .. {_lib.TOK_MAX_BUCKETS}")
+        if self.bidirectional and (n % 2 or n < 4):
+            raise ValueError(f"Buckets: num_buckets {n} must be even and at least 4 for both directions")
+        if not self._side // 2 < far <= _lib.TOK_MAX_DISTANCE:
+            raise ValueError(f"Buckets: max_distance {far} not in {self._side // 2 + 1} .. {_lib.TOK_MAX_DISTANCE}")
 
     @property
     def _side(self) -> int:
@@ -122,75 +137,66 @@ class Buckets:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t, or a copy of it whose rows the kernels can read: contiguous rows in 16-byte steps"""
-    n = 16 // t.element_size()
-    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
-        s % n == 0 for s, m in zip(t.stride()[:-1], t.shape[:-1]) if m > 1)
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            return t
+        n = 16 // t.element_size()
+        if t.stride(-1) == 1 and all(s % n == 0 for s, m in zip(t.stride()[:-1], t.shape[:-1]) if m > 1):
+            return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
-def _strides(t: torch.Tensor):
-    """(batch, token, head) strides; a dimension of one element is never stepped over"""
-    return (ctypes.c_int64 * 3)(*(s if m > 1 else 0 for s, m in zip(t.stride()[:3], t.shape[:3])))
-
-
-@dataclass(frozen=True)
-class _AttnOptions:
-    scale: float
-    causal: bool
-    align_end: bool
-    buckets: Buckets | None
-
-
-def _attn_args(o: _AttnOptions, q, k, v, out, lse, q_len, k_len, key_mask, bias) -> _lib.TokAttn:
-    p = _lib.TokAttn()
-    p.dtype = _DTYPES[q.dtype]
-    p.B, p.Nq, p.H, p.D = q.shape
-    p.Nk, p.Hk = k.shape[1], k.shape[2]
-    p.causal, p.align_end, p.scale = int(o.causal), int(o.align_end), o.scale
-    p.q, p.k, p.v, p.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
-    p.qs, p.ks, p.vs, p.os = _strides(q), _strides(k), _strides(v), _strides(out)
-    p.lse, p.q_len, p.k_len, p.key_mask = _ptr(lse), _ptr(q_len), _ptr(k_len), _ptr(key_mask)
-    p.mask_sb = 0 if key_mask is None or key_mask.shape[0] == 1 else key_mask.stride(0)
+def _attn_args(o, q, k, v, out, lse, out_rest, q_len, k_len, key_mask, bias) -> _lib.TokAttn:
+    scale, causal, align_end, buckets = o
+    B, Nq, H, D = q.shape
+    p = _lib.TokAttn(_DTYPES[q.dtype], B, Nq, k.shape[1], H, k.shape[2], D, causal, align_end, scale, q.data_ptr(),
+                     k.data_ptr(), v.data_ptr(), out.data_ptr(), q.stride()[:3], k.stride()[:3], v.stride()[:3],
+                     out.stride()[:3], _ptr(lse), _ptr(out_rest), _ptr(q_len), _ptr(k_len))
+    if key_mask is not None:
+        p.key_mask, p.mask_sb = key_mask.data_ptr(), 0 if key_mask.shape[0] == 1 else key_mask.stride(0)
     if bias is not None:
-        b = o.buckets
         p.bias, p.bias_dtype = bias.data_ptr(), _DTYPES[bias.dtype]
-        p.num_buckets, p.max_distance, p.both = b.num_buckets, b.max_distance, int(b.bidirectional)
-        p.nthresh = len(b.thresholds)
-        p.thresh[:p.nthresh] = b.thresholds
+        p.num_buckets, p.max_distance, p.both = buckets.num_buckets, buckets.max_distance, buckets.bidirectional
+        t = buckets.thresholds
+        p.nthresh = len(t)
+        p.thresh = t
     return p
 
 
 def _attn_ws(p: _lib.TokAttn, backward: int, device):
-    n = _lib.load().hreg_tok_attn_ws_bytes(ctypes.byref(p), backward)
-    ws = torch.empty(max(n, 16), dtype=torch.uint8, device=device)
+    n = _lib.load(require_gpu=False).hreg_tok_attn_ws_bytes(ctypes.byref(p), backward)
+    if n == 0:
+        return None
+    ws = torch.empty(n, dtype=torch.uint8, device=device)
     p.ws, p.ws_bytes = ws.data_ptr(), n
     return ws
 
 
-def _attn_forward(o, q, k, v, bias, q_len, k_len, key_mask, want_lse: bool):
+def _attn_forward(o, q, k, v, bias, q_len, k_len, key_mask, train: bool):
     q, k, v = _rows(q), _rows(k), _rows(v)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    dev = q.device
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     B, Nq, H, _ = q.shape
-    lse = torch.empty(B, H, Nq, device=q.device) if want_lse else None
-    with _on(q.device) as stream:
-        p = _attn_args(o, q, k, v, out, lse, q_len, k_len, key_mask, bias)
-        ws = _attn_ws(p, 0, q.device)  # noqa: F841 (held until the launch is queued)
-        _launch("hreg_tok_attn_fwd", p, stream)
-    return q, k, v, out, lse
+    lse = torch.empty(2, B, H, Nq, device=dev) if train else None
+    rest = torch.empty_like(out) if train and q.dtype != torch.float32 else None
+    p = _attn_args(o, q, k, v, out, lse, rest, q_len, k_len, key_mask, bias)
+    ws = _attn_ws(p, 0, dev)  # noqa: F841 (held until the launch is queued)
+    _launch(dev, "hreg_tok_attn_fwd", ctypes.byref(p))
+    return q, k, v, out, lse, rest
 
 
 class _TokAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias, o, q_len, k_len, key_mask):
-        q, k, v, out, lse = _attn_forward(o, q, k, v, bias, q_len, k_len, key_mask, True)
-        ctx.save_for_backward(q, k, v, bias, out, lse, q_len, k_len, key_mask)
+        q, k, v, out, lse, rest = _attn_forward(o, q, k, v, bias, q_len, k_len, key_mask, True)
+        ctx.save_for_backward(q, k, v, bias, out, lse, rest, q_len, k_len, key_mask)
         ctx.o = o
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, bias, out, lse, q_len, k_len, key_mask = ctx.saved_tensors
+        q, k, v, bias, out, lse, rest, q_len, k_len, key_mask = ctx.saved_tensors
         need_q, need_k, need_v, need_b = ctx.needs_input_grad[:4]
         dout = _rows(dout)
         dev = q.device
@@ -198,12 +204,11 @@ class _TokAttention(torch.autograd.Function):
         dk = torch.empty(k.shape, dtype=k.dtype, device=dev) if need_k or need_v else None
         dv = torch.empty(v.shape, dtype=v.dtype, device=dev) if need_k or need_v else None
         db = torch.empty(bias.shape, dtype=bias.dtype, device=dev) if need_b else None
-        with _on(dev) as stream:
-            p = _attn_args(ctx.o, q, k, v, out, lse, q_len, k_len, key_mask, bias)
-            p.dout, p.dos = dout.data_ptr(), _strides(dout)
-            p.dq, p.dk, p.dv, p.dbias = _ptr(dq), _ptr(dk), _ptr(dv), _ptr(db)
-            ws = _attn_ws(p, 1, dev)  # noqa: F841
-            _launch("hreg_tok_attn_bwd", p, stream)
+        p = _attn_args(ctx.o, q, k, v, out, lse, rest, q_len, k_len, key_mask, bias)
+        p.dout, p.dos = dout.data_ptr(), dout.stride()[:3]
+        p.dq, p.dk, p.dv, p.dbias = _ptr(dq), _ptr(dk), _ptr(dv), _ptr(db)
+        ws = _attn_ws(p, 1, dev)  # noqa: F841
+        _launch(dev, "hreg_tok_attn_bwd", ctypes.byref(p))
         return dq, dk if need_k else None, dv if need_v else None, db, None, None, None, None
 
 
@@ -211,8 +216,8 @@ def _lengths(name: str, t, B: int, device):
     if t is None:
         return None
     _check_tensor("attention", name, t, device)
-    _check(t.dtype in (torch.int32, torch.int64) and tuple(t.shape) == (B,),
-           f"attention: {name} must be int32 or int64 of shape ({B},), got {t.dtype} {tuple(t.shape)}")
+    if t.dtype not in (torch.int32, torch.int64) or t.shape != (B,):
+        raise ValueError(f"attention: {name} must be int32 or int64 of shape ({B},), got {t.dtype} {tuple(t.shape)}")
     if t.dtype == torch.int64:
         t = t.clamp(0, 2 ** 31 - 1).to(torch.int32)
     return t.contiguous()
@@ -239,34 +244,46 @@ def attention(q, k, v, *, scale=None, causal=False, align_end=None, q_lengths=No
 
     bias [num_buckets, H] (float32 or q's type) and ``Buckets`` add a learned bias by the offset of
     key and query.  With bfloat16 rows its gradient has their accuracy (about 2^-8 of it)."""
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        _check_tensor("attention", name, t, None if name == "q" else q.device, None if name == "q" else q.dtype)
-        _check(t.dim() == 4, f"attention: {name} must be [batch, tokens, heads, width], got {tuple(t.shape)}")
-    _check(q.dtype in _DTYPES, f"attention: type {q.dtype} not supported (float32, bfloat16)")
+    _check_tensor("attention", "q", q)
+    dev, dtype = q.device, q.dtype
+    _check_tensor("attention", "k", k, dev, dtype)
+    _check_tensor("attention", "v", v, dev, dtype)
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError(f"attention: q, k, v must be [batch, tokens, heads, width], got {tuple(q.shape)}, {tuple(k.shape)}, "
+                         f"{tuple(v.shape)}")
+    if dtype not in _DTYPES:
+        raise ValueError(f"attention: type {dtype} not supported (float32, bfloat16)")
     B, Nq, H, D = q.shape
-    Nk, Hk = k.shape[1], k.shape[2]
-    _check(tuple(k.shape) == (B, Nk, Hk, D) and k.shape == v.shape,
-           f"attention: k {tuple(k.shape)} and v {tuple(v.shape)} do not fit q {tuple(q.shape)}")
-    _check(H >= 1 and Hk >= 1 and H % Hk == 0, f"attention: {H} heads are not a multiple of {Hk} key heads")
-    _check(8 <= D <= 128 and D % 8 == 0, f"attention: width {D} is not a multiple of 8 up to 128")
+    _, Nk, Hk, _ = k.shape
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+        raise ValueError(f"attention: k {tuple(k.shape)} and v {tuple(v.shape)} do not fit q {tuple(q.shape)}")
+    if H < 1 or Hk < 1 or H % Hk:
+        raise ValueError(f"attention: {H} heads are not a multiple of {Hk} key heads")
+    if not 8 <= D <= 128 or D % 8:
+        raise ValueError(f"attention: width {D} is not a multiple of 8 up to 128")
     scale = D ** -0.5 if scale is None else float(scale)
-    _check(math.isfinite(scale), f"attention: scale {scale} is not finite")
-    q_len, k_len = _lengths("q_lengths", q_lengths, B, q.device), _lengths("k_lengths", k_lengths, B, q.device)
+    if not math.isfinite(scale):
+        raise ValueError(f"attention: scale {scale} is not finite")
+    q_len, k_len = _lengths("q_lengths", q_lengths, B, dev), _lengths("k_lengths", k_lengths, B, dev)
     if key_mask is not None:
-        _check_tensor("attention", "key_mask", key_mask, q.device, torch.bool)
-        _check(key_mask.dim() == 2 and key_mask.shape[0] in (1, B) and key_mask.shape[1] == Nk,
-               f"attention: key_mask must be [{B} or 1, {Nk}], got {tuple(key_mask.shape)}")
+        _check_tensor("attention", "key_mask", key_mask, dev, torch.bool)
+        if key_mask.dim() != 2 or key_mask.shape[0] not in (1, B) or key_mask.shape[1] != Nk:
+            raise ValueError(f"attention: key_mask must be [{B} or 1, {Nk}], got {tuple(key_mask.shape)}")
         key_mask = key_mask if key_mask.stride(1) == 1 else key_mask.contiguous()
-    _check((bias is None) == (buckets is None), "attention: bias and buckets come together")
+    if (bias is None) != (buckets is None):
+        raise ValueError("attention: bias and buckets come together")
     if bias is not None:
-        _check(isinstance(buckets, Buckets), "attention: buckets must be a Buckets")
-        _check_tensor("attention", "bias", bias, q.device)
-        _check(bias.dtype in (torch.float32, q.dtype), f"attention: bias has type {bias.dtype}, expected float32 or {q.dtype}")
-        _check(tuple(bias.shape) == (buckets.num_buckets, H),
-               f"attention: bias must be [{buckets.num_buckets}, {H}], got {tuple(bias.shape)}")
+        if not isinstance(buckets, Buckets):
+            raise ValueError("attention: buckets must be a Buckets")
+        _check_tensor("attention", "bias", bias, dev)
+        if bias.dtype not in (torch.float32, dtype):
+            raise ValueError(f"attention: bias has type {bias.dtype}, expected float32 or {dtype}")
+        if bias.shape != (buckets.num_buckets, H):
+            raise ValueError(f"attention: bias must be [{buckets.num_buckets}, {H}], got {tuple(bias.shape)}")
         bias = bias.contiguous()
-    o = _AttnOptions(scale, bool(causal), bool(causal if align_end is None else align_end), buckets)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias)):
+    o = scale, bool(causal), bool(causal if align_end is None else align_end), buckets
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                    or (bias is not None and bias.requires_grad)):
         return _TokAttention.apply(q, k, v, bias, o, q_len, k_len, key_mask)
     return _attn_forward(o, q, k, v, bias, q_len, k_len, key_mask, False)[3]
 
@@ -276,23 +293,26 @@ def attention(q, k, v, *, scale=None, causal=False, align_end=None, q_lengths=No
 def _draws(fn: str, p, seed, site, device):
     """(step, seed value, seed tensor): p counts in steps of 2^-16"""
     p = float(p)
-    _check(0.0 <= p < 1.0, f"{fn}: p {p} not in [0, 1)")
+    if not 0.0 <= p < 1.0:
+        raise ValueError(f"{fn}: p {p} not in [0, 1)")
     step = min(int(p * 65536 + 0.5), 65535)
-    _check(isinstance(site, int) and 0 <= site < 2 ** 32, f"{fn}: site must be an int of 32 bits")
+    if not isinstance(site, int) or not 0 <= site < 2 ** 32:
+        raise ValueError(f"{fn}: site must be an int of 32 bits")
     if isinstance(seed, torch.Tensor):
         _check_tensor(fn, "seed", seed, device, torch.int64)
-        _check(seed.numel() == 1, f"{fn}: seed must hold one value, got {tuple(seed.shape)}")
+        if seed.numel() != 1:
+            raise ValueError(f"{fn}: seed must hold one value, got {tuple(seed.shape)}")
         return step, 0, seed
-    _check(step == 0 or (isinstance(seed, int) and not isinstance(seed, bool)),
-           f"{fn}: p > 0 needs a seed (int or int64 GPU tensor)")
+    if step and (not isinstance(seed, int) or isinstance(seed, bool)):
+        raise ValueError(f"{fn}: p > 0 needs a seed (int or int64 GPU tensor)")
     return step, (seed or 0) & (2 ** 64 - 1), None
 
 
 def _dropout(x, step, value, seed, site):
     x = x.contiguous()
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    with _on(x.device) as stream:
-        _lib.call("hreg_tok_dropout", x, y, x.numel(), _DTYPES[x.dtype], step, value, _ptr(seed), site, stream)
+    y = torch.empty_like(x)
+    _launch(x.device, "hreg_tok_dropout", x.data_ptr(), y.data_ptr(), x.numel(), _DTYPES[x.dtype], step, value, _ptr(seed),
+            site)
     return y
 
 
@@ -320,7 +340,8 @@ def dropout(x, p, seed, *, site=0, training=True):
     backward pass).  site (32 bits) tells the places of one model apart that share a seed.
     float32 or bfloat16, any shape; training False returns x."""
     _check_tensor("dropout", "x", x)
-    _check(x.dtype in _DTYPES, f"dropout: type {x.dtype} not supported (float32, bfloat16)")
+    if x.dtype not in _DTYPES:
+        raise ValueError(f"dropout: type {x.dtype} not supported (float32, bfloat16)")
     step, value, seed = _draws("dropout", p, seed, site, x.device)
     if not training or step == 0:
         return x
@@ -329,28 +350,13 @@ def dropout(x, p, seed, *, site=0, training=True):
 
 # ------------------------------------------------------------------ residual, gate and norms
 
-@dataclass(frozen=True)
-class _BlockOptions:
-    scale: float
-    eps: float
-    post: int
-    pre: int
-    step: int
-    value: int
-    site: int
-    gate_rows: int
-
-
-def _block_args(o: _BlockOptions, like, param_dtype, seed, **tensors) -> _lib.TokBlock:
-    p = _lib.TokBlock()
+def _block_args(o, like, param_dtype, seed, x, f, gate, post_w, post_b, pre_w, pre_b, y, h, stats, *back) -> _lib.TokBlock:
+    """back: dy, dh, then the gradients of x .. pre_b"""
+    scale, eps, post, pre, step, value, site, gate_rows = o
     C = like.shape[-1]
-    p.dtype, p.param_dtype = _DTYPES[like.dtype], _DTYPES[param_dtype]
-    p.R, p.C, p.gate_rows = like.numel() // C, C, o.gate_rows
-    p.post, p.pre, p.scale, p.eps = o.post, o.pre, o.scale, o.eps
-    p.step, p.site, p.seed, p.seed_dev = o.step, o.site, o.value, _ptr(seed)
-    for name, t in tensors.items():
-        setattr(p, name, _ptr(t))
-    return p
+    return _lib.TokBlock(_DTYPES[like.dtype], _DTYPES[param_dtype], like.numel() // C, C, gate_rows, post, pre, scale, eps,
+                         step, site, value, _ptr(seed), _ptr(x), _ptr(f), _ptr(gate), _ptr(post_w), _ptr(post_b),
+                         _ptr(pre_w), _ptr(pre_b), _ptr(y), _ptr(h), _ptr(stats), *map(_ptr, back))
 
 
 class _GatedResidualNorm(torch.autograd.Function):
@@ -358,12 +364,10 @@ class _GatedResidualNorm(torch.autograd.Function):
     def forward(ctx, x, f, gate, post_w, post_b, pre_w, pre_b, o, seed, param_dtype):
         dev = x.device
         y = torch.empty_like(x) if f is not None else None
-        h = torch.empty_like(x) if o.pre else None
+        h = torch.empty_like(x) if o[3] else None
         stats = torch.empty(x.numel() // x.shape[-1], 4, device=dev)
-        with _on(dev) as stream:
-            p = _block_args(o, x, param_dtype, seed, x=x, f=f, gate=gate, post_w=post_w, post_b=post_b, pre_w=pre_w,
-                            pre_b=pre_b, y=y, h=h, stats=stats)
-            _launch("hreg_tok_block_fwd", p, stream)
+        p = _block_args(o, x, param_dtype, seed, x, f, gate, post_w, post_b, pre_w, pre_b, y, h, stats)
+        _launch(dev, "hreg_tok_block_fwd", ctypes.byref(p))
         ctx.save_for_backward(f, gate, post_w, post_b, pre_w, pre_b, stats, seed, x if y is None else y)
         ctx.o, ctx.param_dtype = o, param_dtype
         ctx.set_materialize_grads(False)
@@ -381,15 +385,17 @@ class _GatedResidualNorm(torch.autograd.Function):
         grads = [make(t) if n and t is not None else None for t, n in zip(like, need)]
         dy, dh = (None if g is None else g.contiguous() for g in (dy, dh))
         dev = y.device
-        with _on(dev) as stream:
-            p = _block_args(ctx.o, y, ctx.param_dtype, seed, y=y, f=f, gate=gate, post_w=post_w, post_b=post_b,
-                            pre_w=pre_w, pre_b=pre_b, stats=stats, dy=dy, dh=dh,
-                            **dict(zip(("dx", "df", "dgate", "dpost_w", "dpost_b", "dpre_w", "dpre_b"), grads)))
-            n = _lib.load().hreg_tok_block_ws_bytes(ctypes.byref(p))
-            ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
+        p = _block_args(ctx.o, y, ctx.param_dtype, seed, None, f, gate, post_w, post_b, pre_w, pre_b, y, None, stats, dy, dh,
+                        *grads)
+        n = _lib.load(require_gpu=False).hreg_tok_block_ws_bytes(ctypes.byref(p))
+        if n:
+            ws = torch.empty(n, dtype=torch.uint8, device=dev)
             p.ws, p.ws_bytes = ws.data_ptr(), n
-            _launch("hreg_tok_block_bwd", p, stream)
+        _launch(dev, "hreg_tok_block_bwd", ctypes.byref(p))
         return (*grads, None, None, None)
+
+
+_PARAMS = ("post_weight", "post_bias", "pre_weight", "pre_bias")
 
 
 def _gate_of(gate, x):
@@ -417,42 +423,56 @@ def gated_residual_norm(x, f, *, gate=None, scale=1.0, post_norm=None, post_weig
     Differentiable (once) in x, f, gate, weights and biases."""
     fn = "gated_residual_norm"
     _check_tensor(fn, "x", x)
-    _check(x.dtype in _DTYPES, f"{fn}: type {x.dtype} not supported (float32, bfloat16)")
-    _check(x.dim() >= 1 and 1 <= x.shape[-1] <= 8192, f"{fn}: x {tuple(x.shape)} must have 1 .. 8192 channels")
-    C, dev = x.shape[-1], x.device
-    _check(x.numel() // C <= 2 ** 30, f"{fn}: more than 2^30 rows")
-    for name, norm, w, b in (("post", post_norm, post_weight, post_bias), ("pre", pre_norm, pre_weight, pre_bias)):
-        _check(norm in _NORMS, f"{fn}: {name}_norm {norm!r} is not one of None, 'rms', 'layer'")
-        _check(norm is not None or (w is None and b is None), f"{fn}: {name}_weight / {name}_bias without a norm")
-    params = {"post_weight": post_weight, "post_bias": post_bias, "pre_weight": pre_weight, "pre_bias": pre_bias}
-    for name, t in params.items():
-        if t is not None:
-            _check_tensor(fn, name, t, dev)
-            _check(tuple(t.shape) == (C,), f"{fn}: {name} must be [{C}], got {tuple(t.shape)}")
-            _check(t.dtype in (torch.float32, x.dtype), f"{fn}: {name} has type {t.dtype}, expected float32 or {x.dtype}")
+    dtype, dev = x.dtype, x.device
+    if dtype not in _DTYPES:
+        raise ValueError(f"{fn}: type {dtype} not supported (float32, bfloat16)")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= 8192:
+        raise ValueError(f"{fn}: x {tuple(x.shape)} must have 1 .. 8192 channels")
+    C = x.shape[-1]
+    if x.numel() // C > 2 ** 30:
+        raise ValueError(f"{fn}: more than 2^30 rows")
+    if post_norm not in _NORMS or pre_norm not in _NORMS:
+        raise ValueError(f"{fn}: post_norm {post_norm!r}, pre_norm {pre_norm!r}: each one of None, 'rms', 'layer'")
+    params = [post_weight, post_bias, pre_weight, pre_bias]
+    types = set()
+    for name, t, norm in zip(_PARAMS, params, (post_norm, post_norm, pre_norm, pre_norm)):
+        if t is None:
+            continue
+        _check_tensor(fn, name, t, dev)
+        if norm is None:
+            raise ValueError(f"{fn}: {name} without a norm")
+        if t.shape != (C,):
+            raise ValueError(f"{fn}: {name} must be [{C}], got {tuple(t.shape)}")
+        if t.dtype not in (torch.float32, dtype):
+            raise ValueError(f"{fn}: {name} has type {t.dtype}, expected float32 or {dtype}")
+        types.add(t.dtype)
     step, value, seed = _draws(fn, p, seed, site, dev)
     if f is None:
-        _check(gate is None and post_norm is None and step == 0, f"{fn}: gate, post_norm and p need f")
-        _check(pre_norm is not None, f"{fn}: neither f nor pre_norm: nothing to do")
+        if gate is not None or post_norm is not None or step:
+            raise ValueError(f"{fn}: gate, post_norm and p need f")
+        if pre_norm is None:
+            raise ValueError(f"{fn}: neither f nor pre_norm: nothing to do")
     else:
-        _check_tensor(fn, "f", f, dev, x.dtype)
-        _check(f.shape == x.shape, f"{fn}: f {tuple(f.shape)} does not fit x {tuple(x.shape)}")
+        _check_tensor(fn, "f", f, dev, dtype)
+        if f.shape != x.shape:
+            raise ValueError(f"{fn}: f {tuple(f.shape)} does not fit x {tuple(x.shape)}")
         f = f.contiguous()
-    _check(math.isfinite(float(scale)), f"{fn}: scale {scale} is not finite")
-    _check(float(eps) >= 0.0, f"{fn}: eps {eps} is negative")
+    scale, eps = float(scale), float(eps)
+    if not math.isfinite(scale):
+        raise ValueError(f"{fn}: scale {scale} is not finite")
+    if not 0.0 <= eps < math.inf:
+        raise ValueError(f"{fn}: eps {eps} is not a finite number >= 0")
     rows = 1
     if gate is not None:
-        _check_tensor(fn, "gate", gate, dev, x.dtype)
-        _check(1 <= gate.dim() <= x.dim() and all(
-            n in (1, m) for n, m in zip(reversed(gate.shape), reversed(x.shape))),
-            f"{fn}: gate {tuple(gate.shape)} does not broadcast to {tuple(x.shape)}")
+        _check_tensor(fn, "gate", gate, dev, dtype)
+        if not 1 <= gate.dim() <= x.dim() or not all(n in (1, m) for n, m in zip(gate.shape[::-1], x.shape[::-1])):
+            raise ValueError(f"{fn}: gate {tuple(gate.shape)} does not broadcast to {tuple(x.shape)}")
         gate, rows = _gate_of(gate, x)
-    types = {t.dtype for t in params.values() if t is not None} or {torch.float32}
     if len(types) > 1:
-        params = {n: None if t is None else t.float() for n, t in params.items()}
+        params = [None if t is None else t.float() for t in params]
         types = {torch.float32}
-    params = [None if t is None else t.contiguous() for t in params.values()]
-    o = _BlockOptions(float(scale), float(eps), _NORMS[post_norm], _NORMS[pre_norm], step, value, site, rows)
-    x = x.contiguous()
-    y, h = _GatedResidualNorm.apply(x, f, gate, *params, o, seed if step else None, types.pop())
+    params = [None if t is None else t.contiguous() for t in params]
+    o = scale, eps, _NORMS[post_norm], _NORMS[pre_norm], step, value, site, rows
+    y, h = _GatedResidualNorm.apply(x.contiguous(), f, gate, *params, o, seed if step else None,
+                                    types.pop() if types else torch.float32)
     return x if y is None else y, h
