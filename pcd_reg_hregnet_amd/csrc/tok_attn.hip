@@ -108,13 +108,14 @@ struct Stage {
 // one row's pieces as an operand with the row in lane & 31, straight from global memory
 template <class T, int DP>
 __device__ __forceinline__ void load_row(const T *row, bool ok, int D, int lane,
-                                         bf16x8 (&f)[DP / 16][Elem<T>::NP]) {
+                                         bf16x8 (&f)[DP / 16][Elem<T>::NP], bool negate = false) {
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
         const int d = 16 * c + 8 * (lane >> 5);
         Chunk<T> x;
         if (ok && d < D) x.load(row + d);
         else x.zero();
+        if (negate) x.negate();
         x.pieces(f[c]);
     }
 }
@@ -506,8 +507,13 @@ __global__ __launch_bounds__(NT) void attn_bwd_q(Args a) {
     bf16x8 qf[DP / 16][NP], df[DP / 16][NP];
     load_row<T, DP>(static_cast<const T *>(a.q) + w.b * a.qs[0] + (int64_t)i * a.qs[1] + w.h * a.qs[2], i < sp.nq, a.D,
                     lane, qf);
+    // The matrix cores round sums down, not to nearest: do . v comes out about 1e-8 of its size too
+    // low, which a single ds does not feel but a bias gradient's sum over 10^6 of them does (f32: 9
+    // times the error of one rounded to nearest).  Odd queries take -do, and their error the other way.
+    const bool odd = NP > 1 && (lane & 1);
     load_row<T, DP>(static_cast<const T *>(a.dout) + w.b * a.dos[0] + (int64_t)i * a.dos[1] + w.h * a.dos[2], i < sp.nq,
-                    a.D, lane, df);
+                    a.D, lane, df, odd);
+    const float sign = odd ? -1.f : 1.f;
     const size_t row = ((size_t)w.b * a.H + w.h) * a.Nq + i;
     const RowSum rs = row_sum_of<T>(a, row, i < sp.nq);
     const float delta = i < sp.nq ? a.delta[row] : 0.f;
@@ -551,7 +557,7 @@ __global__ __launch_bounds__(NT) void attn_bwd_q(Args a) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const float p = prob<T>(s[r], rs.ref, rs.inv);
-                s[r] = s[r] == -INFINITY ? 0.f : p * (dp[r] - delta);
+                s[r] = s[r] == -INFINITY ? 0.f : p * (NP > 1 ? __builtin_fmaf(dp[r], sign, -delta) : dp[r] - delta);
             }
             if (BIAS && a.dbias) dg.tile(s, j - qw, bins, a.bk.far, lane);
 #pragma unroll

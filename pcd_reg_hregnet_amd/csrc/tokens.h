@@ -124,6 +124,7 @@ template <> struct Chunk<__bf16> {
     u32x4 w;
     __device__ __forceinline__ void zero() { w = u32x4{0, 0, 0, 0}; }
     __device__ __forceinline__ void load(const __bf16 *p) { w = *reinterpret_cast<const u32x4_m *>(p); }
+    __device__ __forceinline__ void negate() { w ^= 0x80008000u; }
     __device__ __forceinline__ void pieces(bf16x8 (&p)[1]) const { p[0] = __builtin_bit_cast(bf16x8, w); }
     __device__ __forceinline__ float dot(const Chunk &o) const {
         float s = 0.f;
@@ -139,6 +140,7 @@ template <> struct Chunk<float> {
         a = *reinterpret_cast<const f32x4_m *>(p);
         b = *reinterpret_cast<const f32x4_m *>(p + 4);
     }
+    __device__ __forceinline__ void negate() { a = -a, b = -b; }
     __device__ __forceinline__ void pieces(bf16x8 (&p)[3]) const {
         const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
         to_pieces<3>(x, p);
