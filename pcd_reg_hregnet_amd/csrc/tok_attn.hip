@@ -34,12 +34,12 @@ struct Buckets {
 struct Args {
     const void *q, *k, *v, *out_r, *dout;
     void *out, *rest, *dq, *dk, *dv, *dbias;
-    float *lse, *delta, *bins;
+    float *lse, *delta, *bins, *part, *sums;
     const int *q_len, *k_len;
     const uint8_t *key_mask;
     const void *bias;
     int64_t qs[3], ks[3], vs[3], os[3], dos[3], mask_sb;
-    int B, Nq, Nk, H, Hk, D, causal, align_end, bias_f32;
+    int B, Nq, Nk, H, Hk, D, causal, align_end, bias_f32, splits;
     float scale;
     Buckets bk;
 };
@@ -291,6 +291,224 @@ __global__ __launch_bounds__(NT) void attn_fwd(Args a) {
             }
         if (a.lse && half == 0) save_sum<T>(a, ((size_t)w.b * a.H + w.h) * a.Nq + i, any, m, l, inv);
     }
+}
+
+// ------------------------------------------------------- forward, keys split --
+
+// Few rows, many keys: a workgroup takes 32 rows of one key head (row r is token r / G, head r % G
+// of the group, so a token's G heads share every key that is read) and one run of the keys; its
+// four waves take 32 keys each in turn and join in LDS, the runs join in attn_join.  Each wave stages
+// its own keys, then its own values, in its own LDS, without a barrier; the next tile is on its way
+// in registers.  Bound by the bytes of the cache.
+template <class T, int DP>
+struct WaveStage {
+    static constexpr int CPR = DP / 8, N = 32 * CPR / 64, NP = Elem<T>::NP, PLANE = 32 * DP;
+    Chunk<T> c[N];
+    __device__ __forceinline__ void load(const T *base, int64_t ld, int row0, int valid, int D, const uint8_t *mask, int lane) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const int id = lane + u * 64, r = row0 + id / CPR, d = id % CPR * 8;
+            if (r < valid && d < D && (!mask || mask[r])) c[u].load(base + (int64_t)r * ld + d);
+            else c[u].zero();
+        }
+    }
+    __device__ __forceinline__ void store(uint16_t *t, int lane) const {
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const int id = lane + u * 64;
+            bf16x8 p[NP];
+            c[u].pieces(p);
+#pragma unroll
+            for (int s = 0; s < NP; ++s)
+                *reinterpret_cast<u32x4_m *>(t + s * PLANE + tile_at<DP>(id / CPR, id % CPR)) = __builtin_bit_cast(u32x4, p[s]);
+        }
+    }
+};
+
+// one row's result: sums over its keys, written as out (and what training keeps)
+template <class T>
+__device__ __forceinline__ void finish_row(const Args &a, int b, int i, int h, int col, const f32x4 &o, float m, float l) {
+    const bool any = l != 0.f;  // (a NaN sum stays NaN)
+    const float inv = any ? 1.f / l : 0.f;
+    float x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = any ? o[e] * inv : 0.f;
+    store4(static_cast<T *>(a.out) + b * a.os[0] + (int64_t)i * a.os[1] + h * a.os[2] + col, x[0], x[1], x[2], x[3]);
+    if constexpr (Elem<T>::NP == 1) {
+        if (a.rest)
+            store4(static_cast<T *>(a.rest) + (((int64_t)b * a.Nq + i) * a.H + h) * a.D + col, x[0] - (float)(T)x[0],
+                   x[1] - (float)(T)x[1], x[2] - (float)(T)x[2], x[3] - (float)(T)x[3]);
+    }
+    if (a.lse && col == 0) save_sum<T>(a, ((size_t)b * a.H + h) * a.Nq + i, any, m, l, inv);
+}
+
+template <class T, int DP, bool BIAS>
+__global__ __launch_bounds__(NT) void attn_split(Args a) {
+    constexpr int NP = Elem<T>::NP, PLANE = 32 * DP, OLD = DP + 4;  // OLD: a joined row's step in LDS
+    extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
+    __shared__ float ml[4][2][32];
+    __shared__ uint8_t lut[BIAS ? MAX_BINS : 1];
+    const int G = a.H / a.Hk, R = a.Nq * G, tiles = (R + 31) / 32;
+    const Where w = where(a.Hk, tiles * a.splits);  // the splits of a tile are neighbours of its keys' others
+    const int split = w.tile % a.splits, tile = w.tile / a.splits;
+    const Span sp = span_of(a, w.b);
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
+    const int r = tile * 32 + (lane & 31), i = r / G, h = w.h * G + r % G;
+    const bool there = r < R && i < sp.nq;
+    const T *K = static_cast<const T *>(a.k) + w.b * a.ks[0] + w.h * a.ks[2];
+    const T *V = static_cast<const T *>(a.v) + w.b * a.vs[0] + w.h * a.vs[2];
+    const uint8_t *mask = a.key_mask ? a.key_mask + w.b * a.mask_sb : nullptr;
+    uint16_t *buf = lds + wave * NP * PLANE;
+    float left = 0.f, right = 0.f;  // the bias beyond the far offsets
+    if constexpr (BIAS) {
+        for (int o = threadIdx.x; o <= 2 * a.bk.far; o += NT) lut[o] = bucket_of(a.bk, o - a.bk.far);
+        const int hb = r < R ? h : 0;
+        left = bias_at(a, bucket_of(a.bk, -a.bk.far), hb) * LOG2E;
+        right = bias_at(a, bucket_of(a.bk, a.bk.far), hb) * LOG2E;
+        __syncthreads();
+    }
+    bf16x8 qf[DP / 16][NP];
+    load_row<T, DP>(static_cast<const T *>(a.q) + w.b * a.qs[0] + (int64_t)i * a.qs[1] + h * a.qs[2], there, a.D, lane, qf);
+    const float scale2 = a.scale * LOG2E;
+    f32x16 acc[DP / 32];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) acc[d] = zero16();
+    float m = -INFINITY, l = 0.f;
+
+    // keys that some row of the tile sees, in `splits` runs of whole 128
+    const int first_pos = tile * 32 / G + sp.start, last_i = min((tile * 32 + 31) / G, sp.nq - 1);
+    const int kend = tile * 32 / G >= sp.nq ? 0 : a.causal ? min(sp.nk, max(last_i + sp.start + 1, 0)) : sp.nk;
+    const int run = ((kend + a.splits - 1) / a.splits + 127) / 128 * 128;
+    const int j_end = min(kend, (split + 1) * run);
+    int j0 = split * run + 32 * wave;
+    WaveStage<T, DP> sk, sv;
+    if (j0 < j_end) {
+        sk.load(K, a.ks[1], j0, sp.nk, a.D, mask, lane);
+        sv.load(V, a.vs[1], j0, sp.nk, a.D, mask, lane);
+    }
+    for (; j0 < j_end; j0 += 128) {
+        sk.store(buf, lane);
+        if (j0 + 128 < j_end) sk.load(K, a.ks[1], j0 + 128, sp.nk, a.D, mask, lane);
+        wave_sync();
+        f32x16 s = zero16();
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) {
+            bf16x8 kf[NP];
+            row_frag<DP>(buf, PLANE, 0, c, lane, kf);
+            mma<NP>(s, kf, qf[c]);
+        }
+        const int kpos = j0 - (i + sp.start);
+        const bool edge = mask || j0 + 32 > sp.nk || (a.causal && j0 + 31 > first_pos);
+        const bool near = BIAS && __any(kpos + 31 > -a.bk.far && kpos < a.bk.far);
+        float top = m;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int kr = 8 * (e >> 2) + 4 * half + (e & 3);
+            float x = s[e] * scale2;
+            if constexpr (BIAS) {
+                if (near) x += bias_at(a, lut[min(max(kpos + kr, -a.bk.far), a.bk.far) + a.bk.far], r < R ? h : 0) * LOG2E;
+                else x += kpos < 0 ? left : right;
+            }
+            if (edge) {
+                const bool keep = j0 + kr < sp.nk && (!a.causal || kpos + kr <= 0) && (!mask || mask[min(j0 + kr, sp.nk - 1)]);
+                x = keep ? x : -INFINITY;
+            }
+            s[e] = x;
+            top = fmaxf(top, x);
+        }
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float ref = top == -INFINITY ? 0.f : top;
+        if (__any(top != m)) {
+            const float shrink = __builtin_amdgcn_exp2f(m - ref);
+            l *= shrink;
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[d][e] *= shrink;
+            m = top;
+        }
+        wave_sync();  // the keys are read
+        sv.store(buf, lane);
+        if (j0 + 128 < j_end) sv.load(V, a.vs[1], j0 + 128, sp.nk, a.D, mask, lane);
+        wave_sync();
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            float p[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                p[e] = __builtin_amdgcn_exp2f(s[8 * c + e] - ref);
+                l += p[e];
+            }
+            bf16x8 pf[NP];
+            to_pieces<NP>(p, pf);
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) {
+                bf16x8 vf[NP];
+                col_frag<DP>(buf, PLANE, 16 * c, 32 * d, lane, vf);
+                mma<NP>(acc[d], vf, pf);
+            }
+        }
+        wave_sync();  // the values are read
+    }
+
+    // join the waves: every one scales its sums to the common maximum, four rows' parts are added
+    l += __shfl_xor(l, 32);
+    if (!there) m = -INFINITY, l = 0.f;
+    if (half == 0) ml[wave][0][lane] = m, ml[wave][1][lane] = l;
+    __syncthreads();
+    float *part = reinterpret_cast<float *>(lds);  // [wave][32][OLD]
+    {
+        const int q = lane & 31;
+        const float all = fmaxf(fmaxf(ml[0][0][q], ml[1][0][q]), fmaxf(ml[2][0][q], ml[3][0][q]));
+        const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - all);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+                *reinterpret_cast<f32x4_m *>(part + (wave * 32 + q) * OLD + 32 * d + 2 * e + 4 * half) =
+                    f32x4{acc[d][e] * f, acc[d][e + 1] * f, acc[d][e + 2] * f, acc[d][e + 3] * f};
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < 32 * DP / 4; e += NT) {
+        const int q = e / (DP / 4), col = e % (DP / 4) * 4, rr = tile * 32 + q;
+        if (rr >= R || col >= a.D) continue;
+        const float all = fmaxf(fmaxf(ml[0][0][q], ml[1][0][q]), fmaxf(ml[2][0][q], ml[3][0][q]));
+        f32x4 o{0.f, 0.f, 0.f, 0.f};
+        float sum = 0.f;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+            o += *reinterpret_cast<const f32x4_m *>(part + (v * 32 + q) * OLD + col);
+            sum += ml[v][0][q] == -INFINITY ? 0.f : ml[v][1][q] * __builtin_amdgcn_exp2f(ml[v][0][q] - all);
+        }
+        if (a.splits == 1) {
+            finish_row<T>(a, w.b, rr / G, w.h * G + rr % G, col, o, all, sum);
+        } else {
+            const size_t at = (((size_t)w.b * a.Hk + w.h) * R + rr) * a.splits + split;
+            *reinterpret_cast<f32x4_m *>(a.part + at * a.D + col) = o;
+            if (col == 0) a.sums[2 * at] = all, a.sums[2 * at + 1] = sum;
+        }
+    }
+}
+
+// out of the runs' partial results: 32 lanes a row, runs in order
+template <class T>
+__global__ __launch_bounds__(NT) void attn_join(Args a) {
+    const int G = a.H / a.Hk, R = a.Nq * G;
+    const int64_t row = (int64_t)blockIdx.x * (NT / 32) + threadIdx.x / 32;
+    const int col = threadIdx.x % 32 * 4;
+    if (row >= (int64_t)a.B * a.Hk * R || col >= a.D) return;
+    const int r = row % R, hk = row / R % a.Hk, b = row / R / a.Hk;
+    const float *sums = a.sums + 2 * row * a.splits, *part = a.part + row * a.splits * a.D + col;
+    float all = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) all = fmaxf(all, sums[2 * s]);
+    f32x4 o{0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f;
+    for (int s = 0; s < a.splits; ++s) {
+        const float f = sums[2 * s] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sums[2 * s] - all);
+        o += *reinterpret_cast<const f32x4_m *>(part + (int64_t)s * a.D) * f;
+        sum += sums[2 * s + 1] * f;
+    }
+    finish_row<T>(a, b, r / G, hk * G + r % G, col, o, all, sum);
 }
 
 // ---------------------------------------------------------------------- backward --
@@ -635,6 +853,7 @@ int take(const hreg_tok_attn_t *p, Args &a) {
     if (p->B < 0 || p->Nq < 0 || p->Nk < 0 || p->H < 1 || p->Hk < 1 || p->H % p->Hk) return HREG_ERR_INVALID;
     if (p->D < 8 || p->D > 128 || p->D % 8) return HREG_ERR_UNSUPPORTED;
     if ((int64_t)p->B * p->H * (row_tiles(p->Nq) + 1) > INT32_MAX || (int64_t)p->B * p->H * (row_tiles(p->Nk) + 1) > INT32_MAX ||
+        (int64_t)p->Nq * (p->H / p->Hk) > (1 << 30) ||
         p->Nq > (1 << 30) || p->Nk > (1 << 30))
         return HREG_ERR_UNSUPPORTED;
     const int es = p->dtype == HREG_TOK_F32 ? 4 : 2;
@@ -681,6 +900,16 @@ int launch(K *kernel, int grid, size_t lds, void *stream, const Args &a) {
 
 template <class T, int DP, bool BIAS>
 int fwd(const Args &a, void *stream) {
+    if (a.splits) {
+        const int R = a.Nq * (a.H / a.Hk);
+        const size_t tile = (size_t)4 * Elem<T>::NP * 32 * DP * 2, join = (size_t)4 * 32 * (DP + 4) * 4;
+        const int rc = launch(attn_split<T, DP, BIAS>, a.B * a.Hk * ((R + 31) / 32) * a.splits, tile > join ? tile : join, stream, a);
+        if (rc != HREG_OK || a.splits == 1) return rc;
+        const int64_t rows = (int64_t)a.B * a.H * a.Nq;
+        hipLaunchKernelGGL(attn_join<T>, dim3((rows + NT / 32 - 1) / (NT / 32)), dim3(NT), 0, as_stream(stream), a);
+        HREG_CHECK_LAUNCH();
+        return HREG_OK;
+    }
     constexpr int KT = sizeof(T) == 2 || DP == 32 ? 64 : 32;
     const size_t lds = (size_t)2 * Elem<T>::NP * KT * DP * 2 + (BIAS ? (2 * a.bk.far + 1) * 4 : 0);
     return launch(attn_fwd<T, DP, KT, BIAS>, a.B * a.H * row_tiles(a.Nq), lds, stream, a);
@@ -722,6 +951,19 @@ int by_type(const hreg_tok_attn_t *p, const Args &a, void *stream) {
     return a.bias ? by_width<__bf16, true, BACK>(a, stream) : by_width<__bf16, false, BACK>(a, stream);
 }
 
+// 0: the row kernel; else the number of runs of the split kernel.  Measured (us, row / split kernel):
+int split_of(const hreg_tok_attn_t *p) {
+    const int64_t R = (int64_t)p->Nq * (p->H / p->Hk), tiles = (int64_t)p->B * p->Hk * ((R + 31) / 32);
+    const int64_t rows = (int64_t)p->B * p->H * row_tiles(p->Nq);
+    if (tiles == 0 || (rows >= 256 && R > 32)) return 0;
+    int64_t s = (1024 + tiles - 1) / tiles, most = (p->Nk + 255) / 256;
+    s = s < most ? s : most;
+    return s < 1 ? 1 : s > 256 ? 256 : (int)s;
+}
+size_t part_floats(const hreg_tok_attn_t *p, int splits) {  // results, then maxima and sums
+    return splits > 1 ? (size_t)p->B * p->H * p->Nq * splits : 0;
+}
+
 size_t delta_bytes(const hreg_tok_attn_t *p) { return ((size_t)p->B * p->H * p->Nq * 4 + 255) / 256 * 256; }
 
 }  // namespace
@@ -729,7 +971,8 @@ size_t delta_bytes(const hreg_tok_attn_t *p) { return ((size_t)p->B * p->H * p->
 extern "C" {
 
 size_t hreg_tok_attn_ws_bytes(const hreg_tok_attn_t *p, int backward) {
-    if (!p || p->B < 0 || p->Nq < 0 || p->H < 1 || !backward) return 0;
+    if (!p || p->B < 0 || p->Nq < 0 || p->Nk < 0 || p->H < 1 || p->Hk < 1 || p->H % p->Hk || p->D < 1) return 0;
+    if (!backward) return part_floats(p, split_of(p)) * (p->D + 2) * 4;
     return delta_bytes(p) + (p->bias ? (size_t)p->B * p->H * row_tiles(p->Nq) * (2 * (size_t)p->max_distance + 1) * 4 : 0);
 }
 
@@ -737,8 +980,12 @@ int hreg_tok_attn_fwd(const hreg_tok_attn_t *p, void *stream) {
     Args a;
     const int rc = take(p, a);
     if (rc != HREG_OK) return rc;
-    if (p->ws_bytes < hreg_tok_attn_ws_bytes(p, 0)) return HREG_ERR_INVALID;
     if (a.B == 0 || a.Nq == 0) return HREG_OK;
+    const size_t need = hreg_tok_attn_ws_bytes(p, 0);
+    if (p->ws_bytes < need || (need && (!p->ws || reinterpret_cast<uintptr_t>(p->ws) % 256))) return HREG_ERR_INVALID;
+    a.splits = split_of(p);
+    a.part = static_cast<float *>(p->ws);
+    a.sums = a.part + part_floats(p, a.splits) * p->D;
     return by_type<false>(p, a, stream);
 }
 
