@@ -24,7 +24,20 @@ using namespace hreg_tok;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int NT = 256;          // threads a workgroup
 constexpr int ROWS = 128;        // rows a workgroup owns: 32 a wave
+constexpr int CUS = 256;
 constexpr int MAX_BINS = 2049;   // offsets -max_distance .. max_distance with max_distance <= 1024
+
+// Rows of a tile that goes through LDS, and the waves a SIMD that the registers are cut to.  Two
+// waves a SIMD hide each other's waits (2 x 4096 x 16 heads x 128 bf16, us: forward 387 with two, 572
+// with one), so long as nothing spills: f32 backward at 128 columns keeps 400 registers and one wave
+// (690 against 1770).  64 rows halve the barriers of 32, but at 128 columns the backward pass has no
+// registers for them (bf16, 746 us with 32, 1939 with 64).
+template <class T, int DP>
+struct Shape {
+    static constexpr bool F32 = Elem<T>::NP > 1;
+    static constexpr int FWD_KEYS = F32 && DP > 32 ? 32 : 64, BWD_ROWS = F32 && DP > 32 ? 32 : DP > 64 ? 32 : 64;
+    static constexpr int BWD_WAVES = F32 && DP > 64 ? 1 : 2;
+};
 
 struct Buckets {
     int n, far, both, exact, nthresh;
@@ -39,7 +52,7 @@ struct Args {
     const uint8_t *key_mask;
     const void *bias;
     int64_t qs[3], ks[3], vs[3], os[3], dos[3], mask_sb;
-    int B, Nq, Nk, H, Hk, D, causal, align_end, bias_f32, splits;
+    int B, Nq, Nk, H, Hk, D, causal, align_end, bias_f32, splits, groups, tile_rows;
     float scale;
     Buckets bk;
 };
@@ -61,11 +74,23 @@ __device__ __forceinline__ float bias_at(const Args &a, int b, int h) {
     return a.bias_f32 ? static_cast<const float *>(a.bias)[at] : (float)static_cast<const __bf16 *>(a.bias)[at];
 }
 
-// this workgroup's batch entry, head and tile: neighbours share keys, and so an L2
+// This workgroup's batch entry, head and tile.  Workgroups go round the 8 XCDs: each XCD takes whole
+// heads, so that tiles that read the same keys share an L2, and walks them tile by tile over its
+// heads, so that the long tiles of a causal call (callers number them first) all start early.
 struct Where { int b, h, tile; };
-__device__ __forceinline__ Where where(int heads, int tiles) {
-    const int n = xcd_block(blockIdx.x, gridDim.x);
-    return {n / (tiles * heads), n / tiles % heads, n % tiles};
+__device__ __forceinline__ Where where(int batch, int heads, int tiles) {
+    const int all = batch * heads;
+    int head, tile;
+    if (all % 8 == 0) {
+        const int k = blockIdx.x >> 3, mine = all >> 3;
+        head = (blockIdx.x & 7) * mine + k % mine;
+        tile = k / mine;
+    } else {
+        const int n = xcd_block(blockIdx.x, gridDim.x);
+        head = n / tiles;
+        tile = n % tiles;
+    }
+    return {head / heads, head % heads, tile};
 }
 
 struct Span { int nq, nk, start; };  // valid rows, valid keys, position of query 0
@@ -77,30 +102,88 @@ __device__ __forceinline__ Span span_of(const Args &a, int b) {
     return s;
 }
 
-// One [R][DP] tile between global memory, registers and LDS pieces.  Rows at or beyond `valid`,
-// rows whose mask is 0 and columns at or beyond D are zero, whatever memory holds there.
+// Two [R][DP] tiles (keys and values, or queries and output gradients) on their way from global
+// memory into LDS while the ones before are used: issue() starts, land() waits and makes them whole.
+// bf16 goes straight into LDS (16 bytes a lane, two buffers, one barrier a tile); f32 goes through
+// registers, where it is cut into its pieces (one buffer, two barriers).  Rows at or beyond `valid`,
+// rows whose mask is 0 and columns at or beyond D are zero, whatever memory holds there; they are
+// never read.
 template <class T, int DP, int R>
-struct Stage {
-    static constexpr int CPR = DP / 8, N = R * CPR / NT, NP = Elem<T>::NP, PLANE = R * DP;
+struct Tiles {
+    static constexpr int CPR = DP / 8, N = R * CPR / NT, NP = Elem<T>::NP, PLANE = R * DP, TILE = NP * PLANE;
+    static constexpr bool DIRECT = NP == 1;
+    static constexpr size_t BYTES = (size_t)(DIRECT ? 2 : 1) * 2 * TILE * 2;
     static_assert(R * CPR % NT == 0, "tile");
-    Chunk<T> c[N];
-    __device__ __forceinline__ void load(const T *base, int64_t ld, int row0, int valid, int D, const uint8_t *mask) {
-#pragma unroll
-        for (int u = 0; u < N; ++u) {
-            const int id = threadIdx.x + u * NT, r = row0 + id / CPR, d = id % CPR * 8;
-            if (r < valid && d < D && (!mask || mask[r])) c[u].load(base + (int64_t)r * ld + d);
-            else c[u].zero();
+    uint16_t *lds;
+    Chunk<T> cx[DIRECT ? 1 : N], cy[DIRECT ? 1 : N];
+    int buf;  // the buffer that is used
+
+    __device__ __forceinline__ const uint16_t *x() const { return lds + buf * 2 * TILE; }
+    __device__ __forceinline__ const uint16_t *y() const { return x() + TILE; }
+
+    __device__ __forceinline__ void init(uint16_t *at, int D) {
+        lds = at;
+        buf = DIRECT ? 1 : 0;
+        if (DIRECT && D < DP) {  // the columns that no load writes
+            for (int e = threadIdx.x; e < 4 * TILE / 8; e += NT) reinterpret_cast<u32x4_m *>(at)[e] = u32x4{0, 0, 0, 0};
+            __syncthreads();
         }
     }
-    __device__ __forceinline__ void store(uint16_t *t) const {
+    __device__ __forceinline__ void issue(const T *px, int64_t ldx, const T *py, int64_t ldy, int row0, int valid, int D,
+                                          const uint8_t *mask) {
+        const bool whole = D == DP && row0 + R <= valid && !mask;  // (uniform)
 #pragma unroll
         for (int u = 0; u < N; ++u) {
-            const int id = threadIdx.x + u * NT;
-            bf16x8 p[NP];
-            c[u].pieces(p);
+            const int id = threadIdx.x + u * NT, tr = id / CPR, r = row0 + tr;
+            const int d = (DIRECT ? (id % CPR) ^ swz<DP>(tr) : id % CPR) * 8;
+            const bool ok = whole || (r < valid && d < D && (!mask || mask[r]));
+            if constexpr (DIRECT) {
+                const uint16_t *to = lds + (buf ^ 1) * 2 * TILE + (u * NT + (threadIdx.x & ~63)) * 8;
+                if (whole || ok) {
+                    global_to_lds(px + (int64_t)r * ldx + d, to);
+                    global_to_lds(py + (int64_t)r * ldy + d, to + TILE);
+                }
+            } else if (ok) {
+                cx[u].load(px + (int64_t)r * ldx + d);
+                cy[u].load(py + (int64_t)r * ldy + d);
+            } else {
+                cx[u].zero();
+                cy[u].zero();
+            }
+        }
+    }
+    __device__ __forceinline__ void land(int row0, int valid, const uint8_t *mask) {
+        if constexpr (DIRECT) {
+            buf ^= 1;
+            __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's rows are there
+            __syncthreads();                     // every wave's are, and the other buffer is free
+            if (mask || row0 + R > valid) {
+                uint16_t *to = lds + buf * 2 * TILE;
 #pragma unroll
-            for (int s = 0; s < NP; ++s)
-                *reinterpret_cast<u32x4_m *>(t + s * PLANE + tile_at<DP>(id / CPR, id % CPR)) = __builtin_bit_cast(u32x4, p[s]);
+                for (int u = 0; u < N; ++u) {
+                    const int id = threadIdx.x + u * NT, r = row0 + id / CPR;
+                    if (r >= valid || (mask && !mask[r])) {
+                        *reinterpret_cast<u32x4_m *>(to + id * 8) = u32x4{0, 0, 0, 0};
+                        *reinterpret_cast<u32x4_m *>(to + TILE + id * 8) = u32x4{0, 0, 0, 0};
+                    }
+                }
+                __syncthreads();
+            }
+        } else {
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                const int id = threadIdx.x + u * NT, at = tile_at<DP>(id / CPR, id % CPR);
+                bf16x8 p[NP];
+                cx[u].pieces(p);
+#pragma unroll
+                for (int s = 0; s < NP; ++s) *reinterpret_cast<u32x4_m *>(lds + s * PLANE + at) = __builtin_bit_cast(u32x4, p[s]);
+                cy[u].pieces(p);
+#pragma unroll
+                for (int s = 0; s < NP; ++s)
+                    *reinterpret_cast<u32x4_m *>(lds + TILE + s * PLANE + at) = __builtin_bit_cast(u32x4, p[s]);
+            }
+            __syncthreads();
         }
     }
 };
@@ -150,37 +233,74 @@ __device__ __forceinline__ float prob(float s, float ref, float inv) {
 
 // ---------------------------------------------------------------------- forward --
 
-// Scores of 32 keys (rows) against the wave's 32 queries (columns) in units of log2, masked.
-// kpos = key index of row 0 - position of this lane's query, krow = key index of row 0.
-template <bool BIAS>
-__device__ __forceinline__ void finish_scores(const Args &a, f32x16 &s, float scale2, const float *tab, int far,
-                                              int krow, int kpos, int nk, bool edge, const uint8_t *mask, int half) {
+// One head's bias over the offsets -far - PAD .. far + PAD, in units of log2, in LDS.  A 32 x 32
+// tile of scores touches 63 offsets: if all lie beyond far it takes one value, else its offsets are
+// inside the table without clamping (lane and register steps are constant: paired LDS reads).
+constexpr int PAD = 64;
+__device__ __forceinline__ int table_size(int far) { return 2 * (far + PAD) + 1; }
+__device__ __forceinline__ void fill_table(const Args &a, float *tab, int h) {
+    const int far = a.bk.far;
+    for (int o = threadIdx.x; o < table_size(far); o += NT)
+        tab[o] = bias_at(a, bucket_of(a.bk, min(max(o - far - PAD, -far), far)), h) * LOG2E;
+}
+
+// Scores of 32 keys (rows) against the wave's 32 queries (columns) in units of log2: s = s * scale2 +
+// bias.  base = first key - first query's position, kpos = first key - this lane's query's.
+__device__ __forceinline__ void add_bias(f32x16 &s, float scale2, const float *tab, int far, int base, int kpos, int half) {
+    if (base - 31 >= far || base + 31 <= -far) {
+        const float b = tab[base < 0 ? 0 : 2 * (far + PAD)];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const int kr = 8 * (r >> 2) + 4 * half + (r & 3);
-        float x = s[r] * scale2;
-        if constexpr (BIAS) x += tab[min(max(kpos + kr, -far), far) + far];
-        if (edge) {
-            const bool keep = krow + kr < nk && (!a.causal || kpos + kr <= 0) && (!mask || mask[min(krow + kr, nk - 1)]);
-            x = keep ? x : -INFINITY;
-        }
-        s[r] = x;
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], scale2, b);
+    } else {
+        const float *t = tab + (kpos + 4 * half + far + PAD);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], scale2, t[8 * (r >> 2) + (r & 3)]);
     }
 }
 
-// the bias of one head over all clamped offsets, in units of log2
-__device__ __forceinline__ void fill_table(const Args &a, float *tab, int h) {
-    for (int o = threadIdx.x; o <= 2 * a.bk.far; o += NT) tab[o] = bias_at(a, bucket_of(a.bk, o - a.bk.far), h) * LOG2E;
+// keys that the lane's query does not see: -inf.  krow = index of the first key; seen: bit k = key
+// krow + k exists and is not masked
+__device__ __forceinline__ void hide(const Args &a, f32x16 &s, int kpos, uint32_t seen, int half) {
+    if (a.causal) {  // the keys up to the query's own position
+        const int n = min(max(1 - kpos, 0), 32);
+        seen &= n == 32 ? ~0u : (1u << n) - 1;
+    }
+    seen >>= 4 * half;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = seen >> (8 * (r >> 2) + (r & 3)) & 1 ? s[r] : -INFINITY;
+}
+__device__ __forceinline__ uint32_t seen_keys(int krow, int nk, const uint8_t *mask) {
+    if (!mask) return krow + 32 <= nk ? ~0u : krow >= nk ? 0u : (1u << (nk - krow)) - 1;
+    const int k = krow + (threadIdx.x & 31);
+    return (uint32_t)__ballot(k < nk && mask[min(k, nk - 1)]);
 }
 
+// one row's result: sums over its keys, written as out (and what training keeps)
+template <class T>
+__device__ __forceinline__ void finish_row(const Args &a, int b, int i, int h, int col, const f32x4 &o, float m, float l) {
+    const bool any = l != 0.f;  // (a NaN sum stays NaN)
+    const float inv = any ? 1.f / l : 0.f;
+    float x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = any ? o[e] * inv : 0.f;
+    store4(static_cast<T *>(a.out) + b * a.os[0] + (int64_t)i * a.os[1] + h * a.os[2] + col, x[0], x[1], x[2], x[3]);
+    if constexpr (Elem<T>::NP == 1) {
+        if (a.rest)
+            store4(static_cast<T *>(a.rest) + (((int64_t)b * a.Nq + i) * a.H + h) * a.D + col, x[0] - (float)(T)x[0],
+                   x[1] - (float)(T)x[1], x[2] - (float)(T)x[2], x[3] - (float)(T)x[3]);
+    }
+    if (a.lse && col == 0) save_sum<T>(a, ((size_t)b * a.H + h) * a.Nq + i, any, m, l, inv);
+}
+
+// 128 rows of one head, 32 a wave: the columns of its scores are its queries.
 template <class T, int DP, int KT, bool BIAS>
-__global__ __launch_bounds__(NT) void attn_fwd(Args a) {
+__global__ __launch_bounds__(NT, 2) void attn_fwd(Args a) {
     constexpr int NP = Elem<T>::NP, MT = KT / 32, PLANE = KT * DP;
     extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
-    uint16_t *kt = lds, *vt = lds + NP * PLANE;
-    float *tab = reinterpret_cast<float *>(lds + 2 * NP * PLANE);
+    typedef Tiles<T, DP, KT> KV;
+    float *tab = reinterpret_cast<float *>(reinterpret_cast<char *>(lds) + KV::BYTES);
     const int tiles = (a.Nq + ROWS - 1) / ROWS;
-    const Where w = where(a.H, tiles);
+    const Where w = where(a.B, a.H, tiles);
     const Span sp = span_of(a, w.b);
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
     const int q0 = (tiles - 1 - w.tile) * ROWS, i = q0 + 32 * wave + (lane & 31);
@@ -190,10 +310,12 @@ __global__ __launch_bounds__(NT) void attn_fwd(Args a) {
     const uint8_t *mask = a.key_mask ? a.key_mask + w.b * a.mask_sb : nullptr;
     if constexpr (BIAS) fill_table(a, tab, w.h);
 
+    // without a bias scores stay as the products give them and their running maximum with them
+    // (q takes a negative scale's sign): one fused multiply-add before each exponential
     bf16x8 qf[DP / 16][NP];
     load_row<T, DP>(static_cast<const T *>(a.q) + w.b * a.qs[0] + (int64_t)i * a.qs[1] + w.h * a.qs[2], i < sp.nq, a.D,
-                    lane, qf);
-    const float scale2 = a.scale * LOG2E;
+                    lane, qf, a.scale < 0.f);
+    const float scale2 = fmaxf(fabsf(a.scale) * LOG2E, 1e-37f), unit = BIAS ? 1.f : scale2;
     f32x16 acc[DP / 32];
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) acc[d] = zero16();
@@ -202,25 +324,17 @@ __global__ __launch_bounds__(NT) void attn_fwd(Args a) {
     // keys that some row of the workgroup sees
     const int last = min(q0 + ROWS, sp.nq) - 1;
     const int kend = last < q0 ? 0 : a.causal ? min(sp.nk, max(last + sp.start + 1, 0)) : sp.nk;
-    Stage<T, DP, KT> sk, sv;
-    if (kend > 0) {
-        sk.load(K, a.ks[1], 0, sp.nk, a.D, mask);
-        sv.load(V, a.vs[1], 0, sp.nk, a.D, mask);
-    }
+    KV kv;
+    kv.init(lds, a.D);
+    if (kend > 0) kv.issue(K, a.ks[1], V, a.vs[1], 0, sp.nk, a.D, mask);
     for (int j0 = 0; j0 < kend; j0 += KT) {
-        __syncthreads();
-        sk.store(kt);
-        sv.store(vt);
-        __syncthreads();
-        if (j0 + KT < kend) {
-            sk.load(K, a.ks[1], j0 + KT, sp.nk, a.D, mask);
-            sv.load(V, a.vs[1], j0 + KT, sp.nk, a.D, mask);
-        }
+        kv.land(j0, sp.nk, mask);
+        const uint16_t *kt = kv.x(), *vt = kv.y();
+        if (j0 + KT < kend) kv.issue(K, a.ks[1], V, a.vs[1], j0 + KT, sp.nk, a.D, mask);
         const int qw = q0 + 32 * wave + sp.start;  // position of the wave's first query
-        if (a.causal && j0 > qw + 31) continue;
+        if (a.causal && j0 > qw + 32 - 1) continue;
         const bool edge = mask || j0 + KT > sp.nk || (a.causal && j0 + KT - 1 > qw);
         f32x16 s[MT];
-        float top = m;
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
             s[t] = zero16();
@@ -230,15 +344,20 @@ __global__ __launch_bounds__(NT) void attn_fwd(Args a) {
                 row_frag<DP>(kt, PLANE, 32 * t, c, lane, kf);
                 mma<NP>(s[t], kf, qf[c]);
             }
-            finish_scores<BIAS>(a, s[t], scale2, tab, a.bk.far, j0 + 32 * t, j0 + 32 * t - (i + sp.start), sp.nk, edge,
-                                mask, half);
+        }
+        const int kpos = j0 - (i + sp.start);
+        float top = m;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            if constexpr (BIAS) add_bias(s[t], scale2, tab, a.bk.far, j0 + 32 * t - qw, kpos + 32 * t, half);
+            if (edge) hide(a, s[t], kpos + 32 * t, seen_keys(j0 + 32 * t, sp.nk, mask), half);
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
         }
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float ref = top == -INFINITY ? 0.f : top;  // a row without a key so far keeps sums of 0
+        const float ref = top == -INFINITY ? 0.f : top * unit;  // a row without a key so far keeps sums of 0
         if (__any(top != m)) {
-            const float shrink = __builtin_amdgcn_exp2f(m - ref);
+            const float shrink = __builtin_amdgcn_exp2f(__builtin_fmaf(m, unit, -ref));
             l *= shrink;
 #pragma unroll
             for (int d = 0; d < DP / 32; ++d)
@@ -247,15 +366,19 @@ __global__ __launch_bounds__(NT) void attn_fwd(Args a) {
             m = top;
         }
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[t][r] = __builtin_amdgcn_exp2f(BIAS ? s[t][r] - ref : __builtin_fmaf(s[t][r], unit, -ref));
+                l += s[t][r];
+            }
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 float p[8];
 #pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    p[r] = __builtin_amdgcn_exp2f(s[t][8 * c + r] - ref);
-                    l += p[r];
-                }
+                for (int r = 0; r < 8; ++r) p[r] = s[t][8 * c + r];
                 bf16x8 pf[NP];
                 to_pieces<NP>(p, pf);
 #pragma unroll
@@ -265,32 +388,18 @@ __global__ __launch_bounds__(NT) void attn_fwd(Args a) {
                     mma<NP>(acc[d], vf, pf);
                 }
             }
-        }
     }
     l += __shfl_xor(l, 32);
-    const bool any = i < sp.nq && l != 0.f;  // (a NaN sum stays NaN)
-    const float inv = any ? 1.f / l : 0.f;
-    if (i < a.Nq) {
-        T *o = static_cast<T *>(a.out) + w.b * a.os[0] + (int64_t)i * a.os[1] + w.h * a.os[2];
-        T *rest = a.rest ? static_cast<T *>(a.rest) + (((int64_t)w.b * a.Nq + i) * a.H + w.h) * a.D : nullptr;
+    if (i >= a.Nq) return;
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
+    for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const int col = 32 * d + 2 * r + 4 * half;
-                if (col >= a.D) continue;
-                float x[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = any ? acc[d][r + e] * inv : 0.f;
-                store4(o + col, x[0], x[1], x[2], x[3]);
-                if constexpr (NP == 1) {
-                    if (rest)
-                        store4(rest + col, x[0] - (float)(T)x[0], x[1] - (float)(T)x[1], x[2] - (float)(T)x[2],
-                               x[3] - (float)(T)x[3]);
-                }
-            }
-        if (a.lse && half == 0) save_sum<T>(a, ((size_t)w.b * a.H + w.h) * a.Nq + i, any, m, l, inv);
-    }
+        for (int r = 0; r < 16; r += 4) {
+            const int col = 32 * d + 2 * r + 4 * half;
+            if (col < a.D)
+                finish_row<T>(a, w.b, i, w.h, col, f32x4{acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]}, m * unit,
+                              i < sp.nq ? l : 0.f);
+        }
 }
 
 // ------------------------------------------------------- forward, keys split --
@@ -325,23 +434,6 @@ struct WaveStage {
     }
 };
 
-// one row's result: sums over its keys, written as out (and what training keeps)
-template <class T>
-__device__ __forceinline__ void finish_row(const Args &a, int b, int i, int h, int col, const f32x4 &o, float m, float l) {
-    const bool any = l != 0.f;  // (a NaN sum stays NaN)
-    const float inv = any ? 1.f / l : 0.f;
-    float x[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = any ? o[e] * inv : 0.f;
-    store4(static_cast<T *>(a.out) + b * a.os[0] + (int64_t)i * a.os[1] + h * a.os[2] + col, x[0], x[1], x[2], x[3]);
-    if constexpr (Elem<T>::NP == 1) {
-        if (a.rest)
-            store4(static_cast<T *>(a.rest) + (((int64_t)b * a.Nq + i) * a.H + h) * a.D + col, x[0] - (float)(T)x[0],
-                   x[1] - (float)(T)x[1], x[2] - (float)(T)x[2], x[3] - (float)(T)x[3]);
-    }
-    if (a.lse && col == 0) save_sum<T>(a, ((size_t)b * a.H + h) * a.Nq + i, any, m, l, inv);
-}
-
 template <class T, int DP, bool BIAS>
 __global__ __launch_bounds__(NT) void attn_split(Args a) {
     constexpr int NP = Elem<T>::NP, PLANE = 32 * DP, OLD = DP + 4;  // OLD: a joined row's step in LDS
@@ -349,7 +441,7 @@ __global__ __launch_bounds__(NT) void attn_split(Args a) {
     __shared__ float ml[4][2][32];
     __shared__ uint8_t lut[BIAS ? MAX_BINS : 1];
     const int G = a.H / a.Hk, R = a.Nq * G, tiles = (R + 31) / 32;
-    const Where w = where(a.Hk, tiles * a.splits);  // the splits of a tile are neighbours of its keys' others
+    const Where w = where(a.B, a.Hk, tiles * a.splits);  // the splits of a tile are neighbours of its keys' others
     const int split = w.tile % a.splits, tile = w.tile / a.splits;
     const Span sp = span_of(a, w.b);
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
@@ -409,13 +501,11 @@ __global__ __launch_bounds__(NT) void attn_split(Args a) {
                 if (near) x += bias_at(a, lut[min(max(kpos + kr, -a.bk.far), a.bk.far) + a.bk.far], r < R ? h : 0) * LOG2E;
                 else x += kpos < 0 ? left : right;
             }
-            if (edge) {
-                const bool keep = j0 + kr < sp.nk && (!a.causal || kpos + kr <= 0) && (!mask || mask[min(j0 + kr, sp.nk - 1)]);
-                x = keep ? x : -INFINITY;
-            }
             s[e] = x;
-            top = fmaxf(top, x);
         }
+        if (edge) hide(a, s, kpos, seen_keys(j0, sp.nk, mask), half);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, s[e]);
         top = fmaxf(top, __shfl_xor(top, 32));
         const float ref = top == -INFINITY ? 0.f : top;
         if (__any(top != m)) {
@@ -534,15 +624,17 @@ __global__ __launch_bounds__(NT) void attn_delta(Args a) {
     if (threadIdx.x % 16 == 0) a.delta[row] = s;
 }
 
-// dk, dv of 128 keys: every wave keeps 32 keys and walks all rows of all heads that share them,
-// so the sums over a group need no second pass and have one order.
+// dk, dv of 128 keys: every wave keeps 32 keys and walks all rows of all heads that share them, so
+// the sums over a group need no second pass and have one order.  Where that leaves too few
+// workgroups (a.groups) each walks one head, and sum_group adds the heads' f32 results.
 template <class T, int DP, int QT, bool BIAS>
-__global__ __launch_bounds__(NT) void attn_bwd_kv(Args a) {
+__global__ __launch_bounds__(NT, (Shape<T, DP>::BWD_WAVES)) void attn_bwd_kv(Args a) {
     constexpr int NP = Elem<T>::NP, PLANE = QT * DP;
     extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
-    uint16_t *qt = lds, *dt = lds + NP * PLANE;
-    float *lt = reinterpret_cast<float *>(lds + 2 * NP * PLANE), *et = lt + QT, *it = et + QT, *tab = it + QT;
-    const Where w = where(a.Hk, (a.Nk + ROWS - 1) / ROWS);
+    typedef Tiles<T, DP, QT> QD;
+    float *lt = reinterpret_cast<float *>(reinterpret_cast<char *>(lds) + QD::BYTES), *et = lt + QT, *it = et + QT, *tab = it + QT;
+    const Where w0 = where(a.B, a.Hk * a.groups, (a.Nk + ROWS - 1) / ROWS);
+    const Where w{w0.b, w0.h / a.groups, w0.tile};
     const Span sp = span_of(a, w.b);
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
     const int k0 = w.tile * ROWS, j = k0 + 32 * wave + (lane & 31);
@@ -557,8 +649,11 @@ __global__ __launch_bounds__(NT) void attn_bwd_kv(Args a) {
     const float scale2 = a.scale * LOG2E;
     const int first = a.causal ? max(k0 - sp.start, 0) / QT * QT : 0;  // rows before see no key of the tile
     const int G = a.H / a.Hk;
+    QD qd;
+    qd.init(lds, a.D);
+    const int g0 = w0.h % a.groups * (G / a.groups);
     if (k0 < sp.nk)
-        for (int g = 0; g < G; ++g) {
+        for (int g = g0; g < g0 + G / a.groups; ++g) {
             const int h = w.h * G + g;
             const T *Q = static_cast<const T *>(a.q) + w.b * a.qs[0] + h * a.qs[2];
             const T *dO = static_cast<const T *>(a.dout) + w.b * a.dos[0] + h * a.dos[2];
@@ -567,15 +662,9 @@ __global__ __launch_bounds__(NT) void attn_bwd_kv(Args a) {
                 __syncthreads();
                 fill_table(a, tab, h);
             }
-            Stage<T, DP, QT> sq, sd;
-            if (first < sp.nq) {
-                sq.load(Q, a.qs[1], first, sp.nq, a.D, nullptr);
-                sd.load(dO, a.dos[1], first, sp.nq, a.D, nullptr);
-            }
+            if (first < sp.nq) qd.issue(Q, a.qs[1], dO, a.dos[1], first, sp.nq, a.D, nullptr);
             for (int i0 = first; i0 < sp.nq; i0 += QT) {
                 __syncthreads();
-                sq.store(qt);
-                sd.store(dt);
                 if (threadIdx.x < QT) {
                     const int i = i0 + threadIdx.x;
                     const RowSum rs = row_sum_of<T>(a, row0 + i, i < sp.nq);
@@ -583,16 +672,16 @@ __global__ __launch_bounds__(NT) void attn_bwd_kv(Args a) {
                     it[threadIdx.x] = rs.inv;
                     et[threadIdx.x] = i < sp.nq ? a.delta[row0 + i] : 0.f;
                 }
-                __syncthreads();
-                if (i0 + QT < sp.nq) {
-                    sq.load(Q, a.qs[1], i0 + QT, sp.nq, a.D, nullptr);
-                    sd.load(dO, a.dos[1], i0 + QT, sp.nq, a.D, nullptr);
-                }
+                qd.land(i0, sp.nq, nullptr);
+                const uint16_t *qt = qd.x(), *dt = qd.y();
+                if (i0 + QT < sp.nq) qd.issue(Q, a.qs[1], dO, a.dos[1], i0 + QT, sp.nq, a.D, nullptr);
 #pragma unroll
                 for (int t = 0; t < QT / 32; ++t) {
                     const int p0 = i0 + 32 * t + sp.start;  // position of the first query
                     if (a.causal && p0 + 31 < k0 + 32 * wave) continue;
                     const bool edge = a.causal && p0 < k0 + 32 * wave + 31;
+                    const bool near = BIAS && !(k0 + 32 * wave - p0 - 31 >= a.bk.far || k0 + 32 * wave - p0 + 31 <= -a.bk.far);
+                    const float b = BIAS ? tab[k0 + 32 * wave < p0 ? 0 : 2 * (a.bk.far + PAD)] : 0.f;
                     f32x16 s = zero16(), dp = zero16();
 #pragma unroll
                     for (int c = 0; c < DP / 16; ++c) {
@@ -608,9 +697,8 @@ __global__ __launch_bounds__(NT) void attn_bwd_kv(Args a) {
 #pragma unroll
                         for (int r = 0; r < 8; ++r) {
                             const int ir = 8 * (2 * c + (r >> 2)) + 4 * half + (r & 3);
-                            float x = s[8 * c + r] * scale2;
                             const int o = j - (p0 + ir);
-                            if constexpr (BIAS) x += tab[min(max(o, -a.bk.far), a.bk.far) + a.bk.far];
+                            const float x = __builtin_fmaf(s[8 * c + r], scale2, near ? tab[o + a.bk.far + PAD] : b);
                             const bool keep = !edge || o <= 0;
                             p[r] = keep ? prob<T>(x, lt[32 * t + ir], it[32 * t + ir]) : 0.f;
                             ds[r] = keep ? p[r] * (dp[8 * c + r] - et[32 * t + ir]) : 0.f;
@@ -631,9 +719,25 @@ __global__ __launch_bounds__(NT) void attn_bwd_kv(Args a) {
             }
         }
     if (j < a.Nk) {
+        const float f = a.scale;
+        if (a.groups > 1) {
+            const int64_t at = (((int64_t)w.b * a.Nk + j) * a.H + w.h * G + g0) * a.D;
+            float *ok_ = a.part + at, *ov = a.sums + at;
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const int col = 32 * d + 2 * r + 4 * half;
+                    if (col >= a.D) continue;
+                    store4(ok_ + col, ok ? dk[d][r] * f : 0.f, ok ? dk[d][r + 1] * f : 0.f, ok ? dk[d][r + 2] * f : 0.f,
+                           ok ? dk[d][r + 3] * f : 0.f);
+                    store4(ov + col, ok ? dv[d][r] : 0.f, ok ? dv[d][r + 1] : 0.f, ok ? dv[d][r + 2] : 0.f,
+                           ok ? dv[d][r + 3] : 0.f);
+                }
+            return;
+        }
         const int64_t at = (((int64_t)w.b * a.Nk + j) * a.Hk + w.h) * a.D;
         T *ok_ = static_cast<T *>(a.dk) + at, *ov = static_cast<T *>(a.dv) + at;
-        const float f = a.scale;
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -646,6 +750,19 @@ __global__ __launch_bounds__(NT) void attn_bwd_kv(Args a) {
                        ok ? dv[d][r + 3] : 0.f);
             }
     }
+}
+
+// dk and dv of a group from its heads' parts, in head order
+template <class T>
+__global__ __launch_bounds__(NT) void sum_group(Args a) {
+    const int G = a.H / a.Hk, C = a.D / 4;
+    const int64_t e = (int64_t)blockIdx.x * NT + threadIdx.x, row = e / C;
+    if (row >= (int64_t)a.B * a.Nk * a.Hk) return;
+    const int col = e % C * 4;
+    const float *from = (blockIdx.y ? a.sums : a.part) + row * G * a.D + col;
+    f32x4 s = *reinterpret_cast<const f32x4_m *>(from);
+    for (int g = 1; g < G; ++g) s += *reinterpret_cast<const f32x4_m *>(from + (int64_t)g * a.D);
+    store4(static_cast<T *>(blockIdx.y ? a.dv : a.dk) + row * a.D + col, s[0], s[1], s[2], s[3]);
 }
 
 // The bias gradient of one wave: sums of ds over the diagonals of its 32 x 32 tiles.  Offset
@@ -702,14 +819,14 @@ struct Diagonals {
 
 // dq of 128 rows, and the bias gradient's sums over their diagonals
 template <class T, int DP, int KT, bool BIAS>
-__global__ __launch_bounds__(NT) void attn_bwd_q(Args a) {
+__global__ __launch_bounds__(NT, (Shape<T, DP>::BWD_WAVES)) void attn_bwd_q(Args a) {
     constexpr int NP = Elem<T>::NP, PLANE = KT * DP;
     extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
-    uint16_t *kt = lds, *vt = lds + NP * PLANE;
+    typedef Tiles<T, DP, KT> KV;
     const int W = 2 * a.bk.far + 1;
-    float *tab = reinterpret_cast<float *>(lds + 2 * NP * PLANE);
+    float *tab = reinterpret_cast<float *>(reinterpret_cast<char *>(lds) + KV::BYTES);
     const int tiles = (a.Nq + ROWS - 1) / ROWS;
-    const Where w = where(a.H, tiles);
+    const Where w = where(a.B, a.H, tiles);
     const Span sp = span_of(a, w.b);
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
     const int tile = tiles - 1 - w.tile, q0 = tile * ROWS, i = q0 + 32 * wave + (lane & 31);
@@ -717,10 +834,10 @@ __global__ __launch_bounds__(NT) void attn_bwd_q(Args a) {
     const T *K = static_cast<const T *>(a.k) + w.b * a.ks[0] + hk * a.ks[2];
     const T *V = static_cast<const T *>(a.v) + w.b * a.vs[0] + hk * a.vs[2];
     const uint8_t *mask = a.key_mask ? a.key_mask + w.b * a.mask_sb : nullptr;
-    float *bins = tab + W + wave * W;
+    float *all_bins = tab + table_size(a.bk.far), *bins = all_bins + wave * W;
     if constexpr (BIAS) {
         fill_table(a, tab, w.h);
-        for (int o = threadIdx.x; o < 4 * W; o += NT) tab[W + o] = 0.f;
+        for (int o = threadIdx.x; o < 4 * W; o += NT) all_bins[o] = 0.f;
     }
     bf16x8 qf[DP / 16][NP], df[DP / 16][NP];
     load_row<T, DP>(static_cast<const T *>(a.q) + w.b * a.qs[0] + (int64_t)i * a.qs[1] + w.h * a.qs[2], i < sp.nq, a.D,
@@ -742,20 +859,13 @@ __global__ __launch_bounds__(NT) void attn_bwd_q(Args a) {
     Diagonals dg;
     const int last = min(q0 + ROWS, sp.nq) - 1;
     const int kend = last < q0 ? 0 : a.causal ? min(sp.nk, max(last + sp.start + 1, 0)) : sp.nk;
-    Stage<T, DP, KT> sk, sv;
-    if (kend > 0) {
-        sk.load(K, a.ks[1], 0, sp.nk, a.D, mask);
-        sv.load(V, a.vs[1], 0, sp.nk, a.D, mask);
-    }
+    KV kv;
+    kv.init(lds, a.D);
+    if (kend > 0) kv.issue(K, a.ks[1], V, a.vs[1], 0, sp.nk, a.D, mask);
     for (int j0 = 0; j0 < kend; j0 += KT) {
-        __syncthreads();
-        sk.store(kt);
-        sv.store(vt);
-        __syncthreads();
-        if (j0 + KT < kend) {
-            sk.load(K, a.ks[1], j0 + KT, sp.nk, a.D, mask);
-            sv.load(V, a.vs[1], j0 + KT, sp.nk, a.D, mask);
-        }
+        kv.land(j0, sp.nk, mask);
+        const uint16_t *kt = kv.x(), *vt = kv.y();
+        if (j0 + KT < kend) kv.issue(K, a.ks[1], V, a.vs[1], j0 + KT, sp.nk, a.D, mask);
         const int qw = q0 + 32 * wave + sp.start;
 #pragma unroll
         for (int t = 0; t < KT / 32; ++t) {
@@ -771,7 +881,13 @@ __global__ __launch_bounds__(NT) void attn_bwd_q(Args a) {
                 row_frag<DP>(vt, PLANE, 32 * t, c, lane, f);
                 mma<NP>(dp, f, df[c]);
             }
-            finish_scores<BIAS>(a, s, scale2, tab, a.bk.far, j, j - (i + sp.start), sp.nk, edge, mask, half);
+            if constexpr (BIAS) {
+                add_bias(s, scale2, tab, a.bk.far, j - qw, j - (i + sp.start), half);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] *= scale2;
+            }
+            if (edge) hide(a, s, j - (i + sp.start), seen_keys(j, sp.nk, mask), half);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const float p = prob<T>(s[r], rs.ref, rs.inv);
@@ -811,29 +927,36 @@ __global__ __launch_bounds__(NT) void attn_bwd_q(Args a) {
         __syncthreads();
         float *to = a.bins + (((size_t)w.b * a.H + w.h) * tiles + tile) * W;
         for (int o = threadIdx.x; o < W; o += NT)
-            to[o] = ((tab[W + o] + tab[2 * W + o]) + tab[3 * W + o]) + tab[4 * W + o];
+            to[o] = ((all_bins[o] + all_bins[W + o]) + all_bins[2 * W + o]) + all_bins[3 * W + o];
     }
 }
 
-// dbias[bucket][h] from the workgroups' diagonal sums: per offset over batch and tiles, then per
-// bucket over its offsets, in 64 bits and in one order
+// dbias[bucket][h] from the workgroups' diagonal sums: a workgroup sums one bucket's offsets (a run:
+// buckets go by distance and side) over batch and tiles, in 64 bits and in one order.
 template <class T>
 __global__ __launch_bounds__(NT) void bias_reduce(Args a) {
-    __shared__ double sum[MAX_BINS];
-    const int h = blockIdx.x, W = 2 * a.bk.far + 1, tiles = (a.Nq + ROWS - 1) / ROWS;
-    for (int o = threadIdx.x; o < W; o += NT) {
-        double s = 0.;
-        for (int b = 0; b < a.B; ++b)
-            for (int t = 0; t < tiles; ++t) s += a.bins[(((size_t)b * a.H + h) * tiles + t) * W + o];
-        sum[o] = s;
-    }
+    __shared__ double sum[NT];
+    __shared__ int from, to;
+    const int h = blockIdx.x, n = blockIdx.y, far = a.bk.far, W = 2 * far + 1, tiles = (a.Nq + a.tile_rows - 1) / a.tile_rows;
+    if (threadIdx.x == 0) from = W, to = 0;
     __syncthreads();
-    for (int n = threadIdx.x; n < a.bk.n; n += NT) {
-        double s = 0.;
-        for (int o = 0; o < W; ++o)
-            if (bucket_of(a.bk, o - a.bk.far) == n) s += sum[o];
-        static_cast<T *>(a.dbias)[(size_t)n * a.H + h] = (T)(float)s;
+    for (int o = threadIdx.x; o < W; o += NT)
+        if (bucket_of(a.bk, o - far) == n) atomicMin(&from, o), atomicMax(&to, o + 1);
+    __syncthreads();
+    const int lo = from, w = to - lo, parts = a.B * tiles;  // (no offset: w <= 0)
+    double s = 0.;
+    if (w > 0)
+        for (int64_t e = threadIdx.x; e < (int64_t)parts * w; e += NT) {
+            const int p = e / w, b = p / tiles, t = p % tiles;
+            s += a.bins[(((size_t)b * a.H + h) * tiles + t) * W + lo + e % w];
+        }
+    sum[threadIdx.x] = s;
+    __syncthreads();
+    for (int k = NT / 2; k > 0; k >>= 1) {
+        if (threadIdx.x < k) sum[threadIdx.x] += sum[threadIdx.x + k];
+        __syncthreads();
     }
+    if (threadIdx.x == 0) static_cast<T *>(a.dbias)[(size_t)n * a.H + h] = (T)(float)sum[0];
 }
 
 // ------------------------------------------------------------------- C interface --
@@ -910,24 +1033,31 @@ int fwd(const Args &a, void *stream) {
         HREG_CHECK_LAUNCH();
         return HREG_OK;
     }
-    constexpr int KT = sizeof(T) == 2 || DP == 32 ? 64 : 32;
-    const size_t lds = (size_t)2 * Elem<T>::NP * KT * DP * 2 + (BIAS ? (2 * a.bk.far + 1) * 4 : 0);
+    constexpr int KT = Shape<T, DP>::FWD_KEYS;
+    const size_t lds = Tiles<T, DP, KT>::BYTES + (BIAS ? (2 * (a.bk.far + PAD) + 1) * 4 : 0);
     return launch(attn_fwd<T, DP, KT, BIAS>, a.B * a.H * row_tiles(a.Nq), lds, stream, a);
 }
 
 template <class T, int DP, bool BIAS>
 int bwd(const Args &a, void *stream) {
-    constexpr int NP = Elem<T>::NP, QT = sizeof(T) == 2 || DP == 32 ? 64 : 32;
-    const size_t W = BIAS ? 2 * a.bk.far + 1 : 0, tile = (size_t)2 * NP * QT * DP * 2;
+    constexpr int QT = Shape<T, DP>::BWD_ROWS;
+    const size_t W = BIAS ? 2 * a.bk.far + 1 : 0, tab = BIAS ? W + 2 * PAD : 0, tile = Tiles<T, DP, QT>::BYTES;
     int rc = HREG_OK;
     if (a.Nq > 0) {
         const int64_t rows = (int64_t)a.B * a.H * a.Nq;
         hipLaunchKernelGGL(attn_delta<T>, dim3((rows + NT / 16 - 1) / (NT / 16)), dim3(NT), 0, as_stream(stream), a);
         HREG_CHECK_LAUNCH();
     }
-    if (a.Nk > 0 && a.dk) rc = launch(attn_bwd_kv<T, DP, QT, BIAS>, a.B * a.Hk * row_tiles(a.Nk), tile + (3 * QT + W) * 4, stream, a);
+    if (a.Nk > 0 && a.dk) {
+        rc = launch(attn_bwd_kv<T, DP, QT, BIAS>, a.B * a.Hk * a.groups * row_tiles(a.Nk), tile + (3 * QT + tab) * 4, stream, a);
+        if (rc == HREG_OK && a.groups > 1) {
+            const int64_t n = (int64_t)a.B * a.Nk * a.Hk * (a.D / 4);
+            hipLaunchKernelGGL(sum_group<T>, dim3((n + NT - 1) / NT, 2), dim3(NT), 0, as_stream(stream), a);
+            HREG_CHECK_LAUNCH();
+        }
+    }
     if (rc == HREG_OK && a.Nq > 0 && (a.dq || a.dbias))
-        rc = launch(attn_bwd_q<T, DP, QT, BIAS>, a.B * a.H * row_tiles(a.Nq), tile + 5 * W * 4, stream, a);
+        rc = launch(attn_bwd_q<T, DP, QT, BIAS>, a.B * a.H * row_tiles(a.Nq), tile + (tab + 4 * W) * 4, stream, a);
     return rc;
 }
 
@@ -964,6 +1094,17 @@ size_t part_floats(const hreg_tok_attn_t *p, int splits) {  // results, then max
     return splits > 1 ? (size_t)p->B * p->H * p->Nq * splits : 0;
 }
 
+// heads of a group that the key gradients are split over
+int groups_of(const hreg_tok_attn_t *p) {
+    const int G = p->H / p->Hk;
+    return p->dk && G > 1 && (int64_t)p->B * p->Hk * row_tiles(p->Nk) < 4 * CUS ? G : 1;
+}
+size_t group_floats(const hreg_tok_attn_t *p) {
+    return groups_of(p) > 1 ? (size_t)p->B * p->Nk * p->H * p->D : 0;
+}
+size_t bins_bytes(const hreg_tok_attn_t *p) {
+    return p->bias ? ((size_t)p->B * p->H * row_tiles(p->Nq) * (2 * (size_t)p->max_distance + 1) * 4 + 255) / 256 * 256 : 0;
+}
 size_t delta_bytes(const hreg_tok_attn_t *p) { return ((size_t)p->B * p->H * p->Nq * 4 + 255) / 256 * 256; }
 
 }  // namespace
@@ -973,7 +1114,7 @@ extern "C" {
 size_t hreg_tok_attn_ws_bytes(const hreg_tok_attn_t *p, int backward) {
     if (!p || p->B < 0 || p->Nq < 0 || p->Nk < 0 || p->H < 1 || p->Hk < 1 || p->H % p->Hk || p->D < 1) return 0;
     if (!backward) return part_floats(p, split_of(p)) * (p->D + 2) * 4;
-    return delta_bytes(p) + (p->bias ? (size_t)p->B * p->H * row_tiles(p->Nq) * (2 * (size_t)p->max_distance + 1) * 4 : 0);
+    return delta_bytes(p) + bins_bytes(p) + 2 * group_floats(p) * 4;
 }
 
 int hreg_tok_attn_fwd(const hreg_tok_attn_t *p, void *stream) {
@@ -1000,15 +1141,19 @@ int hreg_tok_attn_bwd(const hreg_tok_attn_t *p, void *stream) {
     if (!p->dk != !p->dv) return HREG_ERR_INVALID;
     const size_t need = hreg_tok_attn_ws_bytes(p, 1);
     if (p->ws_bytes < need || (need && (!p->ws || reinterpret_cast<uintptr_t>(p->ws) % 256))) return HREG_ERR_INVALID;
+    a.tile_rows = ROWS;
     a.delta = static_cast<float *>(p->ws);
     a.bins = reinterpret_cast<float *>(static_cast<char *>(p->ws) + delta_bytes(p));
+    a.groups = groups_of(p);
+    a.part = reinterpret_cast<float *>(static_cast<char *>(p->ws) + delta_bytes(p) + bins_bytes(p));
+    a.sums = a.part + group_floats(p);
     if (a.B > 0) {
         const int rc2 = by_type<true>(p, a, stream);
         if (rc2 != HREG_OK) return rc2;
     }
     if (a.dbias) {  // an empty batch too: the gradient is zero
-        if (a.bias_f32) hipLaunchKernelGGL(bias_reduce<float>, dim3(a.H), dim3(NT), 0, as_stream(stream), a);
-        else hipLaunchKernelGGL(bias_reduce<__bf16>, dim3(a.H), dim3(NT), 0, as_stream(stream), a);
+        if (a.bias_f32) hipLaunchKernelGGL(bias_reduce<float>, dim3(a.H, a.bk.n), dim3(NT), 0, as_stream(stream), a);
+        else hipLaunchKernelGGL(bias_reduce<__bf16>, dim3(a.H, a.bk.n), dim3(NT), 0, as_stream(stream), a);
         HREG_CHECK_LAUNCH();
     }
     return HREG_OK;

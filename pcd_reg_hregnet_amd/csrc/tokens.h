@@ -18,6 +18,8 @@ typedef u32x2 __attribute__((may_alias)) u32x2_m;
 typedef f32x4 __attribute__((may_alias)) f32x4_m;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(1))) const void glob_void;
 
 // A product of two T values is NP * (NP + 1) / 2 bf16 matrix products of their pieces: one
 // for bf16; six for f32, whose values are the exact sum of three bf16 pieces (the three
@@ -116,6 +118,12 @@ __device__ __forceinline__ void col_frag(const uint16_t *t, int plane, int row0,
         const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(t + s * plane + a1));
         p[s] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
+}
+
+// 16 bytes a lane from global memory straight into LDS: lane l's to `to` + 16 l (`to` alike in the
+// wave), nothing where a lane is inactive.  Counted by vmcnt.
+__device__ __forceinline__ void global_to_lds(const void *from, const uint16_t *to) {
+    __builtin_amdgcn_global_load_lds((glob_void *)from, (lds_void *)to, 16, 0, 0);
 }
 
 // eight consecutive elements in registers
