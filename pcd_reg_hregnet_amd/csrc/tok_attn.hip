@@ -37,6 +37,10 @@ struct Shape {
     static constexpr bool F32 = Elem<T>::NP > 1;
     static constexpr int FWD_KEYS = F32 && DP > 32 ? 32 : 64, BWD_ROWS = F32 && DP > 32 ? 32 : DP > 64 ? 32 : 64;
     static constexpr int BWD_WAVES = F32 && DP > 64 ? 1 : 2;
+    static constexpr int SPLIT_WAVES = F32 && DP > 64 ? 1 : 2;
+    // waves that share 32 rows in a small call (8 x 512 keys x 4 heads x 32 f32: 126 -> 78 us with 4;
+    // 2 x 700 x 8 x 64 f32: 146 -> 99 with 2, 137 with 4, whose tiles leave one workgroup a CU)
+    static constexpr int SHARE = F32 && DP > 64 ? 1 : DP > 32 ? 2 : 4;
 };
 
 struct Buckets {
@@ -52,7 +56,7 @@ struct Args {
     const uint8_t *key_mask;
     const void *bias;
     int64_t qs[3], ks[3], vs[3], os[3], dos[3], mask_sb;
-    int B, Nq, Nk, H, Hk, D, causal, align_end, bias_f32, splits, groups, tile_rows;
+    int B, Nq, Nk, H, Hk, D, causal, align_end, bias_f32, splits, groups, share_kv, tile_rows, group_tables, split_bytes;
     float scale;
     Buckets bk;
 };
@@ -258,6 +262,14 @@ __device__ __forceinline__ void add_bias(f32x16 &s, float scale2, const float *t
     }
 }
 
+// LDS of a kernel whose KW waves share rows: its tiles, then MATS joined matrices of the sharing
+// waves in the same place
+template <class T, int DP, int R, int KW, int MATS>
+constexpr size_t area() {
+    constexpr size_t tiles = Tiles<T, DP, R>::BYTES, join = (size_t)(4 / KW) * (KW - 1) * MATS * 32 * (DP + 4) * 4;
+    return tiles > join ? tiles : join;
+}
+
 // keys that the lane's query does not see: -inf.  krow = index of the first key; seen: bit k = key
 // krow + k exists and is not masked
 __device__ __forceinline__ void hide(const Args &a, f32x16 &s, int kpos, uint32_t seen, int half) {
@@ -435,11 +447,10 @@ struct WaveStage {
 };
 
 template <class T, int DP, bool BIAS>
-__global__ __launch_bounds__(NT) void attn_split(Args a) {
+__global__ __launch_bounds__(NT, (Shape<T, DP>::SPLIT_WAVES)) void attn_split(Args a) {
     constexpr int NP = Elem<T>::NP, PLANE = 32 * DP, OLD = DP + 4;  // OLD: a joined row's step in LDS
     extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
     __shared__ float ml[4][2][32];
-    __shared__ uint8_t lut[BIAS ? MAX_BINS : 1];
     const int G = a.H / a.Hk, R = a.Nq * G, tiles = (R + 31) / 32;
     const Where w = where(a.B, a.Hk, tiles * a.splits);  // the splits of a tile are neighbours of its keys' others
     const int split = w.tile % a.splits, tile = w.tile / a.splits;
@@ -451,10 +462,16 @@ __global__ __launch_bounds__(NT) void attn_split(Args a) {
     const T *V = static_cast<const T *>(a.v) + w.b * a.vs[0] + w.h * a.vs[2];
     const uint8_t *mask = a.key_mask ? a.key_mask + w.b * a.mask_sb : nullptr;
     uint16_t *buf = lds + wave * NP * PLANE;
-    float left = 0.f, right = 0.f;  // the bias beyond the far offsets
+    // the bias of the group's heads: their tables in LDS, or (many heads) bucket by bucket from memory
+    float left = 0.f, right = 0.f;  // beyond the far offsets
+    const float *tab = nullptr;
     if constexpr (BIAS) {
-        for (int o = threadIdx.x; o <= 2 * a.bk.far; o += NT) lut[o] = bucket_of(a.bk, o - a.bk.far);
-        const int hb = r < R ? h : 0;
+        const int W = table_size(a.bk.far), hb = r < R ? h : w.h * G;
+        if (a.group_tables) {
+            float *at = reinterpret_cast<float *>(reinterpret_cast<char *>(lds) + a.split_bytes);
+            for (int g = 0; g < G; ++g) fill_table(a, at + g * W, w.h * G + g);
+            tab = at + (hb - w.h * G) * W + a.bk.far + PAD;
+        }
         left = bias_at(a, bucket_of(a.bk, -a.bk.far), hb) * LOG2E;
         right = bias_at(a, bucket_of(a.bk, a.bk.far), hb) * LOG2E;
         __syncthreads();
@@ -493,15 +510,20 @@ __global__ __launch_bounds__(NT) void attn_split(Args a) {
         const bool edge = mask || j0 + 32 > sp.nk || (a.causal && j0 + 31 > first_pos);
         const bool near = BIAS && __any(kpos + 31 > -a.bk.far && kpos < a.bk.far);
         float top = m;
+        if (!near) {
+            const float bias = kpos < 0 ? left : right;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const int kr = 8 * (e >> 2) + 4 * half + (e & 3);
-            float x = s[e] * scale2;
-            if constexpr (BIAS) {
-                if (near) x += bias_at(a, lut[min(max(kpos + kr, -a.bk.far), a.bk.far) + a.bk.far], r < R ? h : 0) * LOG2E;
-                else x += kpos < 0 ? left : right;
+            for (int e = 0; e < 16; ++e) s[e] = BIAS ? __builtin_fmaf(s[e], scale2, bias) : s[e] * scale2;
+        } else if (a.group_tables) {
+            const float *t = tab + min(max(kpos, -a.bk.far - PAD), a.bk.far + PAD - 31) + 4 * half;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = __builtin_fmaf(s[e], scale2, t[8 * (e >> 2) + (e & 3)]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int o = min(max(kpos + 8 * (e >> 2) + 4 * half + (e & 3), -a.bk.far), a.bk.far);
+                s[e] = __builtin_fmaf(s[e], scale2, bias_at(a, bucket_of(a.bk, o), r < R ? h : w.h * G) * LOG2E);
             }
-            s[e] = x;
         }
         if (edge) hide(a, s, kpos, seen_keys(j0, sp.nk, mask), half);
 #pragma unroll
@@ -583,22 +605,32 @@ __global__ __launch_bounds__(NT) void attn_split(Args a) {
 // out of the runs' partial results: 32 lanes a row, runs in order
 template <class T>
 __global__ __launch_bounds__(NT) void attn_join(Args a) {
-    const int G = a.H / a.Hk, R = a.Nq * G;
+    const int G = a.H / a.Hk, R = a.Nq * G, lane = threadIdx.x % 32, col = lane * 4;
     const int64_t row = (int64_t)blockIdx.x * (NT / 32) + threadIdx.x / 32;
-    const int col = threadIdx.x % 32 * 4;
-    if (row >= (int64_t)a.B * a.Hk * R || col >= a.D) return;
-    const int r = row % R, hk = row / R % a.Hk, b = row / R / a.Hk;
-    const float *sums = a.sums + 2 * row * a.splits, *part = a.part + row * a.splits * a.D + col;
+    if (row >= (int64_t)a.B * a.Hk * R) return;
+    const float *sums = a.sums + 2 * row * a.splits, *part = a.part + row * a.splits * a.D + min(col, a.D - 4);
     float all = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) all = fmaxf(all, sums[2 * s]);
+    for (int s = lane; s < a.splits; s += 32) all = fmaxf(all, sums[2 * s]);
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) all = fmaxf(all, __shfl_xor(all, k));
     f32x4 o{0.f, 0.f, 0.f, 0.f};
     float sum = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
-        const float f = sums[2 * s] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sums[2 * s] - all);
-        o += *reinterpret_cast<const f32x4_m *>(part + (int64_t)s * a.D) * f;
-        sum += sums[2 * s + 1] * f;
+    for (int s0 = 0; s0 < a.splits; s0 += 32) {
+        float f = 0.f, l = 0.f;  // lane s: run s0 + s
+        if (s0 + lane < a.splits) {
+            const float m = sums[2 * (s0 + lane)];
+            f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - all);
+            l = sums[2 * (s0 + lane) + 1] * f;
+        }
+        const int n = min(a.splits - s0, 32);
+#pragma unroll 4
+        for (int s = 0; s < n; ++s) {
+            o += *reinterpret_cast<const f32x4_m *>(part + (int64_t)(s0 + s) * a.D) * __shfl(f, (threadIdx.x & 32) + s);
+            sum += __shfl(l, (threadIdx.x & 32) + s);
+        }
     }
-    finish_row<T>(a, b, r / G, hk * G + r % G, col, o, all, sum);
+    const int r = row % R, hk = row / R % a.Hk, b = row / R / a.Hk;
+    if (col < a.D) finish_row<T>(a, b, r / G, hk * G + r % G, col, o, all, sum);
 }
 
 // ---------------------------------------------------------------------- backward --
@@ -627,17 +659,20 @@ __global__ __launch_bounds__(NT) void attn_delta(Args a) {
 // dk, dv of 128 keys: every wave keeps 32 keys and walks all rows of all heads that share them, so
 // the sums over a group need no second pass and have one order.  Where that leaves too few
 // workgroups (a.groups) each walks one head, and sum_group adds the heads' f32 results.
-template <class T, int DP, int QT, bool BIAS>
-__global__ __launch_bounds__(NT, (Shape<T, DP>::BWD_WAVES)) void attn_bwd_kv(Args a) {
-    constexpr int NP = Elem<T>::NP, PLANE = QT * DP;
+// KW waves share 32 keys, each taking every KW-th 32 rows (a small call has few keys to give a wave
+// of its own): their sums join in LDS, in wave order.
+template <class T, int DP, int QT, int KW, bool BIAS>
+__global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::BWD_WAVES : 1)) void attn_bwd_kv(Args a) {
+    constexpr int NP = Elem<T>::NP, PLANE = QT * DP, ROWS = 128 / KW;
+    static_assert(QT % (32 * KW) == 0, "tile");
     extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
     typedef Tiles<T, DP, QT> QD;
-    float *lt = reinterpret_cast<float *>(reinterpret_cast<char *>(lds) + QD::BYTES), *et = lt + QT, *it = et + QT, *tab = it + QT;
+    float *lt = reinterpret_cast<float *>(reinterpret_cast<char *>(lds) + area<T, DP, QT, KW, 2>()), *et = lt + QT, *it = et + QT, *tab = it + QT;
     const Where w0 = where(a.B, a.Hk * a.groups, (a.Nk + ROWS - 1) / ROWS);
     const Where w{w0.b, w0.h / a.groups, w0.tile};
     const Span sp = span_of(a, w.b);
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
-    const int k0 = w.tile * ROWS, j = k0 + 32 * wave + (lane & 31);
+    const int share = wave % KW, k0 = w.tile * ROWS + 32 * (wave / KW), j = k0 + (lane & 31);
     const uint8_t *mask = a.key_mask ? a.key_mask + w.b * a.mask_sb : nullptr;
     const bool ok = j < sp.nk && (!mask || mask[j]);
     bf16x8 kf[DP / 16][NP], vf[DP / 16][NP];
@@ -647,12 +682,12 @@ __global__ __launch_bounds__(NT, (Shape<T, DP>::BWD_WAVES)) void attn_bwd_kv(Arg
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) dk[d] = dv[d] = zero16();
     const float scale2 = a.scale * LOG2E;
-    const int first = a.causal ? max(k0 - sp.start, 0) / QT * QT : 0;  // rows before see no key of the tile
+    const int first = a.causal ? max(w.tile * ROWS - sp.start, 0) / QT * QT : 0;  // rows before see no key of the tile
     const int G = a.H / a.Hk;
     QD qd;
     qd.init(lds, a.D);
     const int g0 = w0.h % a.groups * (G / a.groups);
-    if (k0 < sp.nk)
+    if (w.tile * ROWS < sp.nk)
         for (int g = g0; g < g0 + G / a.groups; ++g) {
             const int h = w.h * G + g;
             const T *Q = static_cast<const T *>(a.q) + w.b * a.qs[0] + h * a.qs[2];
@@ -676,12 +711,13 @@ __global__ __launch_bounds__(NT, (Shape<T, DP>::BWD_WAVES)) void attn_bwd_kv(Arg
                 const uint16_t *qt = qd.x(), *dt = qd.y();
                 if (i0 + QT < sp.nq) qd.issue(Q, a.qs[1], dO, a.dos[1], i0 + QT, sp.nq, a.D, nullptr);
 #pragma unroll
-                for (int t = 0; t < QT / 32; ++t) {
+                for (int u = 0; u < QT / 32 / KW; ++u) {
+                    const int t = u * KW + share;
                     const int p0 = i0 + 32 * t + sp.start;  // position of the first query
-                    if (a.causal && p0 + 31 < k0 + 32 * wave) continue;
-                    const bool edge = a.causal && p0 < k0 + 32 * wave + 31;
-                    const bool near = BIAS && !(k0 + 32 * wave - p0 - 31 >= a.bk.far || k0 + 32 * wave - p0 + 31 <= -a.bk.far);
-                    const float b = BIAS ? tab[k0 + 32 * wave < p0 ? 0 : 2 * (a.bk.far + PAD)] : 0.f;
+                    if (i0 + 32 * t >= sp.nq || (a.causal && p0 + 31 < k0)) continue;
+                    const bool edge = a.causal && p0 < k0 + 31;
+                    const bool near = BIAS && !(k0 - p0 - 31 >= a.bk.far || k0 - p0 + 31 <= -a.bk.far);
+                    const float b = BIAS ? tab[k0 < p0 ? 0 : 2 * (a.bk.far + PAD)] : 0.f;
                     f32x16 s = zero16(), dp = zero16();
 #pragma unroll
                     for (int c = 0; c < DP / 16; ++c) {
@@ -718,6 +754,36 @@ __global__ __launch_bounds__(NT, (Shape<T, DP>::BWD_WAVES)) void attn_bwd_kv(Arg
                 }
             }
         }
+    if constexpr (KW > 1) {
+        constexpr int LD = DP + 4;
+        float *buf = reinterpret_cast<float *>(lds) + (wave / KW) * (KW - 1) * 2 * 32 * LD + (lane & 31) * LD + 4 * half;
+        __syncthreads();
+#pragma unroll
+        for (int v = 1; v < KW; ++v)
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    float *at = buf + (v - 1) * 2 * 32 * LD + 32 * d + 2 * r;
+                    if (share == v) {
+                        store4(at, dk[d][r], dk[d][r + 1], dk[d][r + 2], dk[d][r + 3]);
+                        store4(at + 32 * LD, dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]);
+                    }
+                }
+        __syncthreads();
+        if (share) return;
+#pragma unroll
+        for (int v = 1; v < KW; ++v)
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const float *at = buf + (v - 1) * 2 * 32 * LD + 32 * d + 2 * r;
+                    const f32x4 x = *reinterpret_cast<const f32x4_m *>(at), y = *reinterpret_cast<const f32x4_m *>(at + 32 * LD);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) dk[d][r + e] += x[e], dv[d][r + e] += y[e];
+                }
+    }
     if (j < a.Nk) {
         const float f = a.scale;
         if (a.groups > 1) {
@@ -768,8 +834,8 @@ __global__ __launch_bounds__(NT) void sum_group(Args a) {
 // The bias gradient of one wave: sums of ds over the diagonals of its 32 x 32 tiles.  Offset
 // o = base - t with t = (query - key) mod 32 (add) or that + 32 (carry): every value moves to
 // lane t of its half, two sums a lane.  The carry of a tile is the add of the next one, so each
-// diagonal goes once to the wave's bins; beyond the far offsets one sum a lane is kept.  No
-// atomics: every sum has one order.
+// diagonal goes once to the wave's bins (twice where the wave's tiles do not follow each other);
+// beyond the far offsets one sum a lane is kept.  No atomics: every sum has one order.
 struct Diagonals {
     float carry = 0.f, left = 0.f, right = 0.f;
     int base = 0;
@@ -785,6 +851,7 @@ struct Diagonals {
     // ds of keys base_key .. +31 (rows) and the wave's queries; b = first key - first query position
     __device__ __forceinline__ void tile(const f32x16 &ds, int b, float *bins, int far, int lane) {
         const int t = lane & 31, half = lane >> 5;
+        if (base != b) flush(carry, base, bins, far, lane), carry = 0.f;  // (uniform)
         float a = carry;
         carry = 0.f;
         if (b - 31 >= far || b + 31 <= -far) {
@@ -817,19 +884,21 @@ struct Diagonals {
     }
 };
 
-// dq of 128 rows, and the bias gradient's sums over their diagonals
-template <class T, int DP, int KT, bool BIAS>
-__global__ __launch_bounds__(NT, (Shape<T, DP>::BWD_WAVES)) void attn_bwd_q(Args a) {
-    constexpr int NP = Elem<T>::NP, PLANE = KT * DP;
+// dq of 128 / KW rows (KW waves share 32, each taking every KW-th 32 keys), and the bias gradient's
+// sums over their diagonals
+template <class T, int DP, int KT, int KW, bool BIAS>
+__global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::BWD_WAVES : 1)) void attn_bwd_q(Args a) {
+    constexpr int NP = Elem<T>::NP, PLANE = KT * DP, ROWS = 128 / KW;
+    static_assert(KT % (32 * KW) == 0, "tile");
     extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
     typedef Tiles<T, DP, KT> KV;
     const int W = 2 * a.bk.far + 1;
-    float *tab = reinterpret_cast<float *>(reinterpret_cast<char *>(lds) + KV::BYTES);
+    float *tab = reinterpret_cast<float *>(reinterpret_cast<char *>(lds) + area<T, DP, KT, KW, 1>());
     const int tiles = (a.Nq + ROWS - 1) / ROWS;
     const Where w = where(a.B, a.H, tiles);
     const Span sp = span_of(a, w.b);
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
-    const int tile = tiles - 1 - w.tile, q0 = tile * ROWS, i = q0 + 32 * wave + (lane & 31);
+    const int tile = tiles - 1 - w.tile, q0 = tile * ROWS, share = wave % KW, i = q0 + 32 * (wave / KW) + (lane & 31);
     const int hk = w.h / (a.H / a.Hk);
     const T *K = static_cast<const T *>(a.k) + w.b * a.ks[0] + hk * a.ks[2];
     const T *V = static_cast<const T *>(a.v) + w.b * a.vs[0] + hk * a.vs[2];
@@ -866,10 +935,10 @@ __global__ __launch_bounds__(NT, (Shape<T, DP>::BWD_WAVES)) void attn_bwd_q(Args
         kv.land(j0, sp.nk, mask);
         const uint16_t *kt = kv.x(), *vt = kv.y();
         if (j0 + KT < kend) kv.issue(K, a.ks[1], V, a.vs[1], j0 + KT, sp.nk, a.D, mask);
-        const int qw = q0 + 32 * wave + sp.start;
+        const int qw = q0 + 32 * (wave / KW) + sp.start;
 #pragma unroll
-        for (int t = 0; t < KT / 32; ++t) {
-            const int j = j0 + 32 * t;
+        for (int u = 0; u < KT / 32 / KW; ++u) {
+            const int t = u * KW + share, j = j0 + 32 * t;
             if (j >= kend || (a.causal && j > qw + 31)) continue;
             const bool edge = mask || j + 32 > sp.nk || (a.causal && j + 31 > qw);
             f32x16 s = zero16(), dp = zero16();
@@ -910,7 +979,31 @@ __global__ __launch_bounds__(NT, (Shape<T, DP>::BWD_WAVES)) void attn_bwd_q(Args
             }
         }
     }
-    if (i < a.Nq && a.dq) {
+    if constexpr (KW > 1) {
+        constexpr int LD = DP + 4;
+        float *buf = reinterpret_cast<float *>(lds) + (wave / KW) * (KW - 1) * 32 * LD + (lane & 31) * LD + 4 * half;
+        __syncthreads();
+#pragma unroll
+        for (int v = 1; v < KW; ++v)
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4)
+                    if (share == v)
+                        store4(buf + (v - 1) * 32 * LD + 32 * d + 2 * r, acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]);
+        __syncthreads();
+#pragma unroll
+        for (int v = 1; v < KW; ++v)
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const f32x4 x = *reinterpret_cast<const f32x4_m *>(buf + (v - 1) * 32 * LD + 32 * d + 2 * r);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[d][r + e] += x[e];
+                }
+    }
+    if (i < a.Nq && a.dq && share == 0) {
         T *o = static_cast<T *>(a.dq) + (((int64_t)w.b * a.Nq + i) * a.H + w.h) * a.D;
         const float f = a.scale;
 #pragma unroll
@@ -1026,7 +1119,12 @@ int fwd(const Args &a, void *stream) {
     if (a.splits) {
         const int R = a.Nq * (a.H / a.Hk);
         const size_t tile = (size_t)4 * Elem<T>::NP * 32 * DP * 2, join = (size_t)4 * 32 * (DP + 4) * 4;
-        const int rc = launch(attn_split<T, DP, BIAS>, a.B * a.Hk * ((R + 31) / 32) * a.splits, tile > join ? tile : join, stream, a);
+        Args b = a;
+        b.split_bytes = tile > join ? tile : join;
+        const size_t tables = BIAS ? (size_t)(a.H / a.Hk) * (2 * (a.bk.far + PAD) + 1) * 4 : 0;
+        b.group_tables = tables <= 32768;
+        const int rc = launch(attn_split<T, DP, BIAS>, a.B * a.Hk * ((R + 31) / 32) * a.splits,
+                              b.split_bytes + (b.group_tables ? tables : 0), stream, b);
         if (rc != HREG_OK || a.splits == 1) return rc;
         const int64_t rows = (int64_t)a.B * a.H * a.Nq;
         hipLaunchKernelGGL(attn_join<T>, dim3((rows + NT / 32 - 1) / (NT / 32)), dim3(NT), 0, as_stream(stream), a);
@@ -1038,10 +1136,22 @@ int fwd(const Args &a, void *stream) {
     return launch(attn_fwd<T, DP, KT, BIAS>, a.B * a.H * row_tiles(a.Nq), lds, stream, a);
 }
 
+template <class T, int DP, int KW, bool BIAS>
+int bwd_kv(const Args &a, void *stream) {
+    constexpr int QT = KW > 1 ? 32 * KW : Shape<T, DP>::BWD_ROWS;
+    const size_t lds = area<T, DP, QT, KW, 2>() + (3 * QT + (BIAS ? 2 * (a.bk.far + PAD) + 1 : 0)) * 4;
+    return launch(attn_bwd_kv<T, DP, QT, KW, BIAS>, a.B * a.Hk * a.groups * ((a.Nk + 128 / KW - 1) / (128 / KW)), lds, stream, a);
+}
+template <class T, int DP, int KW, bool BIAS>
+int bwd_q(const Args &a, void *stream) {
+    constexpr int KT = KW > 1 ? 32 * KW : Shape<T, DP>::BWD_ROWS;
+    const size_t W = 2 * a.bk.far + 1, lds = area<T, DP, KT, KW, 1>() + (BIAS ? W + 2 * PAD + 4 * W : 0) * 4;
+    return launch(attn_bwd_q<T, DP, KT, KW, BIAS>, a.B * a.H * ((a.Nq + a.tile_rows - 1) / a.tile_rows), lds, stream, a);
+}
+
 template <class T, int DP, bool BIAS>
 int bwd(const Args &a, void *stream) {
-    constexpr int QT = Shape<T, DP>::BWD_ROWS;
-    const size_t W = BIAS ? 2 * a.bk.far + 1 : 0, tab = BIAS ? W + 2 * PAD : 0, tile = Tiles<T, DP, QT>::BYTES;
+    constexpr int SHARE = Shape<T, DP>::SHARE;
     int rc = HREG_OK;
     if (a.Nq > 0) {
         const int64_t rows = (int64_t)a.B * a.H * a.Nq;
@@ -1049,7 +1159,7 @@ int bwd(const Args &a, void *stream) {
         HREG_CHECK_LAUNCH();
     }
     if (a.Nk > 0 && a.dk) {
-        rc = launch(attn_bwd_kv<T, DP, QT, BIAS>, a.B * a.Hk * a.groups * row_tiles(a.Nk), tile + (3 * QT + tab) * 4, stream, a);
+        rc = a.share_kv ? bwd_kv<T, DP, SHARE, BIAS>(a, stream) : bwd_kv<T, DP, 1, BIAS>(a, stream);
         if (rc == HREG_OK && a.groups > 1) {
             const int64_t n = (int64_t)a.B * a.Nk * a.Hk * (a.D / 4);
             hipLaunchKernelGGL(sum_group<T>, dim3((n + NT - 1) / NT, 2), dim3(NT), 0, as_stream(stream), a);
@@ -1057,7 +1167,7 @@ int bwd(const Args &a, void *stream) {
         }
     }
     if (rc == HREG_OK && a.Nq > 0 && (a.dq || a.dbias))
-        rc = launch(attn_bwd_q<T, DP, QT, BIAS>, a.B * a.H * row_tiles(a.Nq), tile + (tab + 4 * W) * 4, stream, a);
+        rc = a.tile_rows < ROWS ? bwd_q<T, DP, SHARE, BIAS>(a, stream) : bwd_q<T, DP, 1, BIAS>(a, stream);
     return rc;
 }
 
@@ -1081,12 +1191,15 @@ int by_type(const hreg_tok_attn_t *p, const Args &a, void *stream) {
     return a.bias ? by_width<__bf16, true, BACK>(a, stream) : by_width<__bf16, false, BACK>(a, stream);
 }
 
-// 0: the row kernel; else the number of runs of the split kernel.  Measured (us, row / split kernel):
+// 0: the row kernel; else the number of runs of the split kernel: where all rows of a key head fit
+// one of its tiles, or few row tiles face many keys.  (us, row / split kernel: 1 token x 32768 keys
+// 1110 / 160; 2 x 700 x 8 heads x 128 bf16 29 / 37; 4 x 517 x 8 x 40 f32 with a bias 39 / 47.)  Two
+// workgroups a CU are enough: 4 tokens x 8191 keys take 34 us with 512, 45 with 1024.
 int split_of(const hreg_tok_attn_t *p) {
     const int64_t R = (int64_t)p->Nq * (p->H / p->Hk), tiles = (int64_t)p->B * p->Hk * ((R + 31) / 32);
     const int64_t rows = (int64_t)p->B * p->H * row_tiles(p->Nq);
-    if (tiles == 0 || (rows >= 256 && R > 32)) return 0;
-    int64_t s = (1024 + tiles - 1) / tiles, most = (p->Nk + 255) / 256;
+    if (tiles == 0 || (R > 32 && (rows >= CUS || p->Nk <= 16 * rows))) return 0;
+    int64_t s = (2 * CUS + tiles - 1) / tiles, most = (p->Nk + 255) / 256;
     s = s < most ? s : most;
     return s < 1 ? 1 : s > 256 ? 256 : (int)s;
 }
@@ -1094,16 +1207,31 @@ size_t part_floats(const hreg_tok_attn_t *p, int splits) {  // results, then max
     return splits > 1 ? (size_t)p->B * p->H * p->Nq * splits : 0;
 }
 
-// heads of a group that the key gradients are split over
-int groups_of(const hreg_tok_attn_t *p) {
-    const int G = p->H / p->Hk;
-    return p->dk && G > 1 && (int64_t)p->B * p->Hk * row_tiles(p->Nk) < 4 * CUS ? G : 1;
+// How the backward pass is divided.  groups: heads of a group that the key gradients are split over
+// (2 x 4096 keys x 4 of 16 heads x 128 bf16: one long workgroup a CU otherwise, 1600 -> 938 us);
+// share_kv, tile_rows: whether waves share rows, and the query rows of a workgroup.  Sharing pays
+// while fewer than 160 workgroups are there without it (96: 146 -> 99 us; 160: 141 -> 176).
+struct BwdPlan { int groups, share_kv, tile_rows; };
+template <class T>
+int share_of(int D) {
+    return D <= 32 ? Shape<T, 32>::SHARE : D <= 64 ? Shape<T, 64>::SHARE : Shape<T, 128>::SHARE;
+}
+BwdPlan bwd_plan(const hreg_tok_attn_t *p) {
+    const int G = p->H / p->Hk, share = p->dtype == HREG_TOK_F32 ? share_of<float>(p->D) : share_of<__bf16>(p->D);
+    const int64_t keys = (int64_t)p->B * p->Hk * row_tiles(p->Nk), rows = (int64_t)p->B * p->H * row_tiles(p->Nq);
+    BwdPlan q;
+    q.groups = p->dk && G > 1 && keys < 4 * CUS ? G : 1;
+    q.share_kv = share > 1 && keys * q.groups < 160;
+    q.tile_rows = rows < 160 ? ROWS / share : ROWS;
+    return q;
 }
 size_t group_floats(const hreg_tok_attn_t *p) {
-    return groups_of(p) > 1 ? (size_t)p->B * p->Nk * p->H * p->D : 0;
+    return bwd_plan(p).groups > 1 ? (size_t)p->B * p->Nk * p->H * p->D : 0;
 }
 size_t bins_bytes(const hreg_tok_attn_t *p) {
-    return p->bias ? ((size_t)p->B * p->H * row_tiles(p->Nq) * (2 * (size_t)p->max_distance + 1) * 4 + 255) / 256 * 256 : 0;
+    if (!p->bias) return 0;
+    const size_t rows = bwd_plan(p).tile_rows, tiles = (p->Nq + rows - 1) / rows;
+    return (p->B * p->H * tiles * (2 * (size_t)p->max_distance + 1) * 4 + 255) / 256 * 256;
 }
 size_t delta_bytes(const hreg_tok_attn_t *p) { return ((size_t)p->B * p->H * p->Nq * 4 + 255) / 256 * 256; }
 
@@ -1141,10 +1269,12 @@ int hreg_tok_attn_bwd(const hreg_tok_attn_t *p, void *stream) {
     if (!p->dk != !p->dv) return HREG_ERR_INVALID;
     const size_t need = hreg_tok_attn_ws_bytes(p, 1);
     if (p->ws_bytes < need || (need && (!p->ws || reinterpret_cast<uintptr_t>(p->ws) % 256))) return HREG_ERR_INVALID;
-    a.tile_rows = ROWS;
+    const BwdPlan plan = bwd_plan(p);
+    a.tile_rows = plan.tile_rows;
+    a.share_kv = plan.share_kv;
     a.delta = static_cast<float *>(p->ws);
     a.bins = reinterpret_cast<float *>(static_cast<char *>(p->ws) + delta_bytes(p));
-    a.groups = groups_of(p);
+    a.groups = plan.groups;
     a.part = reinterpret_cast<float *>(static_cast<char *>(p->ws) + delta_bytes(p) + bins_bytes(p));
     a.sums = a.part + group_floats(p);
     if (a.B > 0) {
