@@ -61,13 +61,16 @@ TOK_MAX_BUCKETS, TOK_MAX_THRESH, TOK_MAX_DISTANCE = 128, 64, 1024
 
 
 class TokAttn(ctypes.Structure):
+    # (the header's stride arrays as scalars: setting them takes a tenth of the time)
     _fields_ = [("dtype", _i), ("B", _i), ("Nq", _i), ("Nk", _i), ("H", _i), ("Hk", _i), ("D", _i),
                 ("causal", _i), ("align_end", _i), ("scale", ctypes.c_float), ("q", _vp), ("k", _vp),
-                ("v", _vp), ("out", _vp), ("qs", _i64 * 3), ("ks", _i64 * 3), ("vs", _i64 * 3),
-                ("os", _i64 * 3), ("lse", _vp), ("out_rest", _vp), ("q_len", _vp), ("k_len", _vp), ("key_mask", _vp),
+                ("v", _vp), ("out", _vp),
+                *((f"{t}_{d}", _i64) for t in ("qs", "ks", "vs", "os") for d in "bnh"),
+                ("lse", _vp), ("out_rest", _vp), ("q_len", _vp), ("k_len", _vp), ("key_mask", _vp),
                 ("mask_sb", _i64), ("bias", _vp), ("bias_dtype", _i), ("num_buckets", _i),
                 ("max_distance", _i), ("both", _i), ("nthresh", _i),
-                ("thresh", ctypes.c_int32 * TOK_MAX_THRESH), ("dout", _vp), ("dos", _i64 * 3),
+                ("thresh", ctypes.c_int32 * TOK_MAX_THRESH), ("dout", _vp),
+                ("dos_b", _i64), ("dos_n", _i64), ("dos_h", _i64),
                 ("dq", _vp), ("dk", _vp), ("dv", _vp), ("dbias", _vp), ("ws", _vp),
                 ("ws_bytes", ctypes.c_size_t)]
 

@@ -21,6 +21,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import struct
 from dataclasses import dataclass
 
 import torch
@@ -28,6 +29,7 @@ import torch
 from . import _lib
 
 _DTYPES = {torch.float32: _lib.TOK_F32, torch.bfloat16: _lib.TOK_BF16}
+_DENSE = torch.contiguous_format
 _NORMS = {None: 0, "rms": 1, "layer": 2}
 
 
@@ -71,7 +73,12 @@ def _check_tensor(fn: str, name: str, t, device=None, dtype=None) -> None:
 
 
 def _ptr(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
+
+
+# the leading fields of the C structs, packed in one step (0.5 us; one by one they take 6)
+_ATTN_HEAD = struct.Struct("@9if4P12q4P")  # dtype .. scale, q k v out, their strides, lse .. k_len
+_BLOCK_HEAD = struct.Struct("@7i2f2IQ20P")  # dtype .. seed, seed_dev, x .. dpre_b
 
 
 # --------------------------------------------------------------------- relative positions
@@ -149,9 +156,10 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 def _attn_args(o, q, k, v, out, lse, out_rest, q_len, k_len, key_mask, bias) -> _lib.TokAttn:
     scale, causal, align_end, buckets = o
     B, Nq, H, D = q.shape
-    p = _lib.TokAttn(_DTYPES[q.dtype], B, Nq, k.shape[1], H, k.shape[2], D, causal, align_end, scale, q.data_ptr(),
-                     k.data_ptr(), v.data_ptr(), out.data_ptr(), q.stride()[:3], k.stride()[:3], v.stride()[:3],
-                     out.stride()[:3], _ptr(lse), _ptr(out_rest), _ptr(q_len), _ptr(k_len))
+    p = _lib.TokAttn()
+    _ATTN_HEAD.pack_into(p, 0, _DTYPES[q.dtype], B, Nq, k.shape[1], H, k.shape[2], D, causal, align_end, scale, q.data_ptr(),
+                         k.data_ptr(), v.data_ptr(), out.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+                         *out.stride()[:3], _ptr(lse), _ptr(out_rest), _ptr(q_len), _ptr(k_len))
     if key_mask is not None:
         p.key_mask, p.mask_sb = key_mask.data_ptr(), 0 if key_mask.shape[0] == 1 else key_mask.stride(0)
     if bias is not None:
@@ -175,7 +183,7 @@ def _attn_ws(p: _lib.TokAttn, backward: int, device):
 def _attn_forward(o, q, k, v, bias, q_len, k_len, key_mask, train: bool):
     q, k, v = _rows(q), _rows(k), _rows(v)
     dev = q.device
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    out = torch.empty_like(q, memory_format=_DENSE)
     B, Nq, H, _ = q.shape
     lse = torch.empty(2, B, H, Nq, device=dev) if train else None
     rest = torch.empty_like(out) if train and q.dtype != torch.float32 else None
@@ -200,12 +208,13 @@ class _TokAttention(torch.autograd.Function):
         need_q, need_k, need_v, need_b = ctx.needs_input_grad[:4]
         dout = _rows(dout)
         dev = q.device
-        dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if need_q else None
-        dk = torch.empty(k.shape, dtype=k.dtype, device=dev) if need_k or need_v else None
-        dv = torch.empty(v.shape, dtype=v.dtype, device=dev) if need_k or need_v else None
-        db = torch.empty(bias.shape, dtype=bias.dtype, device=dev) if need_b else None
+        dq = torch.empty_like(q, memory_format=_DENSE) if need_q else None
+        dk = torch.empty_like(k, memory_format=_DENSE) if need_k or need_v else None
+        dv = torch.empty_like(v, memory_format=_DENSE) if need_k or need_v else None
+        db = torch.empty_like(bias) if need_b else None
         p = _attn_args(ctx.o, q, k, v, out, lse, rest, q_len, k_len, key_mask, bias)
-        p.dout, p.dos = dout.data_ptr(), dout.stride()[:3]
+        p.dout = dout.data_ptr()
+        p.dos_b, p.dos_n, p.dos_h, _ = dout.stride()
         p.dq, p.dk, p.dv, p.dbias = _ptr(dq), _ptr(dk), _ptr(dv), _ptr(db)
         ws = _attn_ws(p, 1, dev)  # noqa: F841
         _launch(dev, "hreg_tok_attn_bwd", ctypes.byref(p))
@@ -220,7 +229,7 @@ def _lengths(name: str, t, B: int, device):
         raise ValueError(f"attention: {name} must be int32 or int64 of shape ({B},), got {t.dtype} {tuple(t.shape)}")
     if t.dtype == torch.int64:
         t = t.clamp(0, 2 ** 31 - 1).to(torch.int32)
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def attention(q, k, v, *, scale=None, causal=False, align_end=None, q_lengths=None, k_lengths=None,
@@ -246,8 +255,9 @@ def attention(q, k, v, *, scale=None, causal=False, align_end=None, q_lengths=No
     key and query.  With bfloat16 rows its gradient has their accuracy (about 2^-8 of it)."""
     _check_tensor("attention", "q", q)
     dev, dtype = q.device, q.dtype
-    _check_tensor("attention", "k", k, dev, dtype)
-    _check_tensor("attention", "v", v, dev, dtype)
+    for name, t in (("k", k), ("v", v)):
+        if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != dev:
+            _check_tensor("attention", name, t, dev, dtype)
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError(f"attention: q, k, v must be [batch, tokens, heads, width], got {tuple(q.shape)}, {tuple(k.shape)}, "
                          f"{tuple(v.shape)}")
@@ -354,9 +364,13 @@ def _block_args(o, like, param_dtype, seed, x, f, gate, post_w, post_b, pre_w, p
     """back: dy, dh, then the gradients of x .. pre_b"""
     scale, eps, post, pre, step, value, site, gate_rows = o
     C = like.shape[-1]
-    return _lib.TokBlock(_DTYPES[like.dtype], _DTYPES[param_dtype], like.numel() // C, C, gate_rows, post, pre, scale, eps,
-                         step, site, value, _ptr(seed), _ptr(x), _ptr(f), _ptr(gate), _ptr(post_w), _ptr(post_b),
-                         _ptr(pre_w), _ptr(pre_b), _ptr(y), _ptr(h), _ptr(stats), *map(_ptr, back))
+    p = _lib.TokBlock()
+    dy, dh, dx, df, dgate, dpost_w, dpost_b, dpre_w, dpre_b = back or (None,) * 9
+    _BLOCK_HEAD.pack_into(p, 0, _DTYPES[like.dtype], _DTYPES[param_dtype], like.numel() // C, C, gate_rows, post, pre, scale,
+                          eps, step, site, value, _ptr(seed), _ptr(x), _ptr(f), _ptr(gate), _ptr(post_w), _ptr(post_b),
+                          _ptr(pre_w), _ptr(pre_b), _ptr(y), _ptr(h), _ptr(stats), _ptr(dy), _ptr(dh), _ptr(dx), _ptr(df),
+                          _ptr(dgate), _ptr(dpost_w), _ptr(dpost_b), _ptr(dpre_w), _ptr(dpre_b))
+    return p
 
 
 class _GatedResidualNorm(torch.autograd.Function):

@@ -109,6 +109,19 @@ def test_struct_layout_matches_c():
     assert got == [ctypes.sizeof(A), A.lse.offset, A.ws_bytes.offset, ctypes.sizeof(B), B.seed_dev.offset, B.ws_bytes.offset]
 
 
+def test_packed_fields_match_the_structs():
+    """the leading fields that are packed in one step end where the struct's next field starts"""
+    assert tokens._ATTN_HEAD.size == _lib.TokAttn.key_mask.offset
+    assert tokens._BLOCK_HEAD.size == _lib.TokBlock.ws.offset
+    p = _lib.TokAttn()
+    tokens._ATTN_HEAD.pack_into(p, 0, *range(9), 0.5, *range(10, 30))
+    assert [getattr(p, n) for n, _ in _lib.TokAttn._fields_[:9]] == list(range(9)) and p.scale == 0.5
+    assert [getattr(p, n) for n, _ in _lib.TokAttn._fields_[10:30]] == list(range(10, 30))
+    b = _lib.TokBlock()
+    tokens._BLOCK_HEAD.pack_into(b, 0, *range(1, 8), 0.5, 0.25, *range(10, 33))
+    assert [getattr(b, n) for n, _ in _lib.TokBlock._fields_[:32]] == [*range(1, 8), 0.5, 0.25, *range(10, 33)]
+
+
 def _attn(**over):
     """arguments that pass, on made-up aligned addresses (nothing is launched without a GPU: every
     case below is refused before)"""
@@ -117,7 +130,8 @@ def _attn(**over):
     for n in ("q", "k", "v", "out", "dout", "lse", "dq", "dk", "dv", "ws"):
         setattr(p, n, 4096)
     for n in ("qs", "ks", "vs", "os", "dos"):
-        setattr(p, n, (ctypes.c_int64 * 3)(128, 32, 16))
+        for d, step in (("b", 128), ("n", 32), ("h", 16)):
+            setattr(p, f"{n}_{d}", step)
     p.ws_bytes = 1 << 20
     for n, v in over.items():
         setattr(p, n, v)
@@ -127,7 +141,7 @@ def _attn(**over):
 @pytest.mark.parametrize("over,code", [
     (dict(dtype=2), 1), (dict(B=-1), 1), (dict(Nq=-1), 1), (dict(Nk=-1), 1), (dict(H=3, Hk=2), 1), (dict(Hk=0), 1),
     (dict(D=12), 3), (dict(D=136), 3), (dict(D=0), 3), (dict(q=None), 1), (dict(q=4098), 1), (dict(out=4100), 1),
-    (dict(ks=(ctypes.c_int64 * 3)(128, 36, 16)), 1), (dict(Nq=(1 << 30) + 1), 3), (dict(B=1 << 20, Nq=1 << 20), 3),
+    (dict(ks_n=36), 1), (dict(Nq=(1 << 30) + 1), 3), (dict(B=1 << 20, Nq=1 << 20), 3),
     (dict(bias=4096, bias_dtype=5), 1), (dict(bias=4096, num_buckets=1, max_distance=8), 1),
     (dict(bias=4096, num_buckets=7, both=1, max_distance=8), 1), (dict(bias=4096, num_buckets=32, max_distance=16), 1),
     (dict(bias=4096, num_buckets=32, max_distance=2000, nthresh=15), 3),
@@ -142,7 +156,7 @@ def test_attention_entry_refuses(over, code):
 
 @pytest.mark.parametrize("over", [dict(ws_bytes=16), dict(ws=None), dict(ws=4096 + 16), dict(dout=None), dict(dout=4100),
                                   dict(lse=None), dict(dq=4104), dict(dk=None), dict(dv=None),
-                                  dict(dos=(ctypes.c_int64 * 3)(128, 33, 16))])
+                                  dict(dos_n=33)])
 def test_attention_backward_entry_refuses(over):
     assert _lib.load(require_gpu=False).hreg_tok_attn_bwd(ctypes.byref(_attn(**over)), None) == 1
 
