@@ -39,11 +39,12 @@ __device__ __forceinline__ u32x4 philox(uint64_t group, uint32_t site, uint64_t 
     return u32x4{c0, c1, c2, c3};
 }
 
-// the 16 bits of elements first .. first + 7, two a word; first need not be a multiple of eight
+// the 16 bits of elements first .. first + 7, two a word; EIGHT: first is a multiple of eight
+template <bool EIGHT>
 __device__ __forceinline__ u32x4 bits_of(uint64_t first, uint32_t site, uint64_t seed) {
     const u32x4 a = philox(first >> 3, site, seed);
     const int off = first & 7;
-    if (off == 0) return a;
+    if (EIGHT || off == 0) return a;
     const u32x4 b = philox((first >> 3) + 1, site, seed);
     uint32_t w[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 #pragma unroll
@@ -57,8 +58,9 @@ __device__ __forceinline__ u32x4 bits_of(uint64_t first, uint32_t site, uint64_t
 }
 
 // 1 / (1 - p) or 0 for eight elements
+template <bool EIGHT>
 __device__ __forceinline__ void mask_of(const Rng &g, uint64_t first, uint64_t seed, float (&m)[8]) {
-    const u32x4 w = bits_of(first, g.site, seed);
+    const u32x4 w = bits_of<EIGHT>(first, g.site, seed);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         m[2 * i] = (w[i] & 0xffffu) >= g.step ? g.keep : 0.f;
@@ -119,7 +121,7 @@ __global__ __launch_bounds__(NT) void dropout_kernel(const T *__restrict__ x, T 
     const int have = (int)min((int64_t)8, n - at);
     if (VEC && have == 8) load8<true>(x + at, 8, v);
     else load8<false>(x + at, have, v);
-    mask_of(g, at, rng_seed(g), m);
+    mask_of<true>(g, at, rng_seed(g), m);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = m[i] != 0.f ? v[i] * m[i] : 0.f;  // a dropped NaN is gone
     if (VEC && have == 8) store8<true>(y + at, 8, v);
@@ -132,7 +134,7 @@ struct Block {
     const void *x, *f, *gate, *post_w, *post_b, *pre_w, *pre_b, *dy, *dh;
     void *y, *h, *dx, *df, *dgate;
     float *stats, *part, *gpart;  // part [parts][4][C]; gpart [gate rows][splits][C]
-    int R, C, gate_rows, post, pre, param_f32, splits, want;  // want: bit k = column sum k
+    int R, C, gate_rows, post, pre, param_f32, splits, want;  // want: bit k: column sum k
     float scale, eps;
     Rng rng;
 };
@@ -147,297 +149,259 @@ __device__ __forceinline__ void param8(const void *p, int f32, int c, int n, flo
     else load8<VEC>(static_cast<const __bf16 *>(p) + c, n, v);
 }
 
+// A row has TPR threads of eight elements each: 16, 32 or 64 of a wave (the workgroup's 256 threads
+// then hold several rows), or a workgroup of TPR.  A row's waits are hidden by the other rows of its
+// CU, so the fewer registers and the more rows the better (rows of 4096 bf16, backward: 369 us with
+// 16 elements a thread and two waves a SIMD).
+template <int TPR> constexpr int threads() { return TPR > 64 ? TPR : NT; }
+
+// How a thread's elements are reached.  WHOLE: every thread of a row has eight, 16-byte aligned, and
+// the call is the usual one (both norms, both gradients in, the rows' gradients out): nothing is
+// asked per thread and little per call.  ALIGNED: eight or none.  SINGLE: one by one, any alignment.
+// (rows of 4096 bf16, backward: 900 vector instructions for eight elements without WHOLE)
+enum { SINGLE, ALIGNED, WHOLE };
+
 // sum over the TPR threads of a row, in every one of them
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float *lds) {
-    if constexpr (TPR == 16) return row_sum16(v);
     v = row_sum16(v);
-    v = fadd_rn(v, __shfl_xor(v, 16));
+    if constexpr (TPR >= 32) v = fadd_rn(v, __shfl_xor(v, 16));
     if constexpr (TPR >= 64) v = fadd_rn(v, __shfl_xor(v, 32));
     if constexpr (TPR > 64) {
         __syncthreads();
         if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
         __syncthreads();
-        v = fadd_rn(fadd_rn(lds[0], lds[1]), fadd_rn(lds[2], lds[3]));
+        v = lds[0];
+#pragma unroll
+        for (int w = 1; w < TPR / 64; ++w) v = fadd_rn(v, lds[w]);
     }
     return v;
 }
 
+// the thread's eight elements of a row, of which n > 0 are there; 0 beyond
+template <int MODE, class T>
+__device__ __forceinline__ void get8(const void *p, int64_t at, int n, float (&v)[8]) {
+    if (MODE == WHOLE || n > 0) {
+        load8<(MODE >= ALIGNED)>(static_cast<const T *>(p) + at, n, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    }
+}
+
 // mean and 1 / deviation of a row held in registers (two passes: the mean, then the squares
 // around it)
-template <int TPR, int NCH>
-__device__ __forceinline__ void row_stats(const float (&v)[NCH][8], int kind, int C, int c0, float eps, float &mu, float &rs,
+template <int TPR>
+__device__ __forceinline__ void row_stats(const float (&v)[8], int kind, float inv_c, int n, float eps, float &mu, float &rs,
                                           float *lds) {
     mu = 0.f;
     if (kind == 2) {
         float s = 0.f;
 #pragma unroll
-        for (int k = 0; k < NCH; ++k)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s += v[k][i];  // 0 beyond C
-        mu = row_sum<TPR>(s, lds) / (float)C;
+        for (int i = 0; i < 8; ++i) s += v[i];
+        mu = row_sum<TPR>(s, lds) * inv_c;
     }
     float s = 0.f;
 #pragma unroll
-    for (int k = 0; k < NCH; ++k)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float d = c0 + k * TPR * 8 + i < C ? v[k][i] - mu : 0.f;
-            s = __builtin_fmaf(d, d, s);
-        }
-    rs = 1.f / sqrtf(row_sum<TPR>(s, lds) / (float)C + eps);
+    for (int i = 0; i < 8; ++i) {
+        const float d = i < n ? v[i] - mu : 0.f;
+        s = __builtin_fmaf(d, d, s);
+    }
+    rs = 1.f / sqrtf(row_sum<TPR>(s, lds) * inv_c + eps);
 }
 
-// One row a TPR threads, NCH groups of eight elements a thread: every input is read once and
-// stays in registers through both norms.  Bound by its bytes.
-template <class T, int TPR, int NCH, bool VEC>
-__global__ __launch_bounds__(NT) void block_fwd(Block a) {
-    __shared__ float lds[4];
-    const int r = blockIdx.x * (NT / TPR) + threadIdx.x / TPR, C = a.C, c0 = threadIdx.x % TPR * 8;
+// Every input is read once and stays in registers through both norms.  Bound by its bytes.
+template <class T, int TPR, int MODE>
+__global__ __launch_bounds__(threads<TPR>()) void block_fwd(Block a) {
+    __shared__ float lds[16];
+    constexpr bool VEC = MODE >= ALIGNED, USUAL = MODE == WHOLE;
+    const int r = blockIdx.x * (threads<TPR>() / TPR) + threadIdx.x / TPR, C = a.C, c = threadIdx.x % TPR * 8;
+    const int n = USUAL ? 8 : C - c;
     if (TPR <= 64 && r >= a.R) return;
-    const int64_t row = (int64_t)r * C;
-    float y[NCH][8];
+    const int64_t at = (int64_t)r * C + c;
+    const float inv_c = 1.f / (float)C;
+    float y[8], mu = 0.f, rs = 1.f, mu2 = 0.f, rs2 = 1.f;
+    get8<MODE, T>(a.x, at, n, y);
+    if (USUAL || a.f) {
+        float u[8], w[8], b[8];
+        get8<MODE, T>(a.f, at, n, u);
+        if (USUAL || a.post) {
+            row_stats<TPR>(u, a.post, inv_c, n, a.eps, mu, rs, lds);
+            param8<VEC>(a.post_w, a.param_f32, c, n, 1.f, w);
+            param8<VEC>(a.post_b, a.param_f32, c, n, 0.f, b);
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) {
-        const int c = c0 + k * TPR * 8;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[k][i] = 0.f;
-        if (c < C) load8<VEC>(static_cast<const T *>(a.x) + row + c, C - c, y[k]);
-    }
-    float mu = 0.f, rs = 1.f, mu2 = 0.f, rs2 = 1.f;
-    if (a.f) {
-        float u[NCH][8];
-#pragma unroll
-        for (int k = 0; k < NCH; ++k) {
-            const int c = c0 + k * TPR * 8;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) u[k][i] = 0.f;
-            if (c < C) load8<VEC>(static_cast<const T *>(a.f) + row + c, C - c, u[k]);
+            for (int i = 0; i < 8; ++i) u[i] = __builtin_fmaf((u[i] - mu) * rs, w[i], b[i]);
         }
-        if (a.post) row_stats<TPR, NCH>(u, a.post, C, c0, a.eps, mu, rs, lds);
-        const uint64_t seed = a.rng.step ? rng_seed(a.rng) : 0;
-        const int64_t grow = a.gate ? (int64_t)(r / a.gate_rows) * C : 0;
-#pragma unroll
-        for (int k = 0; k < NCH; ++k) {
-            const int c = c0 + k * TPR * 8;
-            if (c >= C) continue;
-            float w[8], b[8], g[8], m[8];
-            if (a.post) {
-                param8<VEC>(a.post_w, a.param_f32, c, C - c, 1.f, w);
-                param8<VEC>(a.post_b, a.param_f32, c, C - c, 0.f, b);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) u[k][i] = __builtin_fmaf((u[k][i] - mu) * rs, w[i], b[i]);
-            }
-            if (a.rng.step) {
-                mask_of(a.rng, row + c, seed, m);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) u[k][i] = m[i] != 0.f ? u[k][i] * m[i] : 0.f;
-            }
-            if (a.gate) {
-                load8<VEC>(static_cast<const T *>(a.gate) + grow + c, C - c, g);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) u[k][i] *= g[i];
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[k][i] = c + i < C ? __builtin_fmaf(a.scale, u[k][i], y[k][i]) : 0.f;
-            store8<VEC>(static_cast<T *>(a.y) + row + c, C - c, y[k]);
-        }
-    }
-    if (a.pre) {
-        row_stats<TPR, NCH>(y, a.pre, C, c0, a.eps, mu2, rs2, lds);
-#pragma unroll
-        for (int k = 0; k < NCH; ++k) {
-            const int c = c0 + k * TPR * 8;
-            if (c >= C) continue;
-            float w[8], b[8];
-            param8<VEC>(a.pre_w, a.param_f32, c, C - c, 1.f, w);
-            param8<VEC>(a.pre_b, a.param_f32, c, C - c, 0.f, b);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = __builtin_fmaf((y[k][i] - mu2) * rs2, w[i], b[i]);
-            store8<VEC>(static_cast<T *>(a.h) + row + c, C - c, w);
-        }
-    }
-    if (a.stats && threadIdx.x % TPR == 0) *reinterpret_cast<f32x4_m *>(a.stats + 4 * (int64_t)r) = f32x4{mu, rs, mu2, rs2};
-}
-
-// Column sums of the backward pass, in this order: the four parameters' and the gate's.
-enum { S_POST_W, S_POST_B, S_PRE_W, S_PRE_B, S_GATE, NSUM };
-
-// Rows first + slot, first + slot + slots, ... < last: gradients of the rows, column sums in
-// registers.  The statistics are the forward pass's; everything else is computed again.
-// Bound by its bytes (f, y, dy, dh and the gate read, dx, df and the gate's gradient written).
-template <class T, int TPR, int NCH, bool VEC>
-__device__ __forceinline__ void back_row(const Block &a, int r, int c0, uint64_t seed, bool direct_gate, float *lds,
-                                         float (&sum)[NSUM][NCH][8]) {
-    const int C = a.C;
-    const int64_t row = (int64_t)r * C;
-    const f32x4 st = *reinterpret_cast<const f32x4_m *>(a.stats + 4 * (int64_t)r);
-    float dx[NCH][8], n[NCH][8], g[NCH][8];
-    float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-    for (int k = 0; k < NCH; ++k) {
-        const int c = c0 + k * TPR * 8;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) dx[k][i] = n[k][i] = g[k][i] = 0.f;
-        if (c >= C) continue;
-        if (a.dy) load8<VEC>(static_cast<const T *>(a.dy) + row + c, C - c, dx[k]);
-        if (a.pre && a.dh) {
-            float w[8];
-            load8<VEC>(static_cast<const T *>(a.dh) + row + c, C - c, g[k]);
-            load8<VEC>(static_cast<const T *>(a.y) + row + c, C - c, n[k]);
-            param8<VEC>(a.pre_w, a.param_f32, c, C - c, 1.f, w);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                n[k][i] = c + i < C ? (n[k][i] - st[2]) * st[3] : 0.f;
-                sum[S_PRE_W][k][i] = __builtin_fmaf(g[k][i], n[k][i], sum[S_PRE_W][k][i]);
-                sum[S_PRE_B][k][i] += g[k][i];
-                g[k][i] *= w[i];
-                if (c + i >= C) g[k][i] = 0.f;
-                s1 = __builtin_fmaf(g[k][i], n[k][i], s1);
-                s2 += g[k][i];
-            }
-        }
-    }
-    if (a.pre && a.dh) {
-        s1 = row_sum<TPR>(s1, lds) / (float)C;
-        s2 = a.pre == 2 ? row_sum<TPR>(s2, lds) / (float)C : 0.f;
-#pragma unroll
-        for (int k = 0; k < NCH; ++k)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) dx[k][i] += st[3] * (g[k][i] - n[k][i] * s1 - s2);
-    }
-#pragma unroll
-    for (int k = 0; k < NCH; ++k) {
-        const int c = c0 + k * TPR * 8;
-        if (c < C && a.dx) store8<VEC>(static_cast<T *>(a.dx) + row + c, C - c, dx[k]);
-    }
-    if (!a.f) return;
-    s1 = s2 = 0.f;
-    const int64_t grow = a.gate ? (int64_t)(r / a.gate_rows) * C : 0;
-#pragma unroll
-    for (int k = 0; k < NCH; ++k) {
-        const int c = c0 + k * TPR * 8;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) n[k][i] = g[k][i] = 0.f;
-        if (c >= C) continue;
-        float w[8], b[8], m[8], q[8];
-        load8<VEC>(static_cast<const T *>(a.f) + row + c, C - c, n[k]);
-        param8<VEC>(a.post_w, a.param_f32, c, C - c, 1.f, w);
-        param8<VEC>(a.post_b, a.param_f32, c, C - c, 0.f, b);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) g[k][i] = c + i < C ? dx[k][i] * a.scale : 0.f;
         if (a.rng.step) {
-            mask_of(a.rng, row + c, seed, m);
+            mask_of<VEC>(a.rng, at, rng_seed(a.rng), w);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) g[k][i] = m[i] != 0.f ? g[k][i] * m[i] : 0.f;
-        }
-        if (a.post) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) n[k][i] = c + i < C ? (n[k][i] - st[0]) * st[1] : 0.f;
+            for (int i = 0; i < 8; ++i) u[i] = w[i] != 0.f ? u[i] * w[i] : 0.f;
         }
         if (a.gate) {
-            load8<VEC>(static_cast<const T *>(a.gate) + grow + c, C - c, q);
-            float dg[8];
+            get8<MODE, T>(a.gate, (int64_t)(r / a.gate_rows) * C + c, n, w);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                dg[i] = g[k][i] * (a.post ? __builtin_fmaf(n[k][i], w[i], b[i]) : n[k][i]);
-                g[k][i] *= q[i];
-            }
-            if (direct_gate) {
-                if (a.dgate) store8<VEC>(static_cast<T *>(a.dgate) + row + c, C - c, dg);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sum[S_GATE][k][i] += dg[i];
-            }
+            for (int i = 0; i < 8; ++i) u[i] *= w[i];
         }
-        if (a.post) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                sum[S_POST_W][k][i] = __builtin_fmaf(g[k][i], n[k][i], sum[S_POST_W][k][i]);
-                sum[S_POST_B][k][i] += g[k][i];
-                g[k][i] = c + i < C ? g[k][i] * w[i] : 0.f;
-                s1 = __builtin_fmaf(g[k][i], n[k][i], s1);
-                s2 += g[k][i];
-            }
-        }
+        for (int i = 0; i < 8; ++i) y[i] = i < n ? __builtin_fmaf(a.scale, u[i], y[i]) : 0.f;
+        if (n > 0) store8<VEC>(static_cast<T *>(a.y) + at, n, y);
     }
-    if (a.post) {
-        s1 = row_sum<TPR>(s1, lds) / (float)C;
-        s2 = a.post == 2 ? row_sum<TPR>(s2, lds) / (float)C : 0.f;
-    }
-    if (!a.df) return;
+    if (USUAL || a.pre) {
+        float w[8], b[8];
+        row_stats<TPR>(y, a.pre, inv_c, n, a.eps, mu2, rs2, lds);
+        param8<VEC>(a.pre_w, a.param_f32, c, n, 1.f, w);
+        param8<VEC>(a.pre_b, a.param_f32, c, n, 0.f, b);
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) {
-        const int c = c0 + k * TPR * 8;
-        if (c >= C) continue;
-        if (a.post)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) g[k][i] = st[1] * (g[k][i] - n[k][i] * s1 - s2);
-        store8<VEC>(static_cast<T *>(a.df) + row + c, C - c, g[k]);
+        for (int i = 0; i < 8; ++i) w[i] = __builtin_fmaf((y[i] - mu2) * rs2, w[i], b[i]);
+        if (n > 0) store8<VEC>(static_cast<T *>(a.h) + at, n, w);
     }
+    if (a.stats && c == 0) *reinterpret_cast<f32x4_m *>(a.stats + 4 * (int64_t)r) = f32x4{mu, rs, mu2, rs2};
 }
 
-// One column sum of the workgroup's row slots, in slot order, to out[C] (f32)
-template <int TPR, int NCH>
-__device__ __forceinline__ void write_sum(float (&v)[NCH][8], float *out, int C, int c0, float *lds) {
-    constexpr int SLOTS = NT / TPR;
+// Column sums of the backward pass, in this order: the norms' weights and, where they are wanted
+// (FULL), their biases and a gate that several rows share.
+enum { S_POST_W, S_PRE_W, S_POST_B, S_PRE_B, S_GATE };
+template <bool FULL> constexpr int sums() { return FULL ? 5 : 2; }
+
+// One row's gradients; column sums stay in registers.  The statistics are the forward pass's,
+// everything else is computed again.  Bound by its bytes (f, y, dy, dh and the gate read, dx, df and
+// the gate's gradient written) and, with dropout, as much by the generator's arithmetic.
+template <class T, int TPR, int MODE, bool FULL>
+__device__ __forceinline__ void back_row(const Block &a, int r, int c, uint64_t seed, bool direct_gate, float inv_c, float *lds,
+                                         float (&sum)[sums<FULL>()][8]) {
+    constexpr bool VEC = MODE >= ALIGNED, USUAL = MODE == WHOLE;
+    const int C = a.C, n = USUAL ? 8 : C - c;
+    const int64_t at = (int64_t)r * C + c;
+    const f32x4 st = *reinterpret_cast<const f32x4_m *>(a.stats + 4 * (int64_t)r);
+    float dx[8], x[8], g[8], f[8], q[8], w[8], b[8];
+    // all of the row's reads first
+    const bool pre = USUAL || (a.pre && a.dh);
+    get8<MODE, T>(a.dy, at, USUAL || a.dy ? n : 0, dx);
+    get8<MODE, T>(a.dh, at, pre ? n : 0, g);
+    get8<MODE, T>(a.y, at, pre ? n : 0, x);
+    get8<MODE, T>(a.f, at, USUAL || a.f ? n : 0, f);
+    if (a.gate) get8<MODE, T>(a.gate, (int64_t)(r / a.gate_rows) * C + c, n, q);
+    if (pre) {
+        float s1 = 0.f, s2 = 0.f;
+        param8<VEC>(a.pre_w, a.param_f32, c, n, 1.f, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            x[i] = i < n ? (x[i] - st[2]) * st[3] : 0.f;
+            sum[S_PRE_W][i] = __builtin_fmaf(g[i], x[i], sum[S_PRE_W][i]);
+            if constexpr (FULL) sum[S_PRE_B][i] += g[i];
+            g[i] = i < n ? g[i] * w[i] : 0.f;
+            s1 = __builtin_fmaf(g[i], x[i], s1);
+            s2 += g[i];
+        }
+        s1 = row_sum<TPR>(s1, lds) * inv_c;
+        s2 = a.pre == 2 ? row_sum<TPR>(s2, lds) * inv_c : 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dx[i] = __builtin_fmaf(st[3], __builtin_fmaf(-x[i], s1, g[i] - s2), dx[i]);
+    }
+    if (n > 0 && (USUAL || a.dx)) store8<VEC>(static_cast<T *>(a.dx) + at, n, dx);
+    if (!USUAL && !a.f) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) g[i] = i < n ? dx[i] * a.scale : 0.f;
+    if (a.rng.step) {
+        mask_of<VEC>(a.rng, at, seed, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] = w[i] != 0.f ? g[i] * w[i] : 0.f;
+    }
+    const bool post = USUAL || a.post;
+    if (post) {
+        param8<VEC>(a.post_w, a.param_f32, c, n, 1.f, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = i < n ? (f[i] - st[0]) * st[1] : 0.f;
+    }
+    if (a.gate) {
+        float dg[8];
+        if (post) {
+            param8<VEC>(a.post_b, a.param_f32, c, n, 0.f, b);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) dg[i] = g[i] * __builtin_fmaf(f[i], w[i], b[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) dg[i] = g[i] * f[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] *= q[i];
+        if (direct_gate) {
+            if (n > 0 && a.dgate) store8<VEC>(static_cast<T *>(a.dgate) + at, n, dg);
+        } else if constexpr (FULL) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[S_GATE][i] += dg[i];
+        }
+    }
+    if (post) {
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            sum[S_POST_W][i] = __builtin_fmaf(g[i], f[i], sum[S_POST_W][i]);
+            if constexpr (FULL) sum[S_POST_B][i] += g[i];
+            g[i] = i < n ? g[i] * w[i] : 0.f;
+            s1 = __builtin_fmaf(g[i], f[i], s1);
+            s2 += g[i];
+        }
+        s1 = row_sum<TPR>(s1, lds) * inv_c;
+        s2 = a.post == 2 ? row_sum<TPR>(s2, lds) * inv_c : 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] = st[1] * __builtin_fmaf(-f[i], s1, g[i] - s2);
+    }
+    if (n > 0 && (USUAL || a.df)) store8<VEC>(static_cast<T *>(a.df) + at, n, g);
+}
+
+// One column sum of the workgroup's rows in flight, in their order, to out[C] (f32)
+template <int TPR>
+__device__ __forceinline__ void write_sum(float (&v)[8], float *out, int C, int c, float *lds) {
+    constexpr int SLOTS = threads<TPR>() / TPR;
     if constexpr (SLOTS > 1) {
+        __syncthreads();
 #pragma unroll
-        for (int k = 0; k < NCH; ++k) {
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) lds[threadIdx.x * 8 + i] = v[k][i];
-            __syncthreads();
-            for (int e = threadIdx.x; e < TPR * 8; e += NT) {
-                const int c = k * TPR * 8 + e;
-                float s = 0.f;
-                for (int t = 0; t < SLOTS; ++t) s += lds[t * TPR * 8 + e];
-                if (c < C) out[c] = s;
-            }
+        for (int i = 0; i < 8; ++i) lds[threadIdx.x * 8 + i] = v[i];
+        __syncthreads();
+        for (int e = threadIdx.x; e < TPR * 8; e += NT) {
+            float s = 0.f;
+            for (int t = 0; t < SLOTS; ++t) s += lds[t * TPR * 8 + e];
+            if (e < C) out[e] = s;
         }
     } else {
 #pragma unroll
-        for (int k = 0; k < NCH; ++k)
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (c0 + k * TPR * 8 + i < C) out[c0 + k * TPR * 8 + i] = v[k][i];
+        for (int i = 0; i < 8; ++i)
+            if (c + i < C) out[c + i] = v[i];
     }
 #pragma unroll
-    for (int k = 0; k < NCH; ++k)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[k][i] = 0.f;
+    for (int i = 0; i < 8; ++i) v[i] = 0.f;
 }
 
 // grid (splits, groups in flight).  A gate row's rows (all rows without a gate) are cut into
 // `splits` runs; the gate's column sum ends with each run, the parameters' run on.  With a gate
 // for each row the workgroups share all rows and write its gradient directly.
-template <class T, int TPR, int NCH, bool VEC>
-__global__ __launch_bounds__(NT) void block_bwd(Block a) {
-    __shared__ float lds[NT * 8];
-    constexpr int SLOTS = NT / TPR;
-    const int c0 = threadIdx.x % TPR * 8, slot = threadIdx.x / TPR;
+template <class T, int TPR, int MODE, bool FULL>
+__global__ __launch_bounds__(threads<TPR>()) void block_bwd(Block a) {
+    constexpr int SLOTS = threads<TPR>() / TPR, NSUM = sums<FULL>();
+    __shared__ float lds[SLOTS > 1 ? NT * 8 : 16];
+    const int c = threadIdx.x % TPR * 8, slot = threadIdx.x / TPR;
     const uint64_t seed = a.rng.step ? rng_seed(a.rng) : 0;
-    float sum[NSUM][NCH][8];
+    const float inv_c = 1.f / (float)a.C;
+    float sum[NSUM][8];
 #pragma unroll
     for (int s = 0; s < NSUM; ++s)
 #pragma unroll
-        for (int k = 0; k < NCH; ++k)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sum[s][k][i] = 0.f;
+        for (int i = 0; i < 8; ++i) sum[s][i] = 0.f;
     const bool direct = a.gate && a.gate_rows == 1;
     const int len = direct || !a.gate ? a.R : a.gate_rows, groups = a.R / len;
     for (int g = blockIdx.y; g < groups; g += gridDim.y) {
         const int run = (len + a.splits - 1) / a.splits;
         const int first = min((int)blockIdx.x * run, len), last = min(first + run, len);
         for (int r = first + slot; r < last; r += SLOTS)
-            back_row<T, TPR, NCH, VEC>(a, g * len + r, c0, seed, direct, lds, sum);
-        if (a.gpart)
-            write_sum<TPR, NCH>(sum[S_GATE], a.gpart + ((int64_t)g * a.splits + blockIdx.x) * a.C, a.C, c0, lds);
+            back_row<T, TPR, MODE, FULL>(a, g * len + r, c, seed, direct, inv_c, lds, sum);
+        if constexpr (FULL)
+            if (a.gpart) write_sum<TPR>(sum[S_GATE], a.gpart + ((int64_t)g * a.splits + blockIdx.x) * a.C, a.C, c, lds);
     }
     const int64_t part = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
 #pragma unroll
-    for (int s = 0; s < S_GATE; ++s)
-        if (a.want >> s & 1) write_sum<TPR, NCH>(sum[s], a.part + (part * 4 + s) * a.C, a.C, c0, lds);
+    for (int s = 0; s < (FULL ? S_GATE : NSUM); ++s)
+        if (a.want >> s & 1) write_sum<TPR>(sum[s], a.part + (part * 4 + s) * a.C, a.C, c, lds);
 }
 
 // out[s][c] = sum over n of in[s * stride_s + n * stride_n + c], eight lanes a column, one order
@@ -453,6 +417,7 @@ __global__ __launch_bounds__(NT) void sum_parts(Reduce a) {
     void *out = a.out_stride ? a.out[0] : a.out[s];
     float v = 0.f;
     if (c < a.C && out)
+#pragma unroll 8
         for (int n = lane; n < a.n; n += 8) v += a.in[s * a.stride_s + n * a.stride_n + c];
     lds[threadIdx.x] = v;
     __syncthreads();
@@ -472,17 +437,28 @@ Rng make_rng(uint32_t step, uint64_t seed, const uint64_t *dev, uint32_t site) {
 
 bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-// how the backward pass divides its rows: splits of a gate row's rows, gate rows in flight
+// threads of a row
+int row_threads(int C) { return C <= 128 ? 16 : C <= 256 ? 32 : C <= 512 ? 64 : C <= 1024 ? 128 : C <= 2048 ? 256 : C <= 4096 ? 512 : 1024; }
+
+// whether the backward pass sums more columns than the norms' weights
+bool full_sums(const hreg_tok_block_t *p) { return (p->gate && p->gate_rows > 1 && p->dgate) || p->dpost_b || p->dpre_b; }
+
+// How the backward pass divides its rows: splits of a gate row's rows, gate rows in flight.  As many
+// workgroups as the registers let run (12 or 16 waves a CU; rows of 4096 bf16, us: 240 with 16, 274
+// with 12, 247 with 24; rows of 1024 with biases 142 with 12, 178 with 16), but four rows a thread
+// at least: each workgroup's column sums are written and read once more.
 struct Plan { int splits, flight, groups; };
-Plan plan_of(int R, int gate_rows, bool gate) {
-    const int len = gate && gate_rows > 1 ? gate_rows : R, groups = len ? R / len : 0;
-    Plan p;
-    p.groups = groups;
-    p.flight = groups < 512 ? (groups > 0 ? groups : 1) : 512;
-    p.splits = 512 / p.flight;
-    if (p.splits > (len + 7) / 8) p.splits = (len + 7) / 8;
-    if (p.splits < 1) p.splits = 1;
-    return p;
+Plan plan_of(const hreg_tok_block_t *p) {
+    const int len = p->gate && p->gate_rows > 1 ? p->gate_rows : p->R, tpr = row_threads(p->C);
+    const int waves = tpr > 64 ? tpr / 64 : 4, slots = tpr > 64 ? 1 : NT / tpr, most = 256 * (full_sums(p) ? 12 : 16) / waves;
+    Plan q;
+    q.groups = len ? p->R / len : 0;
+    q.flight = q.groups < most ? (q.groups > 0 ? q.groups : 1) : most;
+    q.splits = most / q.flight;
+    const int rows = (len + 4 * slots - 1) / (4 * slots);
+    if (q.splits > rows) q.splits = rows;
+    if (q.splits < 1) q.splits = 1;
+    return q;
 }
 
 size_t part_bytes(const hreg_tok_block_t *p, const Plan &q) {
@@ -506,27 +482,41 @@ int take(const hreg_tok_block_t *p, Block &a) {
     return HREG_OK;
 }
 
-template <bool BACK, class T, int TPR, int NCH, bool VEC>
+template <bool BACK, class T, int TPR, int MODE>
 int go(const Block &a, const Plan &q, void *stream) {
+    const dim3 block(threads<TPR>());
     if constexpr (BACK) {
-        hipLaunchKernelGGL((block_bwd<T, TPR, NCH, VEC>), dim3(q.splits, q.flight), dim3(NT), 0, as_stream(stream), a);
+        const bool full = MODE == SINGLE || a.gpart || a.want >> S_POST_B;
+        if constexpr (MODE != SINGLE) {
+            if (!full) hipLaunchKernelGGL((block_bwd<T, TPR, MODE, false>), dim3(q.splits, q.flight), block, 0, as_stream(stream), a);
+        }
+        if (full) hipLaunchKernelGGL((block_bwd<T, TPR, MODE, true>), dim3(q.splits, q.flight), block, 0, as_stream(stream), a);
     } else {
-        constexpr int SLOTS = NT / TPR;
-        hipLaunchKernelGGL((block_fwd<T, TPR, NCH, VEC>), dim3((a.R + SLOTS - 1) / SLOTS), dim3(NT), 0, as_stream(stream), a);
+        constexpr int SLOTS = threads<TPR>() / TPR;
+        hipLaunchKernelGGL((block_fwd<T, TPR, MODE>), dim3((a.R + SLOTS - 1) / SLOTS), block, 0, as_stream(stream), a);
     }
     HREG_CHECK_LAUNCH();
     return HREG_OK;
 }
 
-template <bool BACK, class T, bool VEC>
-int by_width(const Block &a, const Plan &q, void *stream) {
-    if (a.C <= 128) return go<BACK, T, 16, 1, VEC>(a, q, stream);
-    if (a.C <= 256) return go<BACK, T, 32, 1, VEC>(a, q, stream);
-    if (a.C <= 512) return go<BACK, T, 64, 1, VEC>(a, q, stream);
-    if (a.C <= 1024) return go<BACK, T, 64, 2, VEC>(a, q, stream);
-    if (a.C <= 2048) return go<BACK, T, 256, 1, VEC>(a, q, stream);
-    if (a.C <= 4096) return go<BACK, T, 256, 2, VEC>(a, q, stream);
-    return go<BACK, T, 256, 4, VEC>(a, q, stream);
+template <bool BACK, class T, int TPR>
+int by_mode(const Block &a, int mode, const Plan &q, void *stream) {
+    return mode == WHOLE     ? go<BACK, T, TPR, WHOLE>(a, q, stream)
+           : mode == ALIGNED ? go<BACK, T, TPR, ALIGNED>(a, q, stream)
+                             : go<BACK, T, TPR, SINGLE>(a, q, stream);
+}
+
+template <bool BACK, class T>
+int by_width(const Block &a, int mode, const Plan &q, void *stream) {
+    switch (row_threads(a.C)) {
+        case 16: return by_mode<BACK, T, 16>(a, mode, q, stream);
+        case 32: return by_mode<BACK, T, 32>(a, mode, q, stream);
+        case 64: return by_mode<BACK, T, 64>(a, mode, q, stream);
+        case 128: return by_mode<BACK, T, 128>(a, mode, q, stream);
+        case 256: return by_mode<BACK, T, 256>(a, mode, q, stream);
+        case 512: return by_mode<BACK, T, 512>(a, mode, q, stream);
+        default: return by_mode<BACK, T, 1024>(a, mode, q, stream);
+    }
 }
 
 template <bool BACK>
@@ -535,9 +525,9 @@ int by_type(const hreg_tok_block_t *p, const Block &a, const Plan &q, void *stre
     for (const void *v : {a.x, a.f, a.gate, a.post_w, a.post_b, a.pre_w, a.pre_b, a.dy, a.dh, (const void *)a.y,
                           (const void *)a.h, (const void *)a.dx, (const void *)a.df, (const void *)a.dgate})
         vec = vec && aligned16(v);
-    if (p->dtype == HREG_TOK_F32)
-        return vec ? by_width<BACK, float, true>(a, q, stream) : by_width<BACK, float, false>(a, q, stream);
-    return vec ? by_width<BACK, __bf16, true>(a, q, stream) : by_width<BACK, __bf16, false>(a, q, stream);
+    const bool usual = a.f && a.post && a.pre && (!BACK || (a.dy && a.dh && a.dx && a.df));
+    const int mode = !vec ? SINGLE : usual && a.C == 8 * row_threads(a.C) ? WHOLE : ALIGNED;
+    return p->dtype == HREG_TOK_F32 ? by_width<BACK, float>(a, mode, q, stream) : by_width<BACK, __bf16>(a, mode, q, stream);
 }
 
 }  // namespace
@@ -571,7 +561,7 @@ int hreg_tok_dropout(const void *x, void *y, int64_t n, int dtype, uint32_t step
 
 size_t hreg_tok_block_ws_bytes(const hreg_tok_block_t *p) {
     if (!p || p->R < 1 || p->C < 1 || (p->gate && (p->gate_rows < 1 || p->R % p->gate_rows))) return 0;
-    const Plan q = plan_of(p->R, p->gate_rows, p->gate != nullptr);
+    const Plan q = plan_of(p);
     const bool sums = p->gate && p->gate_rows > 1;
     return part_bytes(p, q) + (sums ? (size_t)q.groups * q.splits * p->C * 4 : 0);
 }
@@ -590,7 +580,7 @@ int hreg_tok_block_bwd(const hreg_tok_block_t *p, void *stream) {
     int rc = take(p, a);
     if (rc != HREG_OK) return rc;
     const bool post = a.R == 0 || (a.f && a.post), pre = a.R == 0 || a.pre;
-    void *const out[4] = {post ? p->dpost_w : nullptr, post ? p->dpost_b : nullptr, pre ? p->dpre_w : nullptr,
+    void *const out[4] = {post ? p->dpost_w : nullptr, pre ? p->dpre_w : nullptr, post ? p->dpost_b : nullptr,
                           pre ? p->dpre_b : nullptr};
     for (int s = 0; s < 4; ++s) a.want |= (out[s] != nullptr) << s;
     Plan q{1, 1, 0};
@@ -598,7 +588,7 @@ int hreg_tok_block_bwd(const hreg_tok_block_t *p, void *stream) {
         if (!a.stats || !aligned16(a.stats) || (a.pre && !a.y)) return HREG_ERR_INVALID;
         const size_t need = hreg_tok_block_ws_bytes(p);
         if (!p->ws || p->ws_bytes < need || reinterpret_cast<uintptr_t>(p->ws) % 256) return HREG_ERR_INVALID;
-        q = plan_of(p->R, p->gate_rows, p->gate != nullptr);
+        q = plan_of(p);
         a.splits = q.splits;
         a.part = static_cast<float *>(p->ws);
         if (a.gate && a.gate_rows > 1 && a.dgate) a.gpart = reinterpret_cast<float *>(static_cast<char *>(p->ws) + part_bytes(p, q));
