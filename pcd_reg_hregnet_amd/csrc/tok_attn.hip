@@ -31,12 +31,16 @@ constexpr int MAX_BINS = 2049;   // offsets -max_distance .. max_distance with m
 // waves a SIMD hide each other's waits (2 x 4096 x 16 heads x 128 bf16, us: forward 387 with two, 572
 // with one), so long as nothing spills: f32 backward at 128 columns keeps 400 registers and one wave
 // (690 against 1770).  64 rows halve the barriers of 32, but at 128 columns the backward pass has no
-// registers for them (bf16, 746 us with 32, 1939 with 64).
+// registers for them (bf16 key gradients: 746 us with 32, 1939 with 64).  There the fragments'
+// addresses are made again at every tile too (TIGHT: 34 spilled registers become 4, 722 -> 660 us;
+// elsewhere it only costs instructions).
 template <class T, int DP>
 struct Shape {
     static constexpr bool F32 = Elem<T>::NP > 1;
     static constexpr int FWD_KEYS = F32 && DP > 32 ? 32 : 64, BWD_ROWS = F32 && DP > 32 ? 32 : DP > 64 ? 32 : 64;
+    static constexpr int Q_KEYS = F32 && DP > 32 ? 32 : 64;
     static constexpr int BWD_WAVES = F32 && DP > 64 ? 1 : 2;
+    static constexpr bool TIGHT = !F32 && DP > 64;
     static constexpr int SPLIT_WAVES = F32 && DP > 64 ? 1 : 2;
     // waves that share 32 rows in a small call (8 x 512 keys x 4 heads x 32 f32: 126 -> 78 us with 4;
     // 2 x 700 x 8 x 64 f32: 146 -> 99 with 2, 137 with 4, whose tiles leave one workgroup a CU)
@@ -338,6 +342,7 @@ __global__ __launch_bounds__(NT, 2) void attn_fwd(Args a) {
     const int kend = last < q0 ? 0 : a.causal ? min(sp.nk, max(last + sp.start + 1, 0)) : sp.nk;
     KV kv;
     kv.init(lds, a.D);
+    Lane<DP> at(lane);
     if (kend > 0) kv.issue(K, a.ks[1], V, a.vs[1], 0, sp.nk, a.D, mask);
     for (int j0 = 0; j0 < kend; j0 += KT) {
         kv.land(j0, sp.nk, mask);
@@ -353,7 +358,7 @@ __global__ __launch_bounds__(NT, 2) void attn_fwd(Args a) {
 #pragma unroll
             for (int c = 0; c < DP / 16; ++c) {
                 bf16x8 kf[NP];
-                row_frag<DP>(kt, PLANE, 32 * t, c, lane, kf);
+                row_frag<DP>(kt, PLANE, 32 * t, c, at, kf);
                 mma<NP>(s[t], kf, qf[c]);
             }
         }
@@ -396,7 +401,7 @@ __global__ __launch_bounds__(NT, 2) void attn_fwd(Args a) {
 #pragma unroll
                 for (int d = 0; d < DP / 32; ++d) {
                     bf16x8 vf[NP];
-                    col_frag<DP>(vt, PLANE, 32 * t + 16 * c, 32 * d, lane, vf);
+                    col_frag<DP>(vt, PLANE, 32 * t + 16 * c, 32 * d, at, vf);
                     mma<NP>(acc[d], vf, pf);
                 }
             }
@@ -490,6 +495,7 @@ __global__ __launch_bounds__(NT, (Shape<T, DP>::SPLIT_WAVES)) void attn_split(Ar
     const int run = ((kend + a.splits - 1) / a.splits + 127) / 128 * 128;
     const int j_end = min(kend, (split + 1) * run);
     int j0 = split * run + 32 * wave;
+    const Lane<DP> at(lane);
     WaveStage<T, DP> sk, sv;
     if (j0 < j_end) {
         sk.load(K, a.ks[1], j0, sp.nk, a.D, mask, lane);
@@ -503,7 +509,7 @@ __global__ __launch_bounds__(NT, (Shape<T, DP>::SPLIT_WAVES)) void attn_split(Ar
 #pragma unroll
         for (int c = 0; c < DP / 16; ++c) {
             bf16x8 kf[NP];
-            row_frag<DP>(buf, PLANE, 0, c, lane, kf);
+            row_frag<DP>(buf, PLANE, 0, c, at, kf);
             mma<NP>(s, kf, qf[c]);
         }
         const int kpos = j0 - (i + sp.start);
@@ -556,7 +562,7 @@ __global__ __launch_bounds__(NT, (Shape<T, DP>::SPLIT_WAVES)) void attn_split(Ar
 #pragma unroll
             for (int d = 0; d < DP / 32; ++d) {
                 bf16x8 vf[NP];
-                col_frag<DP>(buf, PLANE, 16 * c, 32 * d, lane, vf);
+                col_frag<DP>(buf, PLANE, 16 * c, 32 * d, at, vf);
                 mma<NP>(acc[d], vf, pf);
             }
         }
@@ -635,25 +641,38 @@ __global__ __launch_bounds__(NT) void attn_join(Args a) {
 
 // ---------------------------------------------------------------------- backward --
 
-// delta[b][h][i] = do_i . o_i: 16 lanes a row.  Bound by its reads.
-template <class T>
-__global__ __launch_bounds__(NT) void attn_delta(Args a) {
-    const int64_t rows = (int64_t)a.B * a.H * a.Nq, row = (int64_t)blockIdx.x * (NT / 16) + threadIdx.x / 16;
-    if (row >= rows) return;
-    const int i = row % a.Nq, h = row / a.Nq % a.H, b = row / a.Nq / a.H, d = threadIdx.x % 16 * 8;
+// D_i = do_i . o_i of the lane's row, half of it each in lanes l and l + 32.  o and what it lost in
+// rounding (bf16): that error would be common to a row's ds.
+template <class T, int DP>
+__device__ __forceinline__ float row_dot(const Args &a, int b, int h, int i, bool ok, int lane) {
+    const T *x = static_cast<const T *>(a.dout) + b * a.dos[0] + (int64_t)i * a.dos[1] + h * a.dos[2];
+    const T *y = static_cast<const T *>(a.out_r) + b * a.os[0] + (int64_t)i * a.os[1] + h * a.os[2];
+    const T *z = static_cast<const T *>(a.rest) + (((int64_t)b * a.Nq + i) * a.H + h) * a.D;
     float s = 0.f;
-    if (d < a.D && i < span_of(a, b).nq) {
-        Chunk<T> x, y;
-        x.load(static_cast<const T *>(a.dout) + b * a.dos[0] + (int64_t)i * a.dos[1] + h * a.dos[2] + d);
-        y.load(static_cast<const T *>(a.out_r) + b * a.os[0] + (int64_t)i * a.os[1] + h * a.os[2] + d);
-        s = x.dot(y);
-        if (a.rest) {  // what out lost in rounding: it would be common to a row's ds
-            y.load(static_cast<const T *>(a.rest) + (((int64_t)b * a.Nq + i) * a.H + h) * a.D + d);
-            s += x.dot(y);
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+        const int d = 16 * c + 8 * (lane >> 5);
+        if (!ok || d >= a.D) continue;
+        Chunk<T> u, v;
+        u.load(x + d);
+        v.load(y + d);
+        s += u.dot(v);
+        if (a.rest) {
+            v.load(z + d);
+            s += u.dot(v);
         }
     }
-    s = row_sum16(s);
-    if (threadIdx.x % 16 == 0) a.delta[row] = s;
+    return s + __shfl_xor(s, 32);
+}
+
+// the same for a call that wants no query gradients: delta[b][h][i], 32 rows a wave
+template <class T, int DP>
+__global__ __launch_bounds__(NT) void attn_delta(Args a) {
+    const int64_t rows = (int64_t)a.B * a.H * a.Nq, row = (int64_t)blockIdx.x * (NT / 2) + threadIdx.x / 64 * 32 + threadIdx.x % 32;
+    const bool in = row < rows;
+    const int i = in ? row % a.Nq : 0, h = in ? row / a.Nq % a.H : 0, b = in ? row / a.Nq / a.H : 0;
+    const float s = row_dot<T, DP>(a, b, h, i, in && i < span_of(a, b).nq, threadIdx.x & 63);
+    if (in && threadIdx.x % 64 < 32) a.delta[row] = s;
 }
 
 // dk, dv of 128 keys: every wave keeps 32 keys and walks all rows of all heads that share them, so
@@ -686,6 +705,7 @@ __global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::BWD_WAVES : 1)) void a
     const int G = a.H / a.Hk;
     QD qd;
     qd.init(lds, a.D);
+    Lane<DP> at(lane);
     const int g0 = w0.h % a.groups * (G / a.groups);
     if (w.tile * ROWS < sp.nk)
         for (int g = g0; g < g0 + G / a.groups; ++g) {
@@ -709,6 +729,7 @@ __global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::BWD_WAVES : 1)) void a
                 }
                 qd.land(i0, sp.nq, nullptr);
                 const uint16_t *qt = qd.x(), *dt = qd.y();
+                if constexpr (Shape<T, DP>::TIGHT) at.opaque();
                 if (i0 + QT < sp.nq) qd.issue(Q, a.qs[1], dO, a.dos[1], i0 + QT, sp.nq, a.D, nullptr);
 #pragma unroll
                 for (int u = 0; u < QT / 32 / KW; ++u) {
@@ -722,9 +743,9 @@ __global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::BWD_WAVES : 1)) void a
 #pragma unroll
                     for (int c = 0; c < DP / 16; ++c) {
                         bf16x8 f[NP];
-                        row_frag<DP>(qt, PLANE, 32 * t, c, lane, f);
+                        row_frag<DP>(qt, PLANE, 32 * t, c, at, f);
                         mma<NP>(s, f, kf[c]);
-                        row_frag<DP>(dt, PLANE, 32 * t, c, lane, f);
+                        row_frag<DP>(dt, PLANE, 32 * t, c, at, f);
                         mma<NP>(dp, f, vf[c]);
                     }
 #pragma unroll
@@ -745,9 +766,9 @@ __global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::BWD_WAVES : 1)) void a
 #pragma unroll
                         for (int d = 0; d < DP / 32; ++d) {
                             bf16x8 f[NP];
-                            col_frag<DP>(dt, PLANE, 32 * t + 16 * c, 32 * d, lane, f);
+                            col_frag<DP>(dt, PLANE, 32 * t + 16 * c, 32 * d, at, f);
                             mma<NP>(dv[d], f, pf);
-                            col_frag<DP>(qt, PLANE, 32 * t + 16 * c, 32 * d, lane, f);
+                            col_frag<DP>(qt, PLANE, 32 * t + 16 * c, 32 * d, at, f);
                             mma<NP>(dk[d], f, sf);
                         }
                     }
@@ -920,7 +941,8 @@ __global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::BWD_WAVES : 1)) void a
     const float sign = odd ? -1.f : 1.f;
     const size_t row = ((size_t)w.b * a.H + w.h) * a.Nq + i;
     const RowSum rs = row_sum_of<T>(a, row, i < sp.nq);
-    const float delta = i < sp.nq ? a.delta[row] : 0.f;
+    const float delta = row_dot<T, DP>(a, w.b, w.h, i, i < sp.nq, lane);
+    if (half == 0 && share == 0 && i < a.Nq) a.delta[row] = delta;  // (the key gradients read it)
     const float scale2 = a.scale * LOG2E;
     f32x16 acc[DP / 32];
 #pragma unroll
@@ -930,10 +952,12 @@ __global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::BWD_WAVES : 1)) void a
     const int kend = last < q0 ? 0 : a.causal ? min(sp.nk, max(last + sp.start + 1, 0)) : sp.nk;
     KV kv;
     kv.init(lds, a.D);
+    Lane<DP> at(lane);
     if (kend > 0) kv.issue(K, a.ks[1], V, a.vs[1], 0, sp.nk, a.D, mask);
     for (int j0 = 0; j0 < kend; j0 += KT) {
         kv.land(j0, sp.nk, mask);
         const uint16_t *kt = kv.x(), *vt = kv.y();
+        if constexpr (Shape<T, DP>::TIGHT) at.opaque();
         if (j0 + KT < kend) kv.issue(K, a.ks[1], V, a.vs[1], j0 + KT, sp.nk, a.D, mask);
         const int qw = q0 + 32 * (wave / KW) + sp.start;
 #pragma unroll
@@ -945,9 +969,9 @@ __global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::BWD_WAVES : 1)) void a
 #pragma unroll
             for (int c = 0; c < DP / 16; ++c) {
                 bf16x8 f[NP];
-                row_frag<DP>(kt, PLANE, 32 * t, c, lane, f);
+                row_frag<DP>(kt, PLANE, 32 * t, c, at, f);
                 mma<NP>(s, f, qf[c]);
-                row_frag<DP>(vt, PLANE, 32 * t, c, lane, f);
+                row_frag<DP>(vt, PLANE, 32 * t, c, at, f);
                 mma<NP>(dp, f, df[c]);
             }
             if constexpr (BIAS) {
@@ -973,7 +997,7 @@ __global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::BWD_WAVES : 1)) void a
 #pragma unroll
                 for (int d = 0; d < DP / 32; ++d) {
                     bf16x8 f[NP];
-                    col_frag<DP>(kt, PLANE, 32 * t + 16 * c, 32 * d, lane, f);
+                    col_frag<DP>(kt, PLANE, 32 * t + 16 * c, 32 * d, at, f);
                     mma<NP>(acc[d], f, sf);
                 }
             }
@@ -1037,12 +1061,13 @@ __global__ __launch_bounds__(NT) void bias_reduce(Args a) {
         if (bucket_of(a.bk, o - far) == n) atomicMin(&from, o), atomicMax(&to, o + 1);
     __syncthreads();
     const int lo = from, w = to - lo, parts = a.B * tiles;  // (no offset: w <= 0)
+    int bits = 0;  // 2^bits threads go along the offsets, the others along the parts
+    while (bits < 8 && 1 << bits < w) ++bits;
     double s = 0.;
-    if (w > 0)
-        for (int64_t e = threadIdx.x; e < (int64_t)parts * w; e += NT) {
-            const int p = e / w, b = p / tiles, t = p % tiles;
-            s += a.bins[(((size_t)b * a.H + h) * tiles + t) * W + lo + e % w];
-        }
+    for (int p = threadIdx.x >> bits; p < parts; p += NT >> bits) {
+        const float *from_p = a.bins + (((size_t)(p / tiles) * a.H + h) * tiles + p % tiles) * W + lo;
+        for (int o = threadIdx.x & ((1 << bits) - 1); o < w; o += 1 << bits) s += from_p[o];
+    }
     sum[threadIdx.x] = s;
     __syncthreads();
     for (int k = NT / 2; k > 0; k >>= 1) {
@@ -1144,7 +1169,7 @@ int bwd_kv(const Args &a, void *stream) {
 }
 template <class T, int DP, int KW, bool BIAS>
 int bwd_q(const Args &a, void *stream) {
-    constexpr int KT = KW > 1 ? 32 * KW : Shape<T, DP>::BWD_ROWS;
+    constexpr int KT = KW > 1 ? 32 * KW : Shape<T, DP>::Q_KEYS;
     const size_t W = 2 * a.bk.far + 1, lds = area<T, DP, KT, KW, 1>() + (BIAS ? W + 2 * PAD + 4 * W : 0) * 4;
     return launch(attn_bwd_q<T, DP, KT, KW, BIAS>, a.B * a.H * ((a.Nq + a.tile_rows - 1) / a.tile_rows), lds, stream, a);
 }
@@ -1153,12 +1178,15 @@ template <class T, int DP, bool BIAS>
 int bwd(const Args &a, void *stream) {
     constexpr int SHARE = Shape<T, DP>::SHARE;
     int rc = HREG_OK;
-    if (a.Nq > 0) {
+    // the query gradients' kernel first: it leaves the rows' dots for the key gradients
+    if (a.Nq > 0 && (a.dq || a.dbias)) {
+        rc = a.tile_rows < ROWS ? bwd_q<T, DP, SHARE, BIAS>(a, stream) : bwd_q<T, DP, 1, BIAS>(a, stream);
+    } else if (a.Nq > 0) {
         const int64_t rows = (int64_t)a.B * a.H * a.Nq;
-        hipLaunchKernelGGL(attn_delta<T>, dim3((rows + NT / 16 - 1) / (NT / 16)), dim3(NT), 0, as_stream(stream), a);
+        hipLaunchKernelGGL((attn_delta<T, DP>), dim3((rows + NT / 2 - 1) / (NT / 2)), dim3(NT), 0, as_stream(stream), a);
         HREG_CHECK_LAUNCH();
     }
-    if (a.Nk > 0 && a.dk) {
+    if (rc == HREG_OK && a.Nk > 0 && a.dk) {
         rc = a.share_kv ? bwd_kv<T, DP, SHARE, BIAS>(a, stream) : bwd_kv<T, DP, 1, BIAS>(a, stream);
         if (rc == HREG_OK && a.groups > 1) {
             const int64_t n = (int64_t)a.B * a.Nk * a.Hk * (a.D / 4);
@@ -1166,8 +1194,6 @@ int bwd(const Args &a, void *stream) {
             HREG_CHECK_LAUNCH();
         }
     }
-    if (rc == HREG_OK && a.Nq > 0 && (a.dq || a.dbias))
-        rc = a.tile_rows < ROWS ? bwd_q<T, DP, SHARE, BIAS>(a, stream) : bwd_q<T, DP, 1, BIAS>(a, stream);
     return rc;
 }
 

@@ -95,27 +95,38 @@ __device__ __forceinline__ int swz(int r) {
 template <int DP>
 __device__ __forceinline__ int tile_at(int r, int chunk) { return r * DP + ((chunk ^ swz<DP>(r)) << 3); }
 
+// Where a lane's fragments start in a tile.  The permutation only flips bits of the chunk, so every
+// other fragment is this one with constant bits flipped and a constant added.  opaque() keeps the
+// compiler from holding all those addresses in registers across a loop.
+template <int DP>
+struct Lane {
+    int row, col;
+    __device__ __forceinline__ Lane(int lane) {
+        row = tile_at<DP>(lane & 31, lane >> 5);
+        const int i = lane & 15, g = lane >> 4;
+        col = tile_at<DP>(4 * (g >> 1) + (i >> 2), 2 * (g & 1) + ((i & 3) >> 1)) + (i & 1) * 4;
+    }
+    __device__ __forceinline__ void opaque() { asm volatile("" : "+v"(row), "+v"(col)); }
+};
+
 // operand with one tile row per lane (depth along the row): rows row0 .. +31, depth chunk c
 template <int DP, int NP>
-__device__ __forceinline__ void row_frag(const uint16_t *t, int plane, int row0, int c, int lane, bf16x8 (&p)[NP]) {
-    const int at = tile_at<DP>(row0 + (lane & 31), 2 * c + (lane >> 5));
+__device__ __forceinline__ void row_frag(const uint16_t *t, int plane, int row0, int c, const Lane<DP> &at, bf16x8 (&p)[NP]) {
+    const uint16_t *from = t + (at.row ^ (c << 4)) + row0 * DP;
 #pragma unroll
-    for (int s = 0; s < NP; ++s) p[s] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4_m *>(t + s * plane + at));
+    for (int s = 0; s < NP; ++s) p[s] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4_m *>(from + s * plane));
 }
 
 // operand with one tile column per lane (depth along the rows): columns col0 .. +31, rows row0
 // .. +15 in the order in which an MFMA result holds them (registers 8c .. 8c + 7 of half h are
 // rows 16c + 4h + {0..3, 8..11}), so a result is the other operand without any exchange.
 template <int DP, int NP>
-__device__ __forceinline__ void col_frag(const uint16_t *t, int plane, int row0, int col0, int lane, bf16x8 (&p)[NP]) {
-    const int i = lane & 15, g = lane >> 4;
-    const int col = col0 + 16 * (g & 1) + 4 * (i & 3);
-    const int r0 = row0 + 4 * (g >> 1) + (i >> 2), r1 = r0 + 8;
-    const int a0 = tile_at<DP>(r0, col >> 3) + (col & 7), a1 = tile_at<DP>(r1, col >> 3) + (col & 7);
+__device__ __forceinline__ void col_frag(const uint16_t *t, int plane, int row0, int col0, const Lane<DP> &at, bf16x8 (&p)[NP]) {
+    const uint16_t *from = t + (at.col ^ col0) + row0 * DP, *next = t + (at.col ^ col0 ^ 16) + (row0 + 8) * DP;
 #pragma unroll
     for (int s = 0; s < NP; ++s) {
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(t + s * plane + a0));
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(t + s * plane + a1));
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(from + s * plane));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(next + s * plane));
         p[s] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
 }
