@@ -29,17 +29,19 @@ constexpr int MAX_BINS = 2049;   // offsets -max_distance .. max_distance with m
 
 // Rows of a tile that goes through LDS, and the waves a SIMD that the registers are cut to.  Two
 // waves a SIMD hide each other's waits (2 x 4096 x 16 heads x 128 bf16, us: forward 387 with two, 572
-// with one), so long as nothing spills: f32 backward at 128 columns keeps 400 registers and one wave
-// (690 against 1770).  64 rows halve the barriers of 32, but at 128 columns the backward pass has no
-// registers for them (bf16 key gradients: 746 us with 32, 1939 with 64).  There the fragments'
-// addresses are made again at every tile too (TIGHT: 34 spilled registers become 4, 722 -> 660 us;
-// elsewhere it only costs instructions).
+// with one; key gradients and the rest of the backward pass 964 and 1120) as long as little spills:
+// f32 backward at 128 columns keeps 400 registers (620 us with one wave, 1770 with two), f32 key
+// gradients at 64 columns and bf16 ones at 128 with a bias keep 300 (214 / 260, 451 / 531).  64 rows
+// halve the barriers of 32, but at 128 columns the key gradients have no registers for them (746 us
+// with 32, 1939 with 64).  There the fragments' addresses are made again at every tile too (TIGHT:
+// 34 spilled registers become 4, 722 -> 660 us; elsewhere it only costs instructions).
 template <class T, int DP>
 struct Shape {
     static constexpr bool F32 = Elem<T>::NP > 1;
     static constexpr int FWD_KEYS = F32 && DP > 32 ? 32 : 64, BWD_ROWS = F32 && DP > 32 ? 32 : DP > 64 ? 32 : 64;
     static constexpr int Q_KEYS = F32 && DP > 32 ? 32 : 64;
-    static constexpr int BWD_WAVES = F32 && DP > 64 ? 1 : 2;
+    static constexpr int FWD_WAVES = F32 && DP > 64 ? 1 : 2, Q_WAVES = FWD_WAVES;
+    static constexpr int KV_WAVES = F32 && DP > 32 ? 1 : 2, KV_BIAS_WAVES = DP > (F32 ? 32 : 64) ? 1 : 2;
     static constexpr bool TIGHT = !F32 && DP > 64;
     static constexpr int SPLIT_WAVES = F32 && DP > 64 ? 1 : 2;
     // waves that share 32 rows in a small call (8 x 512 keys x 4 heads x 32 f32: 126 -> 78 us with 4;
@@ -234,8 +236,8 @@ __device__ __forceinline__ RowSum row_sum_of(const Args &a, size_t row, bool ok)
     return r;
 }
 template <class T>
-__device__ __forceinline__ float prob(float s, float ref, float inv) {
-    const float p = __builtin_amdgcn_exp2f(s - ref);
+__device__ __forceinline__ float prob(float x, float inv) {  // x = s - ref
+    const float p = __builtin_amdgcn_exp2f(x);
     return Elem<T>::NP == 1 ? p : p * inv;
 }
 
@@ -274,16 +276,21 @@ constexpr size_t area() {
     return tiles > join ? tiles : join;
 }
 
-// keys that the lane's query does not see: -inf.  krow = index of the first key; seen: bit k = key
-// krow + k exists and is not masked
-__device__ __forceinline__ void hide(const Args &a, f32x16 &s, int kpos, uint32_t seen, int half) {
+// Which of 32 keys the lane's query sees, bit 8 (r >> 2) + (r & 3) for register r of its half.  kpos =
+// position of the first key - the query's; seen: bit k = key k exists and is not masked
+__device__ __forceinline__ uint32_t visible(const Args &a, int kpos, uint32_t seen, int half) {
     if (a.causal) {  // the keys up to the query's own position
         const int n = min(max(1 - kpos, 0), 32);
         seen &= n == 32 ? ~0u : (1u << n) - 1;
     }
-    seen >>= 4 * half;
+    return seen >> (4 * half);
+}
+// registers whose bit is 0 become v (only on the edge tiles, hence the empty asm: without it the
+// compiler makes the selections everywhere)
+__device__ __forceinline__ void keep_only(f32x16 &s, uint32_t bits, float v) {
+    asm volatile("");
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = seen >> (8 * (r >> 2) + (r & 3)) & 1 ? s[r] : -INFINITY;
+    for (int r = 0; r < 16; ++r) s[r] = bits >> (8 * (r >> 2) + (r & 3)) & 1 ? s[r] : v;
 }
 __device__ __forceinline__ uint32_t seen_keys(int krow, int nk, const uint8_t *mask) {
     if (!mask) return krow + 32 <= nk ? ~0u : krow >= nk ? 0u : (1u << (nk - krow)) - 1;
@@ -310,7 +317,7 @@ __device__ __forceinline__ void finish_row(const Args &a, int b, int i, int h, i
 
 // 128 rows of one head, 32 a wave: the columns of its scores are its queries.
 template <class T, int DP, int KT, bool BIAS>
-__global__ __launch_bounds__(NT, 2) void attn_fwd(Args a) {
+__global__ __launch_bounds__(NT, (Shape<T, DP>::FWD_WAVES)) void attn_fwd(Args a) {
     constexpr int NP = Elem<T>::NP, MT = KT / 32, PLANE = KT * DP;
     extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
     typedef Tiles<T, DP, KT> KV;
@@ -353,21 +360,22 @@ __global__ __launch_bounds__(NT, 2) void attn_fwd(Args a) {
         const bool edge = mask || j0 + KT > sp.nk || (a.causal && j0 + KT - 1 > qw);
         f32x16 s[MT];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            s[t] = zero16();
+        for (int t = 0; t < MT; ++t) s[t] = zero16();
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) {
+        for (int c = 0; c < DP / 16; ++c)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
                 bf16x8 kf[NP];
                 row_frag<DP>(kt, PLANE, 32 * t, c, at, kf);
                 mma<NP>(s[t], kf, qf[c]);
             }
-        }
+        if constexpr (NP == 1) interleave<MT * DP / 16, 1, 2>();
         const int kpos = j0 - (i + sp.start);
         float top = m;
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
             if constexpr (BIAS) add_bias(s[t], scale2, tab, a.bk.far, j0 + 32 * t - qw, kpos + 32 * t, half);
-            if (edge) hide(a, s[t], kpos + 32 * t, seen_keys(j0 + 32 * t, sp.nk, mask), half);
+            if (edge) keep_only(s[t], visible(a, kpos + 32 * t, seen_keys(j0 + 32 * t, sp.nk, mask), half), -INFINITY);
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
         }
@@ -405,6 +413,7 @@ __global__ __launch_bounds__(NT, 2) void attn_fwd(Args a) {
                     mma<NP>(acc[d], vf, pf);
                 }
             }
+        if constexpr (NP == 1) interleave<MT * DP / 16, 2, 4>();
     }
     l += __shfl_xor(l, 32);
     if (i >= a.Nq) return;
@@ -531,7 +540,7 @@ __global__ __launch_bounds__(NT, (Shape<T, DP>::SPLIT_WAVES)) void attn_split(Ar
                 s[e] = __builtin_fmaf(s[e], scale2, bias_at(a, bucket_of(a.bk, o), r < R ? h : w.h * G) * LOG2E);
             }
         }
-        if (edge) hide(a, s, kpos, seen_keys(j0, sp.nk, mask), half);
+        if (edge) keep_only(s, visible(a, kpos, seen_keys(j0, sp.nk, mask), half), -INFINITY);
 #pragma unroll
         for (int e = 0; e < 16; ++e) top = fmaxf(top, s[e]);
         top = fmaxf(top, __shfl_xor(top, 32));
@@ -681,12 +690,12 @@ __global__ __launch_bounds__(NT) void attn_delta(Args a) {
 // KW waves share 32 keys, each taking every KW-th 32 rows (a small call has few keys to give a wave
 // of its own): their sums join in LDS, in wave order.
 template <class T, int DP, int QT, int KW, bool BIAS>
-__global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::BWD_WAVES : 1)) void attn_bwd_kv(Args a) {
+__global__ __launch_bounds__(NT, (KW > 1 ? 1 : BIAS ? Shape<T, DP>::KV_BIAS_WAVES : Shape<T, DP>::KV_WAVES)) void attn_bwd_kv(Args a) {
     constexpr int NP = Elem<T>::NP, PLANE = QT * DP, ROWS = 128 / KW;
     static_assert(QT % (32 * KW) == 0, "tile");
     extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
     typedef Tiles<T, DP, QT> QD;
-    float *lt = reinterpret_cast<float *>(reinterpret_cast<char *>(lds) + area<T, DP, QT, KW, 2>()), *et = lt + QT, *it = et + QT, *tab = it + QT;
+    float *lt = reinterpret_cast<float *>(reinterpret_cast<char *>(lds) + area<T, DP, QT, KW, 2>()), *et = lt + QT, *it = et + QT, *tab = lt + 6 * QT;
     const Where w0 = where(a.B, a.Hk * a.groups, (a.Nk + ROWS - 1) / ROWS);
     const Where w{w0.b, w0.h / a.groups, w0.tile};
     const Span sp = span_of(a, w.b);
@@ -713,24 +722,31 @@ __global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::BWD_WAVES : 1)) void a
             const T *Q = static_cast<const T *>(a.q) + w.b * a.qs[0] + h * a.qs[2];
             const T *dO = static_cast<const T *>(a.dout) + w.b * a.dos[0] + h * a.dos[2];
             const size_t row0 = ((size_t)w.b * a.H + h) * a.Nq;
-            if constexpr (BIAS) {
-                __syncthreads();
-                fill_table(a, tab, h);
-            }
+            __syncthreads();  // the last head's table and rows are read
+            if constexpr (BIAS) fill_table(a, tab, h);
             if (first < sp.nq) qd.issue(Q, a.qs[1], dO, a.dos[1], first, sp.nq, a.D, nullptr);
-            for (int i0 = first; i0 < sp.nq; i0 += QT) {
-                __syncthreads();
-                if (threadIdx.x < QT) {
-                    const int i = i0 + threadIdx.x;
-                    const RowSum rs = row_sum_of<T>(a, row0 + i, i < sp.nq);
-                    lt[threadIdx.x] = rs.ref;
-                    it[threadIdx.x] = rs.inv;
-                    et[threadIdx.x] = i < sp.nq ? a.delta[row0 + i] : 0.f;
-                }
+            // the rows' sums and dots go through registers into one of two buffers, a tile ahead: a
+            // load that is waited for at each tile costs as much as the tile
+            RowSum rs{INFINITY, 0.f};
+            float dot = 0.f;
+            const bool mine = threadIdx.x < QT;
+            if (mine && first < sp.nq) {
+                const int i = first + threadIdx.x;
+                rs = row_sum_of<T>(a, row0 + i, i < sp.nq);
+                lt[threadIdx.x] = -rs.ref;
+                it[threadIdx.x] = rs.inv;
+                et[threadIdx.x] = i < sp.nq ? a.delta[row0 + i] : 0.f;
+            }
+            for (int i0 = first, now = 0; i0 < sp.nq; i0 += QT, now ^= 3 * QT) {
                 qd.land(i0, sp.nq, nullptr);
                 const uint16_t *qt = qd.x(), *dt = qd.y();
                 if constexpr (Shape<T, DP>::TIGHT) at.opaque();
-                if (i0 + QT < sp.nq) qd.issue(Q, a.qs[1], dO, a.dos[1], i0 + QT, sp.nq, a.D, nullptr);
+                if (i0 + QT < sp.nq) {
+                    qd.issue(Q, a.qs[1], dO, a.dos[1], i0 + QT, sp.nq, a.D, nullptr);
+                    const int i = i0 + QT + threadIdx.x;
+                    rs = row_sum_of<T>(a, row0 + i, mine && i < sp.nq);
+                    dot = mine && i < sp.nq ? a.delta[row0 + i] : 0.f;
+                }
 #pragma unroll
                 for (int u = 0; u < QT / 32 / KW; ++u) {
                     const int t = u * KW + share;
@@ -749,17 +765,36 @@ __global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::BWD_WAVES : 1)) void a
                         mma<NP>(dp, f, vf[c]);
                     }
 #pragma unroll
+                    for (int r0 = 0; r0 < 16; r0 += 4) {  // four rows' sums and dots at once
+                        const int row = now + 32 * t + 2 * r0 + 4 * half;
+                        const f32x4 ref = *reinterpret_cast<const f32x4_m *>(lt + row), dot4 = *reinterpret_cast<const f32x4_m *>(et + row);
+                        f32x4 inv{1.f, 1.f, 1.f, 1.f};
+                        if constexpr (NP > 1) inv = *reinterpret_cast<const f32x4_m *>(it + row);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int r = r0 + e;
+                            float x;
+                            if constexpr (BIAS) {
+                                const float w = near ? tab[j - p0 + a.bk.far + PAD - (2 * r0 + 4 * half + e)] : b;
+                                x = __builtin_fmaf(s[r], scale2, w) + ref[e];
+                            } else {
+                                x = __builtin_fmaf(s[r], scale2, ref[e]);
+                            }
+                            s[r] = prob<T>(x, inv[e]);
+                            dp[r] = s[r] * (dp[r] - dot4[e]);
+                        }
+                    }
+                    if (edge) {  // rows from the key's own position on
+                        const int n = j - p0;
+                        const uint32_t bits = (n <= 0 ? ~0u : n >= 32 ? 0u : ~0u << n) >> (4 * half);
+                        keep_only(s, bits, 0.f);
+                        keep_only(dp, bits, 0.f);
+                    }
+#pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         float p[8], ds[8];
 #pragma unroll
-                        for (int r = 0; r < 8; ++r) {
-                            const int ir = 8 * (2 * c + (r >> 2)) + 4 * half + (r & 3);
-                            const int o = j - (p0 + ir);
-                            const float x = __builtin_fmaf(s[8 * c + r], scale2, near ? tab[o + a.bk.far + PAD] : b);
-                            const bool keep = !edge || o <= 0;
-                            p[r] = keep ? prob<T>(x, lt[32 * t + ir], it[32 * t + ir]) : 0.f;
-                            ds[r] = keep ? p[r] * (dp[8 * c + r] - et[32 * t + ir]) : 0.f;
-                        }
+                        for (int r = 0; r < 8; ++r) p[r] = s[8 * c + r], ds[r] = dp[8 * c + r];
                         bf16x8 pf[NP], sf[NP];
                         to_pieces<NP>(p, pf);
                         to_pieces<NP>(ds, sf);
@@ -772,6 +807,12 @@ __global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::BWD_WAVES : 1)) void a
                             mma<NP>(dk[d], f, sf);
                         }
                     }
+                }
+                if (mine) {
+                    const int next = now ^ (3 * QT);
+                    lt[next + threadIdx.x] = -rs.ref;
+                    it[next + threadIdx.x] = rs.inv;
+                    et[next + threadIdx.x] = dot;
                 }
             }
         }
@@ -908,7 +949,7 @@ struct Diagonals {
 // dq of 128 / KW rows (KW waves share 32, each taking every KW-th 32 keys), and the bias gradient's
 // sums over their diagonals
 template <class T, int DP, int KT, int KW, bool BIAS>
-__global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::BWD_WAVES : 1)) void attn_bwd_q(Args a) {
+__global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::Q_WAVES : 1)) void attn_bwd_q(Args a) {
     constexpr int NP = Elem<T>::NP, PLANE = KT * DP, ROWS = 128 / KW;
     static_assert(KT % (32 * KW) == 0, "tile");
     extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
@@ -974,18 +1015,13 @@ __global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::BWD_WAVES : 1)) void a
                 row_frag<DP>(vt, PLANE, 32 * t, c, at, f);
                 mma<NP>(dp, f, df[c]);
             }
-            if constexpr (BIAS) {
-                add_bias(s, scale2, tab, a.bk.far, j - qw, j - (i + sp.start), half);
-            } else {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] *= scale2;
-            }
-            if (edge) hide(a, s, j - (i + sp.start), seen_keys(j, sp.nk, mask), half);
+            if constexpr (BIAS) add_bias(s, scale2, tab, a.bk.far, j - qw, j - (i + sp.start), half);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const float p = prob<T>(s[r], rs.ref, rs.inv);
-                s[r] = s[r] == -INFINITY ? 0.f : p * (NP > 1 ? __builtin_fmaf(dp[r], sign, -delta) : dp[r] - delta);
+                const float x = BIAS ? s[r] - rs.ref : __builtin_fmaf(s[r], scale2, -rs.ref);
+                s[r] = prob<T>(x, rs.inv) * (NP > 1 ? __builtin_fmaf(dp[r], sign, -delta) : dp[r] - delta);
             }
+            if (edge) keep_only(s, visible(a, j - (i + sp.start), seen_keys(j, sp.nk, mask), half), 0.f);
             if (BIAS && a.dbias) dg.tile(s, j - qw, bins, a.bk.far, lane);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -1164,7 +1200,7 @@ int fwd(const Args &a, void *stream) {
 template <class T, int DP, int KW, bool BIAS>
 int bwd_kv(const Args &a, void *stream) {
     constexpr int QT = KW > 1 ? 32 * KW : Shape<T, DP>::BWD_ROWS;
-    const size_t lds = area<T, DP, QT, KW, 2>() + (3 * QT + (BIAS ? 2 * (a.bk.far + PAD) + 1 : 0)) * 4;
+    const size_t lds = area<T, DP, QT, KW, 2>() + (6 * QT + (BIAS ? 2 * (a.bk.far + PAD) + 1 : 0)) * 4;
     return launch(attn_bwd_kv<T, DP, QT, KW, BIAS>, a.B * a.Hk * a.groups * ((a.Nk + 128 / KW - 1) / (128 / KW)), lds, stream, a);
 }
 template <class T, int DP, int KW, bool BIAS>

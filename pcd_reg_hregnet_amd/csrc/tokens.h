@@ -83,6 +83,20 @@ __device__ __forceinline__ void mma(f32x16 &acc, const bf16x8 (&a)[NP], const bf
         for (int i = 0; i <= s; ++i) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[s - i], acc, 0, 0, 0);
 }
 
+// The order in which a run of MFMA matrix products with READS LDS reads before each is issued: AHEAD
+// products' reads first, then one product and the next reads in turn, so that a product finds its
+// operands there.  (Left to itself the compiler waits for the reads right before each product.)
+template <int MFMA, int READS, int AHEAD>
+__device__ __forceinline__ void interleave() {
+    __builtin_amdgcn_sched_group_barrier(0x100, READS * AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < MFMA - AHEAD; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+}
+
 // ------------------------------------------------------------------- LDS tiles --
 // [rows][DP] bf16, 16-byte chunks permuted in each row so that both reads below touch every
 // bank once: 16 rows at one chunk (row fragments), and 4 rows x 4 chunks (column fragments).
