@@ -1078,7 +1078,7 @@ __global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::Q_WAVES : 1)) void att
         if (kend == 0) __syncthreads();  // the bins were cleared by other waves
         dg.end(bins, a.bk.far, lane);
         __syncthreads();
-        float *to = a.bins + (((size_t)w.b * a.H + w.h) * tiles + tile) * W;
+        float *to = a.bins + (((size_t)w.h * a.B + w.b) * tiles + tile) * W;
         for (int o = threadIdx.x; o < W; o += NT)
             to[o] = ((all_bins[o] + all_bins[W + o]) + all_bins[2 * W + o]) + all_bins[3 * W + o];
     }
@@ -1097,12 +1097,20 @@ __global__ __launch_bounds__(NT) void bias_reduce(Args a) {
         if (bucket_of(a.bk, o - far) == n) atomicMin(&from, o), atomicMax(&to, o + 1);
     __syncthreads();
     const int lo = from, w = to - lo, parts = a.B * tiles;  // (no offset: w <= 0)
-    int bits = 0;  // 2^bits threads go along the offsets, the others along the parts
-    while (bits < 8 && 1 << bits < w) ++bits;
+    const float *in = a.bins + (size_t)h * parts * W + lo;
     double s = 0.;
-    for (int p = threadIdx.x >> bits; p < parts; p += NT >> bits) {
-        const float *from_p = a.bins + (((size_t)(p / tiles) * a.H + h) * tiles + p % tiles) * W + lo;
-        for (int o = threadIdx.x & ((1 << bits) - 1); o < w; o += 1 << bits) s += from_p[o];
+    if (w == 1) {  // (most buckets)
+#pragma unroll 4
+        for (int p = threadIdx.x; p < parts; p += NT) s += in[(size_t)p * W];
+    } else if (w > 1) {
+        for (int p0 = 0; p0 < parts; p0 += 1 << 16) {  // (so that the flat index keeps 32 bits)
+            const uint32_t all = (uint32_t)min(parts - p0, 1 << 16) * w;
+#pragma unroll 4
+            for (uint32_t e = threadIdx.x; e < all; e += NT) {
+                const uint32_t p = e / (uint32_t)w;
+                s += in[(size_t)(p0 + p) * W + (e - p * w)];
+            }
+        }
     }
     sum[threadIdx.x] = s;
     __syncthreads();
