@@ -686,7 +686,7 @@ __global__ __launch_bounds__(NT) void attn_delta(Args a) {
 
 // dk, dv of 128 keys: every wave keeps 32 keys and walks all rows of all heads that share them, so
 // the sums over a group need no second pass and have one order.  Where that leaves too few
-// workgroups (a.groups) each walks one head, and sum_group adds the heads' f32 results.
+// workgroups each walks one of a.groups parts of the group, and sum_group adds the parts' f32 results.
 // KW waves share 32 keys, each taking every KW-th 32 rows (a small call has few keys to give a wave
 // of its own): their sums join in LDS, in wave order.
 template <class T, int DP, int QT, int KW, bool BIAS>
@@ -849,7 +849,7 @@ __global__ __launch_bounds__(NT, (KW > 1 ? 1 : BIAS ? Shape<T, DP>::KV_BIAS_WAVE
     if (j < a.Nk) {
         const float f = a.scale;
         if (a.groups > 1) {
-            const int64_t at = (((int64_t)w.b * a.Nk + j) * a.H + w.h * G + g0) * a.D;
+            const int64_t at = ((((int64_t)w.b * a.Nk + j) * a.Hk + w.h) * a.groups + w0.h % a.groups) * a.D;
             float *ok_ = a.part + at, *ov = a.sums + at;
 #pragma unroll
             for (int d = 0; d < DP / 32; ++d)
@@ -880,10 +880,10 @@ __global__ __launch_bounds__(NT, (KW > 1 ? 1 : BIAS ? Shape<T, DP>::KV_BIAS_WAVE
     }
 }
 
-// dk and dv of a group from its heads' parts, in head order
+// dk and dv of a group from its parts, in order
 template <class T>
 __global__ __launch_bounds__(NT) void sum_group(Args a) {
-    const int G = a.H / a.Hk, C = a.D / 4;
+    const int G = a.groups, C = a.D / 4;
     const int64_t e = (int64_t)blockIdx.x * NT + threadIdx.x, row = e / C;
     if (row >= (int64_t)a.B * a.Nk * a.Hk) return;
     const int col = e % C * 4;
@@ -1277,9 +1277,9 @@ size_t part_floats(const hreg_tok_attn_t *p, int splits) {  // results, then max
     return splits > 1 ? (size_t)p->B * p->H * p->Nq * splits : 0;
 }
 
-// How the backward pass is divided.  groups: heads of a group that the key gradients are split over
-// (2 x 4096 keys x 4 of 16 heads x 128 bf16: one long workgroup a CU otherwise, 1600 -> 938 us);
-// share_kv, tile_rows: whether waves share rows, and the query rows of a workgroup.  Sharing pays
+// How the backward pass is divided.  groups: parts of a group's heads that the key gradients are
+// split over, as few as give four workgroups a CU (2 x 4096 keys x 4 of 16 heads x 128 bf16: one long
+// workgroup a CU otherwise, 1600 -> 938 us); share_kv, tile_rows: whether waves share rows, and the query rows of a workgroup.  Sharing pays
 // while fewer than 160 workgroups are there without it (96: 146 -> 99 us; 160: 141 -> 176).
 struct BwdPlan { int groups, share_kv, tile_rows; };
 template <class T>
@@ -1290,13 +1290,16 @@ BwdPlan bwd_plan(const hreg_tok_attn_t *p) {
     const int G = p->H / p->Hk, share = p->dtype == HREG_TOK_F32 ? share_of<float>(p->D) : share_of<__bf16>(p->D);
     const int64_t keys = (int64_t)p->B * p->Hk * row_tiles(p->Nk), rows = (int64_t)p->B * p->H * row_tiles(p->Nq);
     BwdPlan q;
-    q.groups = p->dk && G > 1 && keys < 4 * CUS ? G : 1;
+    q.groups = 1;
+    if (p->dk)
+        while (q.groups < G && (G % q.groups || keys * q.groups < 4 * CUS)) ++q.groups;
     q.share_kv = share > 1 && keys * q.groups < 160;
     q.tile_rows = rows < 160 ? ROWS / share : ROWS;
     return q;
 }
 size_t group_floats(const hreg_tok_attn_t *p) {
-    return bwd_plan(p).groups > 1 ? (size_t)p->B * p->Nk * p->H * p->D : 0;
+    const int groups = bwd_plan(p).groups;
+    return groups > 1 ? (size_t)p->B * p->Nk * p->Hk * groups * p->D : 0;
 }
 size_t bins_bytes(const hreg_tok_attn_t *p) {
     if (!p->bias) return 0;

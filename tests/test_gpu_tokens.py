@@ -39,6 +39,11 @@ ATTN = [  # B, Nq, Nk, heads, key heads, width, causal, key lengths, query lengt
     (1, 400, 400, 1, 1, 32, True, None, None, True, (32, 100, True)),
     (1, 2, 700, 2, 1, 48, False, None, None, False, (128, 1024, True)),
     (2, 5, 1030, 8, 2, 128, True, [1030, 3], None, False, (32, 128, False)),
+    (8, 40, 1000, 32, 8, 16, True, None, None, False, None),  # a group's heads in two parts
+    (1, 600, 600, 6, 1, 8, False, None, [577], True, (8, 30, True)),  # in six, with a bias
+    (1, 60, 5000, 8, 1, 32, True, [4801], None, True, (32, 128, False)),  # many rows a key head, few tiles
+    (2, 1, 333, 40, 1, 64, True, [333, 1], None, False, (16, 40, False)),  # more heads than a tile has rows
+    (1, 2, 100, 64, 2, 32, True, None, None, False, (32, 1024, True)),  # tables too large for a group
 ]
 
 
@@ -625,6 +630,36 @@ def test_chain_in_two_graphs():
             g.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(outs, want)), k
+
+
+@pytest.mark.parametrize("dtype", [F, H], ids=["fp32", "bf16"])
+def test_attention_in_a_graph(dtype):
+    """wide heads, a group, a bias, lengths that change between the replays, and a token against a cache"""
+    s, kw, bias, spec = attn_case(13, (2, 200, 260, 8, 2, 128, True, [260, 100], None, False, (32, 128, False)), dtype)
+    leaves = [leaf(t) for t in (s["q"], s["k"], s["v"], bias)]
+    lengths = kw["k_lengths"]
+
+    def once(q, k, v, b):
+        out = tokens.attention(q, k, v, causal=True, k_lengths=lengths, bias=b, buckets=tokens.Buckets(*spec))
+        with torch.no_grad():
+            one = tokens.attention(q[:, :1], k, v, causal=True, k_lengths=lengths, bias=b, buckets=tokens.Buckets(*spec))
+        return [out.detach(), one, *torch.autograd.grad(out, [q, k, v, b], s["do"])]
+
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        once(*leaves)
+    torch.cuda.current_stream().wait_stream(st)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = once(*leaves)
+    for k in range(3):
+        lengths.copy_(torch.tensor([260 - 60 * k, 100 + 80 * k]))
+        want = once(*(leaf(t) for t in leaves))
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want)), k
 
 
 def test_inputs_untouched():
