@@ -367,7 +367,7 @@ __global__ __launch_bounds__(NT, (Shape<T, DP>::FWD_WAVES)) void attn_fwd(Args a
             for (int t = 0; t < MT; ++t) {
                 bf16x8 kf[NP];
                 row_frag<DP>(kt, PLANE, 32 * t, c, at, kf);
-                mma<NP>(s[t], kf, qf[c]);
+                mma(s[t], kf, qf[c]);
             }
         if constexpr (NP == 1) interleave<MT * DP / 16, 1, 2>();
         const int kpos = j0 - (i + sp.start);
@@ -410,7 +410,7 @@ __global__ __launch_bounds__(NT, (Shape<T, DP>::FWD_WAVES)) void attn_fwd(Args a
                 for (int d = 0; d < DP / 32; ++d) {
                     bf16x8 vf[NP];
                     col_frag<DP>(vt, PLANE, 32 * t + 16 * c, 32 * d, at, vf);
-                    mma<NP>(acc[d], vf, pf);
+                    mma(acc[d], vf, pf);
                 }
             }
         if constexpr (NP == 1) interleave<MT * DP / 16, 2, 4>();
@@ -519,7 +519,7 @@ __global__ __launch_bounds__(NT, (Shape<T, DP>::SPLIT_WAVES)) void attn_split(Ar
         for (int c = 0; c < DP / 16; ++c) {
             bf16x8 kf[NP];
             row_frag<DP>(buf, PLANE, 0, c, at, kf);
-            mma<NP>(s, kf, qf[c]);
+            mma(s, kf, qf[c]);
         }
         const int kpos = j0 - (i + sp.start);
         const bool edge = mask || j0 + 32 > sp.nk || (a.causal && j0 + 31 > first_pos);
@@ -572,7 +572,7 @@ __global__ __launch_bounds__(NT, (Shape<T, DP>::SPLIT_WAVES)) void attn_split(Ar
             for (int d = 0; d < DP / 32; ++d) {
                 bf16x8 vf[NP];
                 col_frag<DP>(buf, PLANE, 16 * c, 32 * d, at, vf);
-                mma<NP>(acc[d], vf, pf);
+                mma(acc[d], vf, pf);
             }
         }
         wave_sync();  // the values are read
@@ -684,6 +684,13 @@ __global__ __launch_bounds__(NT) void attn_delta(Args a) {
     if (in && threadIdx.x % 64 < 32) a.delta[row] = s;
 }
 
+// The pieces that p and ds go into their products in.  A bf16 call that is too small to fill the card
+// keeps 16 bits of them instead of 8: its products are not what it waits for, and few values
+// average less of the rounding away (gradients 1.05 instead of 1.45 times as far from the exact ones
+// as their own rounding).
+template <class T, int KW>
+constexpr int prob_pieces() { return Elem<T>::NP == 1 && KW > 1 ? 2 : Elem<T>::NP; }
+
 // dk, dv of 128 keys: every wave keeps 32 keys and walks all rows of all heads that share them, so
 // the sums over a group need no second pass and have one order.  Where that leaves too few
 // workgroups each walks one of a.groups parts of the group, and sum_group adds the parts' f32 results.
@@ -691,7 +698,7 @@ __global__ __launch_bounds__(NT) void attn_delta(Args a) {
 // of its own): their sums join in LDS, in wave order.
 template <class T, int DP, int QT, int KW, bool BIAS>
 __global__ __launch_bounds__(NT, (KW > 1 ? 1 : BIAS ? Shape<T, DP>::KV_BIAS_WAVES : Shape<T, DP>::KV_WAVES)) void attn_bwd_kv(Args a) {
-    constexpr int NP = Elem<T>::NP, PLANE = QT * DP, ROWS = 128 / KW;
+    constexpr int NP = Elem<T>::NP, PP = prob_pieces<T, KW>(), PLANE = QT * DP, ROWS = 128 / KW;
     static_assert(QT % (32 * KW) == 0, "tile");
     extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
     typedef Tiles<T, DP, QT> QD;
@@ -760,9 +767,9 @@ __global__ __launch_bounds__(NT, (KW > 1 ? 1 : BIAS ? Shape<T, DP>::KV_BIAS_WAVE
                     for (int c = 0; c < DP / 16; ++c) {
                         bf16x8 f[NP];
                         row_frag<DP>(qt, PLANE, 32 * t, c, at, f);
-                        mma<NP>(s, f, kf[c]);
+                        mma(s, f, kf[c]);
                         row_frag<DP>(dt, PLANE, 32 * t, c, at, f);
-                        mma<NP>(dp, f, vf[c]);
+                        mma(dp, f, vf[c]);
                     }
 #pragma unroll
                     for (int r0 = 0; r0 < 16; r0 += 4) {  // four rows' sums and dots at once
@@ -795,16 +802,16 @@ __global__ __launch_bounds__(NT, (KW > 1 ? 1 : BIAS ? Shape<T, DP>::KV_BIAS_WAVE
                         float p[8], ds[8];
 #pragma unroll
                         for (int r = 0; r < 8; ++r) p[r] = s[8 * c + r], ds[r] = dp[8 * c + r];
-                        bf16x8 pf[NP], sf[NP];
-                        to_pieces<NP>(p, pf);
-                        to_pieces<NP>(ds, sf);
+                        bf16x8 pf[PP], sf[PP];
+                        to_pieces<PP>(p, pf);
+                        to_pieces<PP>(ds, sf);
 #pragma unroll
                         for (int d = 0; d < DP / 32; ++d) {
                             bf16x8 f[NP];
                             col_frag<DP>(dt, PLANE, 32 * t + 16 * c, 32 * d, at, f);
-                            mma<NP>(dv[d], f, pf);
+                            mma(dv[d], f, pf);
                             col_frag<DP>(qt, PLANE, 32 * t + 16 * c, 32 * d, at, f);
-                            mma<NP>(dk[d], f, sf);
+                            mma(dk[d], f, sf);
                         }
                     }
                 }
@@ -950,7 +957,7 @@ struct Diagonals {
 // sums over their diagonals
 template <class T, int DP, int KT, int KW, bool BIAS>
 __global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::Q_WAVES : 1)) void attn_bwd_q(Args a) {
-    constexpr int NP = Elem<T>::NP, PLANE = KT * DP, ROWS = 128 / KW;
+    constexpr int NP = Elem<T>::NP, PP = prob_pieces<T, KW>(), PLANE = KT * DP, ROWS = 128 / KW;
     static_assert(KT % (32 * KW) == 0, "tile");
     extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
     typedef Tiles<T, DP, KT> KV;
@@ -1011,9 +1018,9 @@ __global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::Q_WAVES : 1)) void att
             for (int c = 0; c < DP / 16; ++c) {
                 bf16x8 f[NP];
                 row_frag<DP>(kt, PLANE, 32 * t, c, at, f);
-                mma<NP>(s, f, qf[c]);
+                mma(s, f, qf[c]);
                 row_frag<DP>(vt, PLANE, 32 * t, c, at, f);
-                mma<NP>(dp, f, df[c]);
+                mma(dp, f, df[c]);
             }
             if constexpr (BIAS) add_bias(s, scale2, tab, a.bk.far, j - qw, j - (i + sp.start), half);
 #pragma unroll
@@ -1028,13 +1035,13 @@ __global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::Q_WAVES : 1)) void att
                 float x[8];
 #pragma unroll
                 for (int r = 0; r < 8; ++r) x[r] = s[8 * c + r];
-                bf16x8 sf[NP];
-                to_pieces<NP>(x, sf);
+                bf16x8 sf[PP];
+                to_pieces<PP>(x, sf);
 #pragma unroll
                 for (int d = 0; d < DP / 32; ++d) {
                     bf16x8 f[NP];
                     col_frag<DP>(kt, PLANE, 32 * t + 16 * c, 32 * d, at, f);
-                    mma<NP>(acc[d], f, sf);
+                    mma(acc[d], f, sf);
                 }
             }
         }

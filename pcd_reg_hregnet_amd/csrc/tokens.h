@@ -47,13 +47,20 @@ __device__ __forceinline__ f32x16 zero16() {
 }
 
 // eight values as the NP operand pieces of one lane of a 16-deep product chunk.  NP = 1 rounds
-// to bf16; NP = 3 cuts 8 + 8 + 8 significant bits (exact for normal f32).
+// to bf16; NP = 2 rounds, and rounds the rest; NP = 3 cuts 8 + 8 + 8 significant bits (exact for
+// normal f32).
 template <int NP>
 __device__ __forceinline__ void to_pieces(const float (&x)[8], bf16x8 (&p)[NP]) {
     u32x4 w[NP];
     if constexpr (NP == 1) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[0][i] = pack_bf16(x[2 * i], x[2 * i + 1]);
+    } else if constexpr (NP == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[0][i] = pack_bf16(x[2 * i], x[2 * i + 1]);
+            w[1][i] = pack_bf16(x[2 * i] - bf16_lo(w[0][i]), x[2 * i + 1] - bf16_hi(w[0][i]));
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -73,10 +80,16 @@ __device__ __forceinline__ void to_pieces(const float (&x)[8], bf16x8 (&p)[NP]) 
     for (int s = 0; s < NP; ++s) p[s] = __builtin_bit_cast(bf16x8, w[s]);
 }
 
-// acc += A B on v_mfma_f32_32x32x16_bf16.  Lane l: column / row l & 31, depth 8 (l >> 5) + i;
+// acc += A B on v_mfma_f32_32x32x16_bf16 (A bf16 itself, B in NB pieces, or both f32).  Lane l: column / row l & 31, depth 8 (l >> 5) + i;
 // result register r: row 8 (r >> 2) + 4 (l >> 5) + (r & 3), column l & 31.  Smallest first.
-template <int NP>
-__device__ __forceinline__ void mma(f32x16 &acc, const bf16x8 (&a)[NP], const bf16x8 (&b)[NP]) {
+template <int NP, int NB>
+__device__ __forceinline__ void mma(f32x16 &acc, const bf16x8 (&a)[NP], const bf16x8 (&b)[NB]) {
+    static_assert(NP == NB || NP == 1, "pieces");
+    if constexpr (NP == 1) {
+#pragma unroll
+        for (int s = NB - 1; s >= 0; --s) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[s], acc, 0, 0, 0);
+        return;
+    }
 #pragma unroll
     for (int s = NP - 1; s >= 0; --s)
 #pragma unroll
