@@ -726,7 +726,7 @@ __global__ __launch_bounds__(NT, (KW > 1 ? 1 : BIAS ? Shape<T, DP>::KV_BIAS_WAVE
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) dk[d] = dv[d] = zero16();
     const float scale2 = a.scale * LOG2E;
-    const int first = a.causal ? max(w.tile * ROWS - sp.start, 0) / QT * QT : 0;  // rows before see no key of the tile
+    const int first = a.causal ? max(w.tile * ROWS - sp.start, 0) : 0;  // rows before see no key of the tile
     const int G = a.H / a.Hk;
     QD qd;
     qd.init(lds, a.D);
@@ -1140,6 +1140,7 @@ __global__ __launch_bounds__(NT) void bias_reduce(Args a) {
 
 // ------------------------------------------------------------------- C interface --
 
+constexpr int64_t MAX_GRID = ((int64_t)1 << 32) / NT - 1;
 int row_tiles(int n) { return (n + ROWS - 1) / ROWS; }
 
 // rows of (batch, tokens, heads) in 16-byte steps; a dimension of one is never stepped over
@@ -1154,8 +1155,9 @@ int take(const hreg_tok_attn_t *p, Args &a) {
     if (!p || (p->dtype != HREG_TOK_F32 && p->dtype != HREG_TOK_BF16)) return HREG_ERR_INVALID;
     if (p->B < 0 || p->Nq < 0 || p->Nk < 0 || p->H < 1 || p->Hk < 1 || p->H % p->Hk) return HREG_ERR_INVALID;
     if (p->D < 8 || p->D > 128 || p->D % 8) return HREG_ERR_UNSUPPORTED;
-    if ((int64_t)p->B * p->H * (row_tiles(p->Nq) + 1) > INT32_MAX || (int64_t)p->B * p->H * (row_tiles(p->Nk) + 1) > INT32_MAX ||
-        (int64_t)p->Nq * (p->H / p->Hk) > (1 << 30) ||
+    // (a launch has fewer than 2^32 threads)
+    if ((int64_t)p->B * p->H * row_tiles(p->Nq) > MAX_GRID || (int64_t)p->B * p->H * row_tiles(p->Nk) > MAX_GRID ||
+        (int64_t)p->B * p->H > MAX_GRID || (int64_t)p->Nq * (p->H / p->Hk) > (1 << 30) ||
         p->Nq > (1 << 30) || p->Nk > (1 << 30))
         return HREG_ERR_UNSUPPORTED;
     const int es = p->dtype == HREG_TOK_F32 ? 4 : 2;

@@ -13,6 +13,13 @@ using namespace hreg_tok;
 
 constexpr int NT = 256;
 
+// A launch has fewer than 2^32 threads a dimension: many workgroups go into two
+__device__ __forceinline__ int64_t block_number() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+dim3 grid_of(int64_t blocks) {
+    const int64_t x = blocks < (1 << 21) ? blocks : 1 << 21;
+    return dim3((uint32_t)x, (uint32_t)((blocks + x - 1) / x));
+}
+
 struct Rng {
     uint64_t seed;
     const uint64_t *dev;
@@ -118,7 +125,7 @@ __device__ __forceinline__ void store8(T *p, int n, const float (&v)[8]) {
 
 template <class T, bool VEC>
 __global__ __launch_bounds__(NT) void dropout_kernel(const T *__restrict__ x, T *__restrict__ y, int64_t n, Rng g) {
-    const int64_t at = ((int64_t)blockIdx.x * NT + threadIdx.x) * 8;
+    const int64_t at = (block_number() * NT + threadIdx.x) * 8;
     if (at >= n) return;
     float v[8], m[8];
     const int have = (int)min((int64_t)8, n - at);
@@ -219,9 +226,9 @@ template <class T, int TPR, int MODE>
 __global__ __launch_bounds__(threads<TPR>()) void block_fwd(Block a) {
     __shared__ float lds[16];
     constexpr bool VEC = MODE >= ALIGNED, USUAL = MODE == WHOLE;
-    const int r = blockIdx.x * (threads<TPR>() / TPR) + threadIdx.x / TPR, C = a.C, c = threadIdx.x % TPR * 8;
+    const int r = (int)block_number() * (threads<TPR>() / TPR) + threadIdx.x / TPR, C = a.C, c = threadIdx.x % TPR * 8;
     const int n = USUAL ? 8 : C - c;
-    if (TPR <= 64 && r >= a.R) return;
+    if (r >= a.R) return;  // (a workgroup of one row leaves as a whole)
     const int64_t at = (int64_t)r * C + c;
     const float inv_c = 1.f / (float)C;
     float y[8], mu = 0.f, rs = 1.f, mu2 = 0.f, rs2 = 1.f;
@@ -498,7 +505,7 @@ int go(const Block &a, const Plan &q, void *stream) {
         if (full) hipLaunchKernelGGL((block_bwd<T, TPR, MODE, true>), dim3(q.splits, q.flight), block, 0, as_stream(stream), a);
     } else {
         constexpr int SLOTS = threads<TPR>() / TPR;
-        hipLaunchKernelGGL((block_fwd<T, TPR, MODE>), dim3((a.R + SLOTS - 1) / SLOTS), block, 0, as_stream(stream), a);
+        hipLaunchKernelGGL((block_fwd<T, TPR, MODE>), grid_of((a.R + SLOTS - 1) / SLOTS), block, 0, as_stream(stream), a);
     }
     HREG_CHECK_LAUNCH();
     return HREG_OK;
@@ -545,20 +552,20 @@ int hreg_tok_dropout(const void *x, void *y, int64_t n, int dtype, uint32_t step
     if (n == 0) return HREG_OK;
     if (!x || !y) return HREG_ERR_INVALID;
     const int64_t grid = (n + 8 * NT - 1) / (8 * NT);
-    if (grid > INT32_MAX) return HREG_ERR_UNSUPPORTED;
+    if (grid > (int64_t)65535 << 21) return HREG_ERR_UNSUPPORTED;
     const Rng g = make_rng(step, seed, seed_dev, site);
     const bool vec = aligned16(x) && aligned16(y);
     const hipStream_t st = as_stream(stream);
     if (dtype == HREG_TOK_F32) {
         const float *s = static_cast<const float *>(x);
         float *d = static_cast<float *>(y);
-        if (vec) hipLaunchKernelGGL((dropout_kernel<float, true>), dim3(grid), dim3(NT), 0, st, s, d, n, g);
-        else hipLaunchKernelGGL((dropout_kernel<float, false>), dim3(grid), dim3(NT), 0, st, s, d, n, g);
+        if (vec) hipLaunchKernelGGL((dropout_kernel<float, true>), grid_of(grid), dim3(NT), 0, st, s, d, n, g);
+        else hipLaunchKernelGGL((dropout_kernel<float, false>), grid_of(grid), dim3(NT), 0, st, s, d, n, g);
     } else {
         const __bf16 *s = static_cast<const __bf16 *>(x);
         __bf16 *d = static_cast<__bf16 *>(y);
-        if (vec) hipLaunchKernelGGL((dropout_kernel<__bf16, true>), dim3(grid), dim3(NT), 0, st, s, d, n, g);
-        else hipLaunchKernelGGL((dropout_kernel<__bf16, false>), dim3(grid), dim3(NT), 0, st, s, d, n, g);
+        if (vec) hipLaunchKernelGGL((dropout_kernel<__bf16, true>), grid_of(grid), dim3(NT), 0, st, s, d, n, g);
+        else hipLaunchKernelGGL((dropout_kernel<__bf16, false>), grid_of(grid), dim3(NT), 0, st, s, d, n, g);
     }
     HREG_CHECK_LAUNCH();
     return HREG_OK;

@@ -238,14 +238,16 @@ def attention(q, k, v, *, scale=None, causal=False, align_end=None, q_lengths=No
 
     q [B, Nq, H, D]; k, v [B, Nk, Hk, D] with H a multiple of Hk (each key head serves H // Hk
     consecutive query heads); float32 or bfloat16, D a multiple of 8 up to 128.  Any strides:
-    rows that are not contiguous 16-byte aligned steps are copied first.  scale: D ** -0.5 by
-    default.  Differentiable (once) in q, k, v and bias.
+    rows that are not contiguous 16-byte aligned steps are copied first.  Batch x heads x tokens / 128
+    (rounded up) stays below 2^24.  scale: D ** -0.5 by default.  Differentiable (once) in q, k, v
+    and bias.
 
     k_lengths, q_lengths [B] int32 / int64 on the GPU (clamped to the tensors): keys and queries
     from there on do not exist.  key_mask [B or 1, Nk] bool: False keys are not seen.  Their
     values, NaN among them, have no influence.  Queries that do not exist or see no key give 0
     and take no gradient.  A key that is not finite and that any query sees may reach every query
-    of its batch entry.
+    of its batch entry, and a query or an output gradient that is not finite every key's gradient
+    unless its position is behind the lengths or, where causal, before the first key.
 
     Positions: key j stands at j; query i at i, or with align_end (the default where causal) at
     i + keys - queries, so that the last query stands at the last key.  causal: a query sees keys

@@ -172,6 +172,20 @@ def test_attention_hidden_values(dtype, train):
         assert torch.equal(a, b) and not torch.isnan(a).any()
 
 
+@pytest.mark.parametrize("dtype", [F, H], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("B", [2, 90])  # waves that share rows, and not
+def test_attention_queries_before_the_keys(dtype, B):
+    """the last of more queries than keys: what stands in those before the first key reaches nothing"""
+    s, kw, _, _ = attn_case(31, (B, 203, 33, 4, 2, 16, True, None, None, False, None), dtype)
+    early = 203 - 33
+    s["q"][:, :early] = s["do"][:, :early] = 0
+    want = oracle.attention(s["q"], s["k"], s["v"], do=s["do"], **kw)
+    s["q"][:, :early], s["do"][:, :early] = float("nan"), float("inf")
+    got = run_attn(s, kw, None, None)
+    for n in want:
+        assert_within(got[n], want[n], n)
+
+
 def test_attention_lowest_and_large_scores():
     """scores far apart and a bias of the type's lowest value: no overflow, no NaN"""
     for dtype in (F, H):
@@ -461,6 +475,17 @@ def test_block_one_gradient_missing():
         zero = {n: None if n == missing else g for n, g in d.items()}
         got = {"y": y, "h": h, **{"d" + n: torch.zeros_like(v) if g is None else g for (n, v), g in zip(wrt.items(), got)}}
         check_block(got, t, zero, cfg)
+
+
+def test_block_more_threads_than_a_launch_holds():
+    """2^28 and a few rows of eight channels: sixteen threads a row pass 2^32"""
+    R = (1 << 28) + 3
+    x = torch.ones(R, 8, device="cuda", dtype=H)
+    x[-3:] = torch.tensor([2.0, 0.0, -3.0], device="cuda", dtype=H)[:, None]
+    with torch.no_grad():
+        _, h = tokens.gated_residual_norm(x, None)  # 1 / sqrt(1 + 1e-6) rounds to 1
+    assert h[-3:, 0].tolist() == [1.0, 0.0, -1.0]
+    assert bool((h[:-3] == 1).all())
 
 
 def test_block_same_bits_and_views():

@@ -141,7 +141,7 @@ def _attn(**over):
 @pytest.mark.parametrize("over,code", [
     (dict(dtype=2), 1), (dict(B=-1), 1), (dict(Nq=-1), 1), (dict(Nk=-1), 1), (dict(H=3, Hk=2), 1), (dict(Hk=0), 1),
     (dict(D=12), 3), (dict(D=136), 3), (dict(D=0), 3), (dict(q=None), 1), (dict(q=4098), 1), (dict(out=4100), 1),
-    (dict(ks_n=36), 1), (dict(Nq=(1 << 30) + 1), 3), (dict(B=1 << 20, Nq=1 << 20), 3),
+    (dict(ks_n=36), 1), (dict(Nq=(1 << 30) + 1), 3), (dict(B=1 << 20, Nq=1 << 20), 3), (dict(B=1 << 23, Nq=1, Nk=1), 3), (dict(B=1 << 16, Nq=1, Nk=1 << 15), 3),
     (dict(bias=4096, bias_dtype=5), 1), (dict(bias=4096, num_buckets=1, max_distance=8), 1),
     (dict(bias=4096, num_buckets=7, both=1, max_distance=8), 1), (dict(bias=4096, num_buckets=32, max_distance=16), 1),
     (dict(bias=4096, num_buckets=32, max_distance=2000, nthresh=15), 3),
