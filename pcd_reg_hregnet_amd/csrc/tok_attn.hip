@@ -27,6 +27,13 @@ constexpr int ROWS = 128;        // rows a workgroup owns: 32 a wave
 constexpr int CUS = 256;
 constexpr int MAX_BINS = 2049;   // offsets -max_distance .. max_distance with max_distance <= 1024
 
+// DW: a call's width rounded up to 32, 48, 64, 96 or 128 columns, which scores are summed over and
+// results are kept for (in blocks of 32); a tile's rows in LDS step by a power of two.  (2 x 4096 x 16
+// heads x 96 bf16, forward and backward: 1101 us with 96, 1230 with 128; 2 x 2048 x 8 x 40 f32: 408
+// with 48, 444 with 64.)
+constexpr int pitch(int dw) { return dw <= 32 ? 32 : dw <= 64 ? 64 : 128; }
+constexpr int blocks(int dw) { return (dw + 31) / 32; }
+
 // Rows of a tile that goes through LDS, and the waves a SIMD that the registers are cut to.  Two
 // waves a SIMD hide each other's waits (2 x 4096 x 16 heads x 128 bf16, us: forward 387 with two, 572
 // with one; key gradients and the rest of the backward pass 964 and 1120) as long as little spills:
@@ -35,18 +42,18 @@ constexpr int MAX_BINS = 2049;   // offsets -max_distance .. max_distance with m
 // halve the barriers of 32, but at 128 columns the key gradients have no registers for them (746 us
 // with 32, 1939 with 64).  There the fragments' addresses are made again at every tile too (TIGHT:
 // 34 spilled registers become 4, 722 -> 660 us; elsewhere it only costs instructions).
-template <class T, int DP>
+template <class T, int DW>
 struct Shape {
     static constexpr bool F32 = Elem<T>::NP > 1;
-    static constexpr int FWD_KEYS = F32 && DP > 32 ? 32 : 64, BWD_ROWS = F32 && DP > 32 ? 32 : DP > 64 ? 32 : 64;
-    static constexpr int Q_KEYS = F32 && DP > 32 ? 32 : 64;
-    static constexpr int FWD_WAVES = F32 && DP > 64 ? 1 : 2, Q_WAVES = FWD_WAVES;
-    static constexpr int KV_WAVES = F32 && DP > 32 ? 1 : 2, KV_BIAS_WAVES = DP > (F32 ? 32 : 64) ? 1 : 2;
-    static constexpr bool TIGHT = !F32 && DP > 64;
-    static constexpr int SPLIT_WAVES = F32 && DP > 64 ? 1 : 2;
+    static constexpr int FWD_KEYS = F32 && DW > 32 ? 32 : 64, BWD_ROWS = F32 && DW > 32 ? 32 : DW > 64 ? 32 : 64;
+    static constexpr int Q_KEYS = F32 && DW > 32 ? 32 : 64;
+    static constexpr int FWD_WAVES = F32 && DW > 64 ? 1 : 2, Q_WAVES = FWD_WAVES;
+    static constexpr int KV_WAVES = F32 && DW > 32 ? 1 : 2, KV_BIAS_WAVES = DW > (F32 ? 32 : 64) ? 1 : 2;
+    static constexpr bool TIGHT = !F32 && DW > 64;
+    static constexpr int SPLIT_WAVES = F32 && DW > 64 ? 1 : 2;
     // waves that share 32 rows in a small call (8 x 512 keys x 4 heads x 32 f32: 126 -> 78 us with 4;
     // 2 x 700 x 8 x 64 f32: 146 -> 99 with 2, 137 with 4, whose tiles leave one workgroup a CU)
-    static constexpr int SHARE = F32 && DP > 64 ? 1 : DP > 32 ? 2 : 4;
+    static constexpr int SHARE = F32 && DW > 64 ? 1 : DW > 32 ? 2 : 4;
 };
 
 struct Buckets {
@@ -199,11 +206,11 @@ struct Tiles {
 };
 
 // one row's pieces as an operand with the row in lane & 31, straight from global memory
-template <class T, int DP>
+template <class T, int DW>
 __device__ __forceinline__ void load_row(const T *row, bool ok, int D, int lane,
-                                         bf16x8 (&f)[DP / 16][Elem<T>::NP], bool negate = false) {
+                                         bf16x8 (&f)[DW / 16][Elem<T>::NP], bool negate = false) {
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) {
+    for (int c = 0; c < DW / 16; ++c) {
         const int d = 16 * c + 8 * (lane >> 5);
         Chunk<T> x;
         if (ok && d < D) x.load(row + d);
@@ -321,9 +328,9 @@ __device__ __forceinline__ void finish_row(const Args &a, int b, int i, int h, i
 // and a quarter-rate exponential a score against 16 cycles of matrix product), at 128 columns by both
 // and by the waits between them; f32 by its six products.  2 x 4096 x 16 heads: 128 columns 302 us
 // (910 TFLOP/s), 64 columns 183 us (750); f32 2 x 2048 x 8 x 64: 116 us (148).
-template <class T, int DP, int KT, bool BIAS>
-__global__ __launch_bounds__(NT, (Shape<T, DP>::FWD_WAVES)) void attn_fwd(Args a) {
-    constexpr int NP = Elem<T>::NP, MT = KT / 32, PLANE = KT * DP;
+template <class T, int DW, int KT, bool BIAS>
+__global__ __launch_bounds__(NT, (Shape<T, DW>::FWD_WAVES)) void attn_fwd(Args a) {
+    constexpr int NP = Elem<T>::NP, DP = pitch(DW), ND = blocks(DW), MT = KT / 32, PLANE = KT * DP;
     extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
     typedef Tiles<T, DP, KT> KV;
     float *tab = reinterpret_cast<float *>(reinterpret_cast<char *>(lds) + KV::BYTES);
@@ -340,13 +347,13 @@ __global__ __launch_bounds__(NT, (Shape<T, DP>::FWD_WAVES)) void attn_fwd(Args a
 
     // without a bias scores stay as the products give them and their running maximum with them
     // (q takes a negative scale's sign): one fused multiply-add before each exponential
-    bf16x8 qf[DP / 16][NP];
-    load_row<T, DP>(static_cast<const T *>(a.q) + w.b * a.qs[0] + (int64_t)i * a.qs[1] + w.h * a.qs[2], i < sp.nq, a.D,
+    bf16x8 qf[DW / 16][NP];
+    load_row<T, DW>(static_cast<const T *>(a.q) + w.b * a.qs[0] + (int64_t)i * a.qs[1] + w.h * a.qs[2], i < sp.nq, a.D,
                     lane, qf, a.scale < 0.f);
     const float scale2 = fmaxf(fabsf(a.scale) * LOG2E, 1e-37f), unit = BIAS ? 1.f : scale2;
-    f32x16 acc[DP / 32];
+    f32x16 acc[ND];
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d) acc[d] = zero16();
+    for (int d = 0; d < ND; ++d) acc[d] = zero16();
     float m = -INFINITY, l = 0.f;
 
     // keys that some row of the workgroup sees
@@ -367,14 +374,14 @@ __global__ __launch_bounds__(NT, (Shape<T, DP>::FWD_WAVES)) void attn_fwd(Args a
 #pragma unroll
         for (int t = 0; t < MT; ++t) s[t] = zero16();
 #pragma unroll
-        for (int c = 0; c < DP / 16; ++c)
+        for (int c = 0; c < DW / 16; ++c)
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
                 bf16x8 kf[NP];
                 row_frag<DP>(kt, PLANE, 32 * t, c, at, kf);
                 mma(s[t], kf, qf[c]);
             }
-        if constexpr (NP == 1) interleave<MT * DP / 16, 1, 2>();
+        if constexpr (NP == 1) interleave<MT * DW / 16, 1, 2>();
         const int kpos = j0 - (i + sp.start);
         float top = m;
 #pragma unroll
@@ -390,7 +397,7 @@ __global__ __launch_bounds__(NT, (Shape<T, DP>::FWD_WAVES)) void attn_fwd(Args a
             const float shrink = __builtin_amdgcn_exp2f(__builtin_fmaf(m, unit, -ref));
             l *= shrink;
 #pragma unroll
-            for (int d = 0; d < DP / 32; ++d)
+            for (int d = 0; d < ND; ++d)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[d][r] *= shrink;
             m = top;
@@ -412,18 +419,18 @@ __global__ __launch_bounds__(NT, (Shape<T, DP>::FWD_WAVES)) void attn_fwd(Args a
                 bf16x8 pf[NP];
                 to_pieces<NP>(p, pf);
 #pragma unroll
-                for (int d = 0; d < DP / 32; ++d) {
+                for (int d = 0; d < ND; ++d) {
                     bf16x8 vf[NP];
                     col_frag<DP>(vt, PLANE, 32 * t + 16 * c, 32 * d, at, vf);
                     mma(acc[d], vf, pf);
                 }
             }
-        if constexpr (NP == 1) interleave<MT * DP / 16, 2, 4>();
+        if constexpr (NP == 1) interleave<MT * 2 * ND, 2, 4>();
     }
     l += __shfl_xor(l, 32);
     if (i >= a.Nq) return;
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
+    for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
             const int col = 32 * d + 2 * r + 4 * half;
@@ -466,9 +473,9 @@ struct WaveStage {
     }
 };
 
-template <class T, int DP, bool BIAS>
-__global__ __launch_bounds__(NT, (Shape<T, DP>::SPLIT_WAVES)) void attn_split(Args a) {
-    constexpr int NP = Elem<T>::NP, PLANE = 32 * DP, OLD = DP + 4;  // OLD: a joined row's step in LDS
+template <class T, int DW, bool BIAS>
+__global__ __launch_bounds__(NT, (Shape<T, DW>::SPLIT_WAVES)) void attn_split(Args a) {
+    constexpr int NP = Elem<T>::NP, DP = pitch(DW), ND = blocks(DW), PLANE = 32 * DP, OLD = DP + 4;  // OLD: a joined row's step in LDS
     extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
     __shared__ float ml[4][2][32];
     const int G = a.H / a.Hk, R = a.Nq * G, tiles = (R + 31) / 32;
@@ -496,12 +503,12 @@ __global__ __launch_bounds__(NT, (Shape<T, DP>::SPLIT_WAVES)) void attn_split(Ar
         right = bias_at(a, bucket_of(a.bk, a.bk.far), hb) * LOG2E;
         __syncthreads();
     }
-    bf16x8 qf[DP / 16][NP];
-    load_row<T, DP>(static_cast<const T *>(a.q) + w.b * a.qs[0] + (int64_t)i * a.qs[1] + h * a.qs[2], there, a.D, lane, qf);
+    bf16x8 qf[DW / 16][NP];
+    load_row<T, DW>(static_cast<const T *>(a.q) + w.b * a.qs[0] + (int64_t)i * a.qs[1] + h * a.qs[2], there, a.D, lane, qf);
     const float scale2 = a.scale * LOG2E;
-    f32x16 acc[DP / 32];
+    f32x16 acc[ND];
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d) acc[d] = zero16();
+    for (int d = 0; d < ND; ++d) acc[d] = zero16();
     float m = -INFINITY, l = 0.f;
 
     // keys that some row of the tile sees, in `splits` runs of whole 128
@@ -522,7 +529,7 @@ __global__ __launch_bounds__(NT, (Shape<T, DP>::SPLIT_WAVES)) void attn_split(Ar
         wave_sync();
         f32x16 s = zero16();
 #pragma unroll
-        for (int c = 0; c < DP / 16; ++c) {
+        for (int c = 0; c < DW / 16; ++c) {
             bf16x8 kf[NP];
             row_frag<DP>(buf, PLANE, 0, c, at, kf);
             mma(s, kf, qf[c]);
@@ -555,7 +562,7 @@ __global__ __launch_bounds__(NT, (Shape<T, DP>::SPLIT_WAVES)) void attn_split(Ar
             const float shrink = __builtin_amdgcn_exp2f(m - ref);
             l *= shrink;
 #pragma unroll
-            for (int d = 0; d < DP / 32; ++d)
+            for (int d = 0; d < ND; ++d)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[d][e] *= shrink;
             m = top;
@@ -575,7 +582,7 @@ __global__ __launch_bounds__(NT, (Shape<T, DP>::SPLIT_WAVES)) void attn_split(Ar
             bf16x8 pf[NP];
             to_pieces<NP>(p, pf);
 #pragma unroll
-            for (int d = 0; d < DP / 32; ++d) {
+            for (int d = 0; d < ND; ++d) {
                 bf16x8 vf[NP];
                 col_frag<DP>(buf, PLANE, 16 * c, 32 * d, at, vf);
                 mma(acc[d], vf, pf);
@@ -595,7 +602,7 @@ __global__ __launch_bounds__(NT, (Shape<T, DP>::SPLIT_WAVES)) void attn_split(Ar
         const float all = fmaxf(fmaxf(ml[0][0][q], ml[1][0][q]), fmaxf(ml[2][0][q], ml[3][0][q]));
         const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - all);
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
+        for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int e = 0; e < 16; e += 4)
                 *reinterpret_cast<f32x4_m *>(part + (wave * 32 + q) * OLD + 32 * d + 2 * e + 4 * half) =
@@ -658,14 +665,14 @@ __global__ __launch_bounds__(NT) void attn_join(Args a) {
 
 // D_i = do_i . o_i of the lane's row, half of it each in lanes l and l + 32.  o and what it lost in
 // rounding (bf16): that error would be common to a row's ds.
-template <class T, int DP>
+template <class T, int DW>
 __device__ __forceinline__ float row_dot(const Args &a, int b, int h, int i, bool ok, int lane) {
     const T *x = static_cast<const T *>(a.dout) + b * a.dos[0] + (int64_t)i * a.dos[1] + h * a.dos[2];
     const T *y = static_cast<const T *>(a.out_r) + b * a.os[0] + (int64_t)i * a.os[1] + h * a.os[2];
     const T *z = static_cast<const T *>(a.rest) + (((int64_t)b * a.Nq + i) * a.H + h) * a.D;
     float s = 0.f;
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) {
+    for (int c = 0; c < DW / 16; ++c) {
         const int d = 16 * c + 8 * (lane >> 5);
         if (!ok || d >= a.D) continue;
         Chunk<T> u, v;
@@ -681,12 +688,12 @@ __device__ __forceinline__ float row_dot(const Args &a, int b, int h, int i, boo
 }
 
 // the same for a call that wants no query gradients: delta[b][h][i], 32 rows a wave
-template <class T, int DP>
+template <class T, int DW>
 __global__ __launch_bounds__(NT) void attn_delta(Args a) {
     const int64_t rows = (int64_t)a.B * a.H * a.Nq, row = (int64_t)blockIdx.x * (NT / 2) + threadIdx.x / 64 * 32 + threadIdx.x % 32;
     const bool in = row < rows;
     const int i = in ? row % a.Nq : 0, h = in ? row / a.Nq % a.H : 0, b = in ? row / a.Nq / a.H : 0;
-    const float s = row_dot<T, DP>(a, b, h, i, in && i < span_of(a, b).nq, threadIdx.x & 63);
+    const float s = row_dot<T, DW>(a, b, h, i, in && i < span_of(a, b).nq, threadIdx.x & 63);
     if (in && threadIdx.x % 64 < 32) a.delta[row] = s;
 }
 
@@ -705,9 +712,9 @@ constexpr int prob_pieces() { return Elem<T>::NP == 1 && KW > 1 ? 2 : Elem<T>::N
 // and ds are operands of the second products as they stand.  Bound by the matrix products and the
 // waits for their operands: 256 registers leave no room to read far ahead.  2 x 4096 x 16 heads x 128
 // bf16: 580 us (950 TFLOP/s); 64 columns 320 us (860); f32 2 x 2048 x 8 x 64: 215 us (160).
-template <class T, int DP, int QT, int KW, bool BIAS>
-__global__ __launch_bounds__(NT, (KW > 1 ? 1 : BIAS ? Shape<T, DP>::KV_BIAS_WAVES : Shape<T, DP>::KV_WAVES)) void attn_bwd_kv(Args a) {
-    constexpr int NP = Elem<T>::NP, PP = prob_pieces<T, KW>(), PLANE = QT * DP, ROWS = 128 / KW;
+template <class T, int DW, int QT, int KW, bool BIAS>
+__global__ __launch_bounds__(NT, (KW > 1 ? 1 : BIAS ? Shape<T, DW>::KV_BIAS_WAVES : Shape<T, DW>::KV_WAVES)) void attn_bwd_kv(Args a) {
+    constexpr int NP = Elem<T>::NP, PP = prob_pieces<T, KW>(), DP = pitch(DW), ND = blocks(DW), PLANE = QT * DP, ROWS = 128 / KW;
     static_assert(QT % (32 * KW) == 0, "tile");
     extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
     typedef Tiles<T, DP, QT> QD;
@@ -719,12 +726,12 @@ __global__ __launch_bounds__(NT, (KW > 1 ? 1 : BIAS ? Shape<T, DP>::KV_BIAS_WAVE
     const int share = wave % KW, k0 = w.tile * ROWS + 32 * (wave / KW), j = k0 + (lane & 31);
     const uint8_t *mask = a.key_mask ? a.key_mask + w.b * a.mask_sb : nullptr;
     const bool ok = j < sp.nk && (!mask || mask[j]);
-    bf16x8 kf[DP / 16][NP], vf[DP / 16][NP];
-    load_row<T, DP>(static_cast<const T *>(a.k) + w.b * a.ks[0] + (int64_t)j * a.ks[1] + w.h * a.ks[2], ok, a.D, lane, kf);
-    load_row<T, DP>(static_cast<const T *>(a.v) + w.b * a.vs[0] + (int64_t)j * a.vs[1] + w.h * a.vs[2], ok, a.D, lane, vf);
-    f32x16 dk[DP / 32], dv[DP / 32];
+    bf16x8 kf[DW / 16][NP], vf[DW / 16][NP];
+    load_row<T, DW>(static_cast<const T *>(a.k) + w.b * a.ks[0] + (int64_t)j * a.ks[1] + w.h * a.ks[2], ok, a.D, lane, kf);
+    load_row<T, DW>(static_cast<const T *>(a.v) + w.b * a.vs[0] + (int64_t)j * a.vs[1] + w.h * a.vs[2], ok, a.D, lane, vf);
+    f32x16 dk[ND], dv[ND];
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d) dk[d] = dv[d] = zero16();
+    for (int d = 0; d < ND; ++d) dk[d] = dv[d] = zero16();
     const float scale2 = a.scale * LOG2E;
     const int first = a.causal ? max(w.tile * ROWS - sp.start, 0) : 0;  // rows before see no key of the tile
     const int G = a.H / a.Hk;
@@ -756,7 +763,7 @@ __global__ __launch_bounds__(NT, (KW > 1 ? 1 : BIAS ? Shape<T, DP>::KV_BIAS_WAVE
             for (int i0 = first, now = 0; i0 < sp.nq; i0 += QT, now ^= 3 * QT) {
                 qd.land(i0, sp.nq, nullptr);
                 const uint16_t *qt = qd.x(), *dt = qd.y();
-                if constexpr (Shape<T, DP>::TIGHT) at.opaque();
+                if constexpr (Shape<T, DW>::TIGHT) at.opaque();
                 if (i0 + QT < sp.nq) {
                     qd.issue(Q, a.qs[1], dO, a.dos[1], i0 + QT, sp.nq, a.D, nullptr);
                     const int i = i0 + QT + threadIdx.x;
@@ -773,7 +780,7 @@ __global__ __launch_bounds__(NT, (KW > 1 ? 1 : BIAS ? Shape<T, DP>::KV_BIAS_WAVE
                     const float b = BIAS ? tab[k0 < p0 ? 0 : 2 * (a.bk.far + PAD)] : 0.f;
                     f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-                    for (int c = 0; c < DP / 16; ++c) {
+                    for (int c = 0; c < DW / 16; ++c) {
                         bf16x8 f[NP];
                         row_frag<DP>(qt, PLANE, 32 * t, c, at, f);
                         mma(s, f, kf[c]);
@@ -815,7 +822,7 @@ __global__ __launch_bounds__(NT, (KW > 1 ? 1 : BIAS ? Shape<T, DP>::KV_BIAS_WAVE
                         to_pieces<PP>(p, pf);
                         to_pieces<PP>(ds, sf);
 #pragma unroll
-                        for (int d = 0; d < DP / 32; ++d) {
+                        for (int d = 0; d < ND; ++d) {
                             bf16x8 f[NP];
                             col_frag<DP>(dt, PLANE, 32 * t + 16 * c, 32 * d, at, f);
                             mma(dv[d], f, pf);
@@ -839,7 +846,7 @@ __global__ __launch_bounds__(NT, (KW > 1 ? 1 : BIAS ? Shape<T, DP>::KV_BIAS_WAVE
 #pragma unroll
         for (int v = 1; v < KW; ++v)
 #pragma unroll
-            for (int d = 0; d < DP / 32; ++d)
+            for (int d = 0; d < ND; ++d)
 #pragma unroll
                 for (int r = 0; r < 16; r += 4) {
                     float *at = buf + (v - 1) * 2 * 32 * LD + 32 * d + 2 * r;
@@ -853,7 +860,7 @@ __global__ __launch_bounds__(NT, (KW > 1 ? 1 : BIAS ? Shape<T, DP>::KV_BIAS_WAVE
 #pragma unroll
         for (int v = 1; v < KW; ++v)
 #pragma unroll
-            for (int d = 0; d < DP / 32; ++d)
+            for (int d = 0; d < ND; ++d)
 #pragma unroll
                 for (int r = 0; r < 16; r += 4) {
                     const float *at = buf + (v - 1) * 2 * 32 * LD + 32 * d + 2 * r;
@@ -868,7 +875,7 @@ __global__ __launch_bounds__(NT, (KW > 1 ? 1 : BIAS ? Shape<T, DP>::KV_BIAS_WAVE
             const int64_t at = ((((int64_t)w.b * a.Nk + j) * a.Hk + w.h) * a.groups + w0.h % a.groups) * a.D;
             float *ok_ = a.part + at, *ov = a.sums + at;
 #pragma unroll
-            for (int d = 0; d < DP / 32; ++d)
+            for (int d = 0; d < ND; ++d)
 #pragma unroll
                 for (int r = 0; r < 16; r += 4) {
                     const int col = 32 * d + 2 * r + 4 * half;
@@ -883,7 +890,7 @@ __global__ __launch_bounds__(NT, (KW > 1 ? 1 : BIAS ? Shape<T, DP>::KV_BIAS_WAVE
         const int64_t at = (((int64_t)w.b * a.Nk + j) * a.Hk + w.h) * a.D;
         T *ok_ = static_cast<T *>(a.dk) + at, *ov = static_cast<T *>(a.dv) + at;
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
+        for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
                 const int col = 32 * d + 2 * r + 4 * half;
@@ -965,9 +972,9 @@ struct Diagonals {
 // dq of 128 / KW rows (KW waves share 32, each taking every KW-th 32 keys), and the bias gradient's
 // sums over their diagonals.  2 x 4096 x 16 heads x 128 bf16: 435 us (950 TFLOP/s); 64 columns 257 us
 // (800); f32 2 x 2048 x 8 x 64: 164 us (157).
-template <class T, int DP, int KT, int KW, bool BIAS>
-__global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::Q_WAVES : 1)) void attn_bwd_q(Args a) {
-    constexpr int NP = Elem<T>::NP, PP = prob_pieces<T, KW>(), PLANE = KT * DP, ROWS = 128 / KW;
+template <class T, int DW, int KT, int KW, bool BIAS>
+__global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DW>::Q_WAVES : 1)) void attn_bwd_q(Args a) {
+    constexpr int NP = Elem<T>::NP, PP = prob_pieces<T, KW>(), DP = pitch(DW), ND = blocks(DW), PLANE = KT * DP, ROWS = 128 / KW;
     static_assert(KT % (32 * KW) == 0, "tile");
     extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
     typedef Tiles<T, DP, KT> KV;
@@ -987,24 +994,24 @@ __global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::Q_WAVES : 1)) void att
         fill_table(a, tab, w.h);
         for (int o = threadIdx.x; o < 4 * W; o += NT) all_bins[o] = 0.f;
     }
-    bf16x8 qf[DP / 16][NP], df[DP / 16][NP];
-    load_row<T, DP>(static_cast<const T *>(a.q) + w.b * a.qs[0] + (int64_t)i * a.qs[1] + w.h * a.qs[2], i < sp.nq, a.D,
+    bf16x8 qf[DW / 16][NP], df[DW / 16][NP];
+    load_row<T, DW>(static_cast<const T *>(a.q) + w.b * a.qs[0] + (int64_t)i * a.qs[1] + w.h * a.qs[2], i < sp.nq, a.D,
                     lane, qf);
     // The matrix cores round sums down, not to nearest: do . v comes out about 1e-8 of its size too
     // low, which a single ds does not feel but a bias gradient's sum over 10^6 of them does (f32: 9
     // times the error of one rounded to nearest).  Odd queries take -do, and their error the other way.
     const bool odd = NP > 1 && (lane & 1);
-    load_row<T, DP>(static_cast<const T *>(a.dout) + w.b * a.dos[0] + (int64_t)i * a.dos[1] + w.h * a.dos[2], i < sp.nq,
+    load_row<T, DW>(static_cast<const T *>(a.dout) + w.b * a.dos[0] + (int64_t)i * a.dos[1] + w.h * a.dos[2], i < sp.nq,
                     a.D, lane, df, odd);
     const float sign = odd ? -1.f : 1.f;
     const size_t row = ((size_t)w.b * a.H + w.h) * a.Nq + i;
     const RowSum rs = row_sum_of<T>(a, row, i < sp.nq);
-    const float delta = row_dot<T, DP>(a, w.b, w.h, i, i < sp.nq, lane);
+    const float delta = row_dot<T, DW>(a, w.b, w.h, i, i < sp.nq, lane);
     if (half == 0 && share == 0 && i < a.Nq) a.delta[row] = delta;  // (the key gradients read it)
     const float scale2 = a.scale * LOG2E;
-    f32x16 acc[DP / 32];
+    f32x16 acc[ND];
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d) acc[d] = zero16();
+    for (int d = 0; d < ND; ++d) acc[d] = zero16();
     Diagonals dg;
     const int last = min(q0 + ROWS, sp.nq) - 1;
     const int kend = last < q0 ? 0 : a.causal ? min(sp.nk, max(last + sp.start + 1, 0)) : sp.nk;
@@ -1015,7 +1022,7 @@ __global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::Q_WAVES : 1)) void att
     for (int j0 = 0; j0 < kend; j0 += KT) {
         kv.land(j0, sp.nk, mask);
         const uint16_t *kt = kv.x(), *vt = kv.y();
-        if constexpr (Shape<T, DP>::TIGHT) at.opaque();
+        if constexpr (Shape<T, DW>::TIGHT) at.opaque();
         if (j0 + KT < kend) kv.issue(K, a.ks[1], V, a.vs[1], j0 + KT, sp.nk, a.D, mask);
         const int qw = q0 + 32 * (wave / KW) + sp.start;
 #pragma unroll
@@ -1025,7 +1032,7 @@ __global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::Q_WAVES : 1)) void att
             const bool edge = mask || j + 32 > sp.nk || (a.causal && j + 31 > qw);
             f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) {
+            for (int c = 0; c < DW / 16; ++c) {
                 bf16x8 f[NP];
                 row_frag<DP>(kt, PLANE, 32 * t, c, at, f);
                 mma(s, f, qf[c]);
@@ -1048,7 +1055,7 @@ __global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::Q_WAVES : 1)) void att
                 bf16x8 sf[PP];
                 to_pieces<PP>(x, sf);
 #pragma unroll
-                for (int d = 0; d < DP / 32; ++d) {
+                for (int d = 0; d < ND; ++d) {
                     bf16x8 f[NP];
                     col_frag<DP>(kt, PLANE, 32 * t + 16 * c, 32 * d, at, f);
                     mma(acc[d], f, sf);
@@ -1063,7 +1070,7 @@ __global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::Q_WAVES : 1)) void att
 #pragma unroll
         for (int v = 1; v < KW; ++v)
 #pragma unroll
-            for (int d = 0; d < DP / 32; ++d)
+            for (int d = 0; d < ND; ++d)
 #pragma unroll
                 for (int r = 0; r < 16; r += 4)
                     if (share == v)
@@ -1072,7 +1079,7 @@ __global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::Q_WAVES : 1)) void att
 #pragma unroll
         for (int v = 1; v < KW; ++v)
 #pragma unroll
-            for (int d = 0; d < DP / 32; ++d)
+            for (int d = 0; d < ND; ++d)
 #pragma unroll
                 for (int r = 0; r < 16; r += 4) {
                     const f32x4 x = *reinterpret_cast<const f32x4_m *>(buf + (v - 1) * 32 * LD + 32 * d + 2 * r);
@@ -1084,7 +1091,7 @@ __global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DP>::Q_WAVES : 1)) void att
         T *o = static_cast<T *>(a.dq) + (((int64_t)w.b * a.Nq + i) * a.H + w.h) * a.D;
         const float f = a.scale;
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
+        for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
                 const int col = 32 * d + 2 * r + 4 * half;
@@ -1191,7 +1198,7 @@ int take(const hreg_tok_attn_t *p, Args &a) {
     return HREG_OK;
 }
 
-// launches F<T, DP, tile, BIAS> with its dynamic LDS (above the 64 KB default where needed)
+// launches F<T, DW, tile, BIAS> with its dynamic LDS (above the 64 KB default where needed)
 template <class K>
 int launch(K *kernel, int grid, size_t lds, void *stream, const Args &a) {
     if (lds > 65536 &&
@@ -1202,16 +1209,17 @@ int launch(K *kernel, int grid, size_t lds, void *stream, const Args &a) {
     return HREG_OK;
 }
 
-template <class T, int DP, bool BIAS>
+template <class T, int DW, bool BIAS>
 int fwd(const Args &a, void *stream) {
     if (a.splits) {
         const int R = a.Nq * (a.H / a.Hk);
+        constexpr int DP = pitch(DW);
         const size_t tile = (size_t)4 * Elem<T>::NP * 32 * DP * 2, join = (size_t)4 * 32 * (DP + 4) * 4;
         Args b = a;
         b.split_bytes = tile > join ? tile : join;
         const size_t tables = BIAS ? (size_t)(a.H / a.Hk) * (2 * (a.bk.far + PAD) + 1) * 4 : 0;
         b.group_tables = tables <= 32768;
-        const int rc = launch(attn_split<T, DP, BIAS>, a.B * a.Hk * ((R + 31) / 32) * a.splits,
+        const int rc = launch(attn_split<T, DW, BIAS>, a.B * a.Hk * ((R + 31) / 32) * a.splits,
                               b.split_bytes + (b.group_tables ? tables : 0), stream, b);
         if (rc != HREG_OK || a.splits == 1) return rc;
         const int64_t rows = (int64_t)a.B * a.H * a.Nq;
@@ -1219,38 +1227,38 @@ int fwd(const Args &a, void *stream) {
         HREG_CHECK_LAUNCH();
         return HREG_OK;
     }
-    constexpr int KT = Shape<T, DP>::FWD_KEYS;
-    const size_t lds = Tiles<T, DP, KT>::BYTES + (BIAS ? (2 * (a.bk.far + PAD) + 1) * 4 : 0);
-    return launch(attn_fwd<T, DP, KT, BIAS>, a.B * a.H * row_tiles(a.Nq), lds, stream, a);
+    constexpr int KT = Shape<T, DW>::FWD_KEYS;
+    const size_t lds = Tiles<T, pitch(DW), KT>::BYTES + (BIAS ? (2 * (a.bk.far + PAD) + 1) * 4 : 0);
+    return launch(attn_fwd<T, DW, KT, BIAS>, a.B * a.H * row_tiles(a.Nq), lds, stream, a);
 }
 
-template <class T, int DP, int KW, bool BIAS>
+template <class T, int DW, int KW, bool BIAS>
 int bwd_kv(const Args &a, void *stream) {
-    constexpr int QT = KW > 1 ? 32 * KW : Shape<T, DP>::BWD_ROWS;
-    const size_t lds = area<T, DP, QT, KW, 2>() + (6 * QT + (BIAS ? 2 * (a.bk.far + PAD) + 1 : 0)) * 4;
-    return launch(attn_bwd_kv<T, DP, QT, KW, BIAS>, a.B * a.Hk * a.groups * ((a.Nk + 128 / KW - 1) / (128 / KW)), lds, stream, a);
+    constexpr int QT = KW > 1 ? 32 * KW : Shape<T, DW>::BWD_ROWS;
+    const size_t lds = area<T, pitch(DW), QT, KW, 2>() + (6 * QT + (BIAS ? 2 * (a.bk.far + PAD) + 1 : 0)) * 4;
+    return launch(attn_bwd_kv<T, DW, QT, KW, BIAS>, a.B * a.Hk * a.groups * ((a.Nk + 128 / KW - 1) / (128 / KW)), lds, stream, a);
 }
-template <class T, int DP, int KW, bool BIAS>
+template <class T, int DW, int KW, bool BIAS>
 int bwd_q(const Args &a, void *stream) {
-    constexpr int KT = KW > 1 ? 32 * KW : Shape<T, DP>::Q_KEYS;
-    const size_t W = 2 * a.bk.far + 1, lds = area<T, DP, KT, KW, 1>() + (BIAS ? W + 2 * PAD + 4 * W : 0) * 4;
-    return launch(attn_bwd_q<T, DP, KT, KW, BIAS>, a.B * a.H * ((a.Nq + a.tile_rows - 1) / a.tile_rows), lds, stream, a);
+    constexpr int KT = KW > 1 ? 32 * KW : Shape<T, DW>::Q_KEYS;
+    const size_t W = 2 * a.bk.far + 1, lds = area<T, pitch(DW), KT, KW, 1>() + (BIAS ? W + 2 * PAD + 4 * W : 0) * 4;
+    return launch(attn_bwd_q<T, DW, KT, KW, BIAS>, a.B * a.H * ((a.Nq + a.tile_rows - 1) / a.tile_rows), lds, stream, a);
 }
 
-template <class T, int DP, bool BIAS>
+template <class T, int DW, bool BIAS>
 int bwd(const Args &a, void *stream) {
-    constexpr int SHARE = Shape<T, DP>::SHARE;
+    constexpr int SHARE = Shape<T, DW>::SHARE;
     int rc = HREG_OK;
     // the query gradients' kernel first: it leaves the rows' dots for the key gradients
     if (a.Nq > 0 && (a.dq || a.dbias)) {
-        rc = a.tile_rows < ROWS ? bwd_q<T, DP, SHARE, BIAS>(a, stream) : bwd_q<T, DP, 1, BIAS>(a, stream);
+        rc = a.tile_rows < ROWS ? bwd_q<T, DW, SHARE, BIAS>(a, stream) : bwd_q<T, DW, 1, BIAS>(a, stream);
     } else if (a.Nq > 0) {
         const int64_t rows = (int64_t)a.B * a.H * a.Nq;
-        hipLaunchKernelGGL((attn_delta<T, DP>), dim3((rows + NT / 2 - 1) / (NT / 2)), dim3(NT), 0, as_stream(stream), a);
+        hipLaunchKernelGGL((attn_delta<T, DW>), dim3((rows + NT / 2 - 1) / (NT / 2)), dim3(NT), 0, as_stream(stream), a);
         HREG_CHECK_LAUNCH();
     }
     if (rc == HREG_OK && a.Nk > 0 && a.dk) {
-        rc = a.share_kv ? bwd_kv<T, DP, SHARE, BIAS>(a, stream) : bwd_kv<T, DP, 1, BIAS>(a, stream);
+        rc = a.share_kv ? bwd_kv<T, DW, SHARE, BIAS>(a, stream) : bwd_kv<T, DW, 1, BIAS>(a, stream);
         if (rc == HREG_OK && a.groups > 1) {
             const int64_t n = (int64_t)a.B * a.Nk * a.Hk * (a.D / 4);
             hipLaunchKernelGGL(sum_group<T>, dim3((n + NT - 1) / NT, 2), dim3(NT), 0, as_stream(stream), a);
@@ -1264,11 +1272,15 @@ template <class T, bool BIAS, bool BACK>
 int by_width(const Args &a, void *stream) {
     if constexpr (BACK) {
         if (a.D <= 32) return bwd<T, 32, BIAS>(a, stream);
+        if (a.D <= 48) return bwd<T, 48, BIAS>(a, stream);
         if (a.D <= 64) return bwd<T, 64, BIAS>(a, stream);
+        if (a.D <= 96) return bwd<T, 96, BIAS>(a, stream);
         return bwd<T, 128, BIAS>(a, stream);
     } else {
         if (a.D <= 32) return fwd<T, 32, BIAS>(a, stream);
+        if (a.D <= 48) return fwd<T, 48, BIAS>(a, stream);
         if (a.D <= 64) return fwd<T, 64, BIAS>(a, stream);
+        if (a.D <= 96) return fwd<T, 96, BIAS>(a, stream);
         return fwd<T, 128, BIAS>(a, stream);
     }
 }

@@ -44,6 +44,12 @@ ATTN = [  # B, Nq, Nk, heads, key heads, width, causal, key lengths, query lengt
     (1, 60, 5000, 8, 1, 32, True, [4801], None, True, (32, 128, False)),  # many rows a key head, few tiles
     (2, 1, 333, 40, 1, 64, True, [333, 1], None, False, (16, 40, False)),  # more heads than a tile has rows
     (1, 2, 100, 64, 2, 32, True, None, None, False, (32, 1024, True)),  # tables too large for a group
+    (2, 70, 150, 4, 2, 96, True, [150, 33], None, False, None),
+    (1, 140, 90, 2, 2, 56, False, None, None, True, (16, 20, True)),
+    (1, 75, 75, 4, 1, 104, True, None, None, False, None),
+    (2, 3, 400, 8, 2, 88, True, [400, 129], None, False, (32, 128, False)),
+    (20, 130, 140, 8, 2, 48, True, None, None, False, None),  # waves with rows of their own
+    (20, 130, 140, 8, 2, 88, False, None, None, True, (16, 20, True)),
 ]
 
 
