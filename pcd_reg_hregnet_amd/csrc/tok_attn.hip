@@ -25,6 +25,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int NT = 256;          // threads a workgroup
 constexpr int ROWS = 128;        // rows a workgroup owns: 32 a wave
 constexpr int CUS = 256;
+constexpr int FEW_KEYS = 64;     // one tile
 constexpr int MAX_BINS = 2049;   // offsets -max_distance .. max_distance with max_distance <= 1024
 
 // DW: a call's width rounded up to 32, 48, 64, 96 or 128 columns, which scores are summed over and
@@ -359,7 +360,7 @@ __device__ __forceinline__ void finish_row(const Args &a, int b, int i, int h, i
 // and a quarter-rate exponential a score against 16 cycles of matrix product), at 128 columns by both
 // and by the waits between them; f32 by its six products.  2 x 4096 x 16 heads: 128 columns 302 us
 // (910 TFLOP/s), 64 columns 183 us (750); f32 2 x 2048 x 8 x 64: 116 us (148).
-template <class T, int DW, int KT, bool BIAS>
+template <class T, int DW, int KT, bool BIAS, int PP>
 __global__ __launch_bounds__(NT, (Shape<T, DW>::FWD_WAVES)) void attn_fwd(Args a) {
     constexpr int NP = Elem<T>::NP, DP = pitch(DW), ND = blocks(DW), MT = KT / 32, PLANE = KT * DP;
     extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
@@ -444,13 +445,13 @@ __global__ __launch_bounds__(NT, (Shape<T, DW>::FWD_WAVES)) void attn_fwd(Args a
         l += sum;
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-            bf16x8 pf[2][NP];
+            bf16x8 pf[2][PP];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 float p[8];
 #pragma unroll
                 for (int r = 0; r < 8; ++r) p[r] = s[t][8 * c + r];
-                to_pieces<NP>(p, pf[c]);
+                to_pieces<PP>(p, pf[c]);
             }
             add_rows<DP, ND, NP>(acc, vt, PLANE, 32 * t, at, pf);
         }
@@ -1256,7 +1257,14 @@ int fwd(const Args &a, void *stream) {
     }
     constexpr int KT = Shape<T, DW>::FWD_KEYS;
     const size_t lds = Tiles<T, pitch(DW), KT>::BYTES + (BIAS ? (2 * (a.bk.far + PAD) + 1) * 4 : 0);
-    return launch(attn_fwd<T, DW, KT, BIAS>, a.B * a.H * row_tiles(a.Nq), lds, stream, a);
+    // Few keys average little of p's rounding to 8 bits away, and its error in out, through D = do . o,
+    // is common to a row's ds: a bias gradient takes 16 bits of p there (3 x 237 queries x 32 heads x 72:
+    // 9 keys 3.1e-3 -> 1.6e-3 off, of which 1.6e-3 is its own rounding, 60 keys 2.3e-3 -> 1.6e-3, the
+    // same 24 and 22 us; 120 keys are at 1.9e-3 without).
+    constexpr int NP = Elem<T>::NP;
+    if constexpr (BIAS && NP == 1)
+        if (a.rest && a.Nk <= FEW_KEYS) return launch(attn_fwd<T, DW, KT, BIAS, 2>, a.B * a.H * row_tiles(a.Nq), lds, stream, a);
+    return launch(attn_fwd<T, DW, KT, BIAS, NP>, a.B * a.H * row_tiles(a.Nq), lds, stream, a);
 }
 
 template <class T, int DW, int KW, bool BIAS>
@@ -1326,6 +1334,7 @@ int by_type(const hreg_tok_attn_t *p, const Args &a, void *stream) {
 int split_of(const hreg_tok_attn_t *p) {
     const int64_t R = (int64_t)p->Nq * (p->H / p->Hk), tiles = (int64_t)p->B * p->Hk * ((R + 31) / 32);
     const int64_t rows = (int64_t)p->B * p->H * row_tiles(p->Nq);
+    if (p->bias && p->out_rest && p->Nk <= FEW_KEYS) return 0;  // (fwd() has a form of its own for them)
     if (tiles == 0 || (R > 32 && (rows >= CUS || p->Nk <= 16 * rows))) return 0;
     int64_t s = (2 * CUS + tiles - 1) / tiles, most = (p->Nk + 255) / 256;
     s = s < most ? s : most;

@@ -115,6 +115,19 @@ def test_attention_float32_table_with_bf16_rows():
     check_attn(got, *case)
 
 
+@pytest.mark.parametrize("Nq", [237, 3])
+def test_attention_few_keys_bias_gradient(Nq):
+    """bf16 rows, nine keys, a float32 table: p in 16 bits and out with its remainder leave 2^-15 of the
+    terms of D = do . o, which the sums over rows bring down to no less than a sixteenth (8 bits of p
+    would be 2^-8 of them)"""
+    case = attn_case(13, (3, Nq, 9, 32, 8, 72, False, None, None, False, (64, 64, True)), H, bias_dtype=F)
+    got = run_attn(*case)
+    check_attn(got, *case)
+    s, kw, bias, spec = case
+    want = oracle.attention(s["q"], s["k"], s["v"], do=s["do"], bias=bias, spec=spec, **kw)["dbias"][0]
+    assert ((got["dbias"].double() - want).norm() / want.norm()).item() < 2 ** -11
+
+
 def test_attention_strides():
     """a packed projection, head-major storage, rows that are not aligned, a batch that is broadcast"""
     B, N, h, D = 2, 45, 3, 32
