@@ -149,16 +149,6 @@ struct Block {
     Rng rng;
 };
 
-// a parameter's elements c .. c + 7, `other` where there is no such parameter
-template <bool VEC>
-__device__ __forceinline__ void param8(const void *p, int f32, int c, int n, float other, float (&v)[8]) {
-    if (!p) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = other;
-    } else if (f32) load8<VEC>(static_cast<const float *>(p) + c, n, v);
-    else load8<VEC>(static_cast<const __bf16 *>(p) + c, n, v);
-}
-
 // A row has TPR threads of eight elements each: 16, 32 or 64 of a wave (the workgroup's 256 threads
 // then hold several rows), or a workgroup of TPR.  A row's waits are hidden by the other rows of its
 // CU, so the fewer registers and the more rows the better (rows of 4096 bf16, backward: 369 us with
@@ -197,6 +187,17 @@ __device__ __forceinline__ void get8(const void *p, int64_t at, int n, float (&v
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = 0.f;
     }
+}
+
+// a parameter's elements c .. c + 7, of which n are there; `other` where there is no such parameter
+// and in a thread behind the row's end (n <= 0), which must not read there
+template <int MODE>
+__device__ __forceinline__ void param8(const void *p, int f32, int c, int n, float other, float (&v)[8]) {
+    if (!p || (MODE != WHOLE && n <= 0)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = other;
+    } else if (f32) load8<(MODE >= ALIGNED)>(static_cast<const float *>(p) + c, n, v);
+    else load8<(MODE >= ALIGNED)>(static_cast<const __bf16 *>(p) + c, n, v);
 }
 
 // mean and 1 / deviation of a row held in registers (two passes: the mean, then the squares
@@ -238,8 +239,8 @@ __global__ __launch_bounds__(threads<TPR>()) void block_fwd(Block a) {
         get8<MODE, T>(a.f, at, n, u);
         if (USUAL || a.post) {
             row_stats<TPR>(u, a.post, inv_c, n, a.eps, mu, rs, lds);
-            param8<VEC>(a.post_w, a.param_f32, c, n, 1.f, w);
-            param8<VEC>(a.post_b, a.param_f32, c, n, 0.f, b);
+            param8<MODE>(a.post_w, a.param_f32, c, n, 1.f, w);
+            param8<MODE>(a.post_b, a.param_f32, c, n, 0.f, b);
 #pragma unroll
             for (int i = 0; i < 8; ++i) u[i] = __builtin_fmaf((u[i] - mu) * rs, w[i], b[i]);
         }
@@ -260,8 +261,8 @@ __global__ __launch_bounds__(threads<TPR>()) void block_fwd(Block a) {
     if (USUAL || a.pre) {
         float w[8], b[8];
         row_stats<TPR>(y, a.pre, inv_c, n, a.eps, mu2, rs2, lds);
-        param8<VEC>(a.pre_w, a.param_f32, c, n, 1.f, w);
-        param8<VEC>(a.pre_b, a.param_f32, c, n, 0.f, b);
+        param8<MODE>(a.pre_w, a.param_f32, c, n, 1.f, w);
+        param8<MODE>(a.pre_b, a.param_f32, c, n, 0.f, b);
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = __builtin_fmaf((y[i] - mu2) * rs2, w[i], b[i]);
         if (n > 0) store8<VEC>(static_cast<T *>(a.h) + at, n, w);
@@ -295,7 +296,7 @@ __device__ __forceinline__ void back_row(const Block &a, int r, int c, uint64_t 
     if (a.gate) get8<MODE, T>(a.gate, (int64_t)(r / a.gate_rows) * C + c, n, q);
     if (pre) {
         float s1 = 0.f, s2 = 0.f;
-        param8<VEC>(a.pre_w, a.param_f32, c, n, 1.f, w);
+        param8<MODE>(a.pre_w, a.param_f32, c, n, 1.f, w);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             x[i] = i < n ? (x[i] - st[2]) * st[3] : 0.f;
@@ -321,14 +322,14 @@ __device__ __forceinline__ void back_row(const Block &a, int r, int c, uint64_t 
     }
     const bool post = USUAL || a.post;
     if (post) {
-        param8<VEC>(a.post_w, a.param_f32, c, n, 1.f, w);
+        param8<MODE>(a.post_w, a.param_f32, c, n, 1.f, w);
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i] = i < n ? (f[i] - st[0]) * st[1] : 0.f;
     }
     if (a.gate) {
         float dg[8];
         if (post) {
-            param8<VEC>(a.post_b, a.param_f32, c, n, 0.f, b);
+            param8<MODE>(a.post_b, a.param_f32, c, n, 0.f, b);
 #pragma unroll
             for (int i = 0; i < 8; ++i) dg[i] = g[i] * __builtin_fmaf(f[i], w[i], b[i]);
         } else {
