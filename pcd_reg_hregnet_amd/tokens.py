@@ -185,7 +185,7 @@ def _attn_forward(o, q, k, v, bias, q_len, k_len, key_mask, train: bool):
     dev = q.device
     out = torch.empty_like(q, memory_format=_DENSE)
     B, Nq, H, _ = q.shape
-    lse = torch.empty(2, B, H, Nq, device=dev) if train else None
+    lse = torch.empty(2, B, H, Nq, dtype=torch.float32, device=dev) if train else None
     rest = torch.empty_like(out) if train and q.dtype != torch.float32 else None
     p = _attn_args(o, q, k, v, out, lse, rest, q_len, k_len, key_mask, bias)
     ws = _attn_ws(p, 0, dev)  # noqa: F841 (held until the launch is queued)
@@ -381,7 +381,7 @@ class _GatedResidualNorm(torch.autograd.Function):
         dev = x.device
         y = torch.empty_like(x) if f is not None else None
         h = torch.empty_like(x) if o[3] else None
-        stats = torch.empty(x.numel() // x.shape[-1], 4, device=dev)
+        stats = torch.empty(x.numel() // x.shape[-1], 4, dtype=torch.float32, device=dev)
         p = _block_args(o, x, param_dtype, seed, x, f, gate, post_w, post_b, pre_w, pre_b, y, h, stats)
         _launch(dev, "hreg_tok_block_fwd", ctypes.byref(p))
         ctx.save_for_backward(f, gate, post_w, post_b, pre_w, pre_b, stats, seed, x if y is None else y)

@@ -1,0 +1,40 @@
+"""What the token operators hand to their C entries and how they answer calls around them, without a GPU:
+the checks for a GPU tensor and the launches are replaced, everything before and after them runs."""
+import pytest
+import torch
+
+from pcd_reg_hregnet_amd import tokens
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """names of the entries that would have run"""
+    names = []
+    monkeypatch.setattr(tokens, "_check_tensor", lambda *a, **k: None)
+    monkeypatch.setattr(tokens, "_launch", lambda device, name, *a: names.append(name))
+    return names
+
+
+def normal(*shape, dtype=torch.float32):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(1)).to(dtype)
+
+
+@pytest.fixture(params=[torch.bfloat16, torch.float16, torch.float64])
+def default_dtype(request):
+    old = torch.get_default_dtype()
+    torch.set_default_dtype(request.param)
+    yield request.param
+    torch.set_default_dtype(old)
+
+
+def test_statistics_are_float32_whatever_the_default_type(launches, default_dtype):
+    """the kernels write float32 statistics: a buffer of torch's default type would be too short"""
+    x = normal(2, 4, 2, 16, dtype=torch.float32)
+    for t in (x, x.bfloat16()):
+        lse = tokens._attn_forward((0.25, False, False, None), t, t, t, None, None, None, None, True)[4]
+        assert lse.dtype == torch.float32 and lse.shape == (2, 2, 2, 4)
+        leaf = t.detach().requires_grad_(True)
+        _, h = tokens.gated_residual_norm(leaf, t)
+        stats = [s for s in h.grad_fn.saved_tensors if s is not None and s.shape == (16, 4)]
+        assert [s.dtype for s in stats] == [torch.float32]
+    assert launches == ["hreg_tok_attn_fwd", "hreg_tok_block_fwd"] * 2
