@@ -25,6 +25,7 @@ import struct
 from dataclasses import dataclass
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -70,6 +71,13 @@ def _check_tensor(fn: str, name: str, t, device=None, dtype=None) -> None:
         raise ValueError(f"{fn}: {name} is on {t.device}, expected {device}")
     if dtype is not None and t.dtype != dtype:
         raise ValueError(f"{fn}: {name} has type {t.dtype}, expected {dtype}")
+
+
+def _any_tangent(*tensors) -> bool:
+    """whether forward-mode differentiation goes through one of them: no operator has that derivative, and
+    an autograd function raises on such a tensor (a plain launch would return a result without it)"""
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _ptr(t):
@@ -240,7 +248,7 @@ def attention(q, k, v, *, scale=None, causal=False, align_end=None, q_lengths=No
     consecutive query heads); float32 or bfloat16, D a multiple of 8 up to 128.  Any strides:
     rows that are not contiguous 16-byte aligned steps are copied first.  Batch x heads x tokens / 128
     (rounded up) stays below 2^24.  scale: D ** -0.5 by default.  Differentiable (once) in q, k, v
-    and bias.
+    and bias; forward-mode derivatives raise.
 
     k_lengths, q_lengths [B] int32 / int64 on the GPU (clamped to the tensors): keys and queries
     from there on do not exist.  key_mask [B or 1, Nk] bool: False keys are not seen.  Their
@@ -294,8 +302,8 @@ def attention(q, k, v, *, scale=None, causal=False, align_end=None, q_lengths=No
             raise ValueError(f"attention: bias must be [{buckets.num_buckets}, {H}], got {tuple(bias.shape)}")
         bias = bias.contiguous()
     o = scale, bool(causal), bool(causal if align_end is None else align_end), buckets
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
-                                    or (bias is not None and bias.requires_grad)):
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                     or (bias is not None and bias.requires_grad))) or _any_tangent(q, k, v, bias):
         return _TokAttention.apply(q, k, v, bias, o, q_len, k_len, key_mask)
     return _attn_forward(o, q, k, v, bias, q_len, k_len, key_mask, False)[3]
 

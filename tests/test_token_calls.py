@@ -38,3 +38,22 @@ def test_statistics_are_float32_whatever_the_default_type(launches, default_dtyp
         stats = [s for s in h.grad_fn.saved_tensors if s is not None and s.shape == (16, 4)]
         assert [s.dtype for s in stats] == [torch.float32]
     assert launches == ["hreg_tok_attn_fwd", "hreg_tok_block_fwd"] * 2
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_derivatives_raise(launches, grad):
+    """no operator returns a result that has lost its tangent"""
+    x, table = normal(1, 5, 2, 16), normal(8, 2)
+    kw = dict(bias=table, buckets=tokens.Buckets(8, 6))
+    with torch.autograd.forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        bias = torch.autograd.forward_ad.make_dual(table, torch.ones_like(table))
+        for call in (lambda: tokens.attention(dual, x, x), lambda: tokens.attention(x, dual, x),
+                     lambda: tokens.attention(x, x, dual), lambda: tokens.attention(x, x, x, **kw | dict(bias=bias)),
+                     lambda: tokens.dropout(dual, 0.5, 1), lambda: tokens.gated_residual_norm(dual, None),
+                     lambda: tokens.gated_residual_norm(x, dual, p=0.1, seed=1)):
+            with pytest.raises(NotImplementedError, match="forward mode"):
+                call()
+        # tensors without a tangent are welcome there
+        assert not tokens.attention(x, x, x, **kw).requires_grad
+    assert not tokens.attention(x, x, x).requires_grad
