@@ -645,7 +645,8 @@ __global__ __launch_bounds__(NT, (Shape<T, DW>::SPLIT_WAVES)) void attn_split(Ar
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
             o += *reinterpret_cast<const f32x4_m *>(part + (v * 32 + q) * OLD + col);
-            sum += ml[v][0][q] == -INFINITY ? 0.f : ml[v][1][q] * __builtin_amdgcn_exp2f(ml[v][0][q] - all);
+            // (no maximum: the sum is 0 where the wave's keys are none, NaN where its scores all are)
+            sum += ml[v][0][q] == -INFINITY ? ml[v][1][q] : ml[v][1][q] * __builtin_amdgcn_exp2f(ml[v][0][q] - all);
         }
         if (a.splits == 1) {
             finish_row<T>(a, w.b, rr / G, w.h * G + rr % G, col, o, all, sum);
@@ -674,8 +675,9 @@ __global__ __launch_bounds__(NT) void attn_join(Args a) {
         float f = 0.f, l = 0.f;  // lane s: run s0 + s
         if (s0 + lane < a.splits) {
             const float m = sums[2 * (s0 + lane)];
+            l = sums[2 * (s0 + lane) + 1];  // (no maximum: 0, or NaN where all scores are)
             f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - all);
-            l = sums[2 * (s0 + lane) + 1] * f;
+            if (m != -INFINITY) l *= f;
         }
         const int n = min(a.splits - s0, 32);
 #pragma unroll 4

@@ -34,3 +34,27 @@ def test_default_type_of_the_program(dtype):
     finally:
         torch.set_default_dtype(torch.float32)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [F, H], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("train", [True, False])
+@pytest.mark.parametrize("shape", [(2, 1, 129, 4, 2, 64), (2, 1, 2000, 4, 2, 64), (2, 300, 150, 4, 4, 64)],
+                         ids=["one run", "eight runs", "row kernel"])
+def test_a_query_that_is_nan_gives_nan(shape, train, dtype):
+    """a row whose scores are NaN is NaN, not the 0 of a row without keys, however the keys are divided;
+    the other rows keep their bits"""
+    B, Nq, Nk, heads, key_heads, D = shape
+    q, k, v = (normal(i, B, n, h, D, dtype=dtype) for i, (n, h) in enumerate(((Nq, heads), (Nk, key_heads), (Nk, key_heads))))
+    bad = q.clone()
+    bad[1, Nq - 1, 1] = float("nan")
+    with torch.set_grad_enabled(train):
+        clean, got = (tokens.attention(t.clone().requires_grad_(train), k, v, causal=True) for t in (q, bad))
+    assert torch.isnan(got[1, Nq - 1, 1]).all()
+    same = torch.ones(B, Nq, heads, dtype=torch.bool, device="cuda")
+    same[1, Nq - 1, 1] = False
+    assert torch.equal(got[same], clean[same]) and torch.isfinite(clean).all()
+    one = v.clone()  # and a single value among many that is NaN reaches every row that sees it
+    one[0, Nk // 2] = float("nan")
+    with torch.no_grad():
+        got = tokens.attention(q, k, one)
+    assert torch.isnan(got[0]).all() and torch.isfinite(got[1]).all()
