@@ -32,6 +32,7 @@ from . import _lib
 _DTYPES = {torch.float32: _lib.TOK_F32, torch.bfloat16: _lib.TOK_BF16}
 _DENSE = torch.contiguous_format
 _NORMS = {None: 0, "rms": 1, "layer": 2}
+_MOST = 1e38  # a scale or eps goes to the kernels as float32, some of them multiplied by log2(e)
 
 
 _ENTRIES = {}
@@ -282,8 +283,8 @@ def attention(q, k, v, *, scale=None, causal=False, align_end=None, q_lengths=No
     if not 8 <= D <= 128 or D % 8:
         raise ValueError(f"attention: width {D} is not a multiple of 8 up to 128")
     scale = D ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError(f"attention: scale {scale} is not finite")
+    if not abs(scale) <= _MOST:
+        raise ValueError(f"attention: scale {scale} is not finite in float32")
     q_len, k_len = _lengths("q_lengths", q_lengths, B, dev), _lengths("k_lengths", k_lengths, B, dev)
     if key_mask is not None:
         _check_tensor("attention", "key_mask", key_mask, dev, torch.bool)
@@ -482,10 +483,10 @@ def gated_residual_norm(x, f, *, gate=None, scale=1.0, post_norm=None, post_weig
             raise ValueError(f"{fn}: f {tuple(f.shape)} does not fit x {tuple(x.shape)}")
         f = f.contiguous()
     scale, eps = float(scale), float(eps)
-    if not math.isfinite(scale):
-        raise ValueError(f"{fn}: scale {scale} is not finite")
-    if not 0.0 <= eps < math.inf:
-        raise ValueError(f"{fn}: eps {eps} is not a finite number >= 0")
+    if not abs(scale) <= _MOST:
+        raise ValueError(f"{fn}: scale {scale} is not finite in float32")
+    if not 0.0 <= eps <= _MOST:
+        raise ValueError(f"{fn}: eps {eps} is not a finite number >= 0 in float32")
     rows = 1
     if gate is not None:
         _check_tensor(fn, "gate", gate, dev, dtype)

@@ -57,3 +57,16 @@ def test_forward_mode_derivatives_raise(launches, grad):
         # tensors without a tangent are welcome there
         assert not tokens.attention(x, x, x, **kw).requires_grad
     assert not tokens.attention(x, x, x).requires_grad
+
+
+@pytest.mark.parametrize("scale", [1e300, -1e300, 3e38, float("inf"), float("nan")])
+def test_scales_that_float32_does_not_hold_are_refused(launches, scale):
+    x = normal(1, 5, 2, 16)
+    with pytest.raises(ValueError, match="scale"):
+        tokens.attention(x, x, x, scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        tokens.gated_residual_norm(x, x, scale=scale)
+    with pytest.raises(ValueError, match="eps"):
+        tokens.gated_residual_norm(x, x, eps=scale)
+    tokens.attention(x, x, x, scale=1e38)
+    assert launches == ["hreg_tok_attn_fwd"]
