@@ -13,7 +13,8 @@
 // the next product sums over keys, and straight (queries x keys) where it sums over queries:
 // the result registers are then already the next product's operand.  Scores, sums and
 // accumulators are f32; p and ds are rounded to bf16 for bf16 tensors (off by at most 2^-8 of
-// each, as the tensors themselves are), and cut into three exact pieces for f32 tensors.
+// each, as the tensors themselves are; to 16 bits where that costs nothing or few keys average too little
+// of it: attn_split, few_keys, prob_pieces), and cut into three exact pieces for f32 tensors.
 
 #include "tokens.h"
 
@@ -25,7 +26,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int NT = 256;          // threads a workgroup
 constexpr int ROWS = 128;        // rows a workgroup owns: 32 a wave
 constexpr int CUS = 256;
-constexpr int FEW_KEYS = 64;     // one tile
+constexpr int FEW_KEYS = 64;
 constexpr int MAX_BINS = 2049;   // offsets -max_distance .. max_distance with max_distance <= 1024
 
 // DW: a call's width rounded up to 32, 48, 64, 96 or 128 columns, which scores are summed over and
@@ -337,6 +338,25 @@ __device__ __forceinline__ void add_rows(f32x16 (&acc)[ND], const uint16_t *tile
     }
 }
 
+// Whether the workgroup's first query sees at most FEW_KEYS keys (the same in every wave), of which
+// `first` exist for it.  Where a bias gradient is to come, bf16 rows take 16 bits of p there: few keys
+// average little of p's rounding to 8 away, and its error in out, through D = do . o, is common to a row's
+// ds (3 x 237 queries x 32 heads x 72: 9 keys 3.1e-3 -> 1.6e-3 off, of which 1.6e-3 is its own rounding, 60
+// keys 2.3e-3 -> 1.6e-3; 120 keys are at 1.9e-3 without).  It is asked of the keys that are seen, not of those
+// that the tensors have room for, so that padding does not change it.
+__device__ __forceinline__ bool few_keys(int first, const uint8_t *mask, int lane) {
+    if (first <= FEW_KEYS) return true;
+    if (!mask) return false;
+    int n = 0;
+    for (int k0 = 0; k0 < first && n <= FEW_KEYS; k0 += 256)
+#pragma unroll
+        for (int u = 0; u < 256; u += 64) {
+            const int k = k0 + u + lane;
+            n += __popcll(__ballot(k < first && mask[min(k, first - 1)]));
+        }
+    return n <= FEW_KEYS;
+}
+
 // one row's result: sums over its keys, written as out (and what training keeps)
 template <class T>
 __device__ __forceinline__ void finish_row(const Args &a, int b, int i, int h, int col, const f32x4 &o, float m, float l) {
@@ -361,7 +381,7 @@ __device__ __forceinline__ void finish_row(const Args &a, int b, int i, int h, i
 // and by the waits between them; f32 by its six products.  2 x 4096 x 16 heads: 128 columns 302 us
 // (910 TFLOP/s), 64 columns 183 us (750); f32 2 x 2048 x 8 x 64: 116 us (148).
 template <class T, int DW, int KT, bool BIAS, int PP>
-__global__ __launch_bounds__(NT, (Shape<T, DW>::FWD_WAVES)) void attn_fwd(Args a) {
+__device__ __forceinline__ void fwd_rows(const Args &a) {
     constexpr int NP = Elem<T>::NP, DP = pitch(DW), ND = blocks(DW), MT = KT / 32, PLANE = KT * DP;
     extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
     typedef Tiles<T, DP, KT> KV;
@@ -470,6 +490,23 @@ __global__ __launch_bounds__(NT, (Shape<T, DW>::FWD_WAVES)) void attn_fwd(Args a
         }
 }
 
+// PP is chosen here, by the keys that the workgroup sees
+template <class T, int DW, int KT, bool BIAS>
+__global__ __launch_bounds__(NT, (Shape<T, DW>::FWD_WAVES)) void attn_fwd(Args a) {
+    constexpr int NP = Elem<T>::NP;
+    if constexpr (BIAS && NP == 1) {
+        const int tiles = (a.Nq + ROWS - 1) / ROWS;
+        const Where w = where(a.B, a.H, tiles);
+        const Span sp = span_of(a, w.b);
+        const int seen = a.causal ? min(sp.nk, (tiles - 1 - w.tile) * ROWS + sp.start + 1) : sp.nk;  // by its first query
+        if (a.rest && few_keys(seen, a.key_mask ? a.key_mask + w.b * a.mask_sb : nullptr, threadIdx.x & 63)) {
+            fwd_rows<T, DW, KT, BIAS, 2>(a);
+            return;
+        }
+    }
+    fwd_rows<T, DW, KT, BIAS, NP>(a);
+}
+
 // ------------------------------------------------------- forward, keys split --
 
 // Few rows, many keys: a workgroup takes 32 rows of one key head (row r is token r / G, head r % G
@@ -477,7 +514,8 @@ __global__ __launch_bounds__(NT, (Shape<T, DW>::FWD_WAVES)) void attn_fwd(Args a
 // four waves take 32 keys each in turn and join in LDS, the runs join in attn_join.  Each wave stages
 // its own keys, then its own values, in its own LDS, without a barrier; the next tile is on its way
 // in registers.  Bound by the bytes of the cache: 8 x up to 32768 keys x 8 key heads x 128 bf16, 805 MB:
-// 153 us (5.3 TB/s; a large copy reaches 4.7).
+// 153 us (5.3 TB/s; a large copy reaches 4.7).  So bf16 keeps 16 bits of p: its second product is 1 % (2 x
+// 16384 keys x 64 heads on 8: 36.7 -> 37.0 us), and out is as near as its own rounding (error 2.2e-3 -> 1.7e-3).
 template <class T, int DP>
 struct WaveStage {
     static constexpr int CPR = DP / 8, N = 32 * CPR / 64, NP = Elem<T>::NP, PLANE = 32 * DP;
@@ -505,7 +543,8 @@ struct WaveStage {
 
 template <class T, int DW, bool BIAS>
 __global__ __launch_bounds__(NT, (Shape<T, DW>::SPLIT_WAVES)) void attn_split(Args a) {
-    constexpr int NP = Elem<T>::NP, DP = pitch(DW), ND = blocks(DW), PLANE = 32 * DP, OLD = DP + 4;  // OLD: a joined row's step in LDS
+    constexpr int NP = Elem<T>::NP, PP = NP == 1 ? 2 : NP, DP = pitch(DW), ND = blocks(DW), PLANE = 32 * DP;
+    constexpr int OLD = DP + 4;  // a joined row's step in LDS
     extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
     __shared__ float ml[4][2][32];
     const int G = a.H / a.Hk, R = a.Nq * G, tiles = (R + 31) / 32;
@@ -602,7 +641,7 @@ __global__ __launch_bounds__(NT, (Shape<T, DW>::SPLIT_WAVES)) void attn_split(Ar
         if (j0 + 128 < j_end) sv.load(V, a.vs[1], j0 + 128, sp.nk, a.D, mask, lane);
         wave_sync();
         float sum = 0.f;
-        bf16x8 pf[2][NP];
+        bf16x8 pf[2][PP];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             float p[8];
@@ -611,7 +650,7 @@ __global__ __launch_bounds__(NT, (Shape<T, DW>::SPLIT_WAVES)) void attn_split(Ar
                 p[e] = __builtin_amdgcn_exp2f(s[8 * c + e] - ref);
                 sum += p[e];
             }
-            to_pieces<NP>(p, pf[c]);
+            to_pieces<PP>(p, pf[c]);
         }
         l += sum;
         add_rows<DP, ND, NP>(acc, buf, PLANE, 0, at, pf);
@@ -1259,14 +1298,7 @@ int fwd(const Args &a, void *stream) {
     }
     constexpr int KT = Shape<T, DW>::FWD_KEYS;
     const size_t lds = Tiles<T, pitch(DW), KT>::BYTES + (BIAS ? (2 * (a.bk.far + PAD) + 1) * 4 : 0);
-    // Few keys average little of p's rounding to 8 bits away, and its error in out, through D = do . o,
-    // is common to a row's ds: a bias gradient takes 16 bits of p there (3 x 237 queries x 32 heads x 72:
-    // 9 keys 3.1e-3 -> 1.6e-3 off, of which 1.6e-3 is its own rounding, 60 keys 2.3e-3 -> 1.6e-3, the
-    // same 24 and 22 us; 120 keys are at 1.9e-3 without).
-    constexpr int NP = Elem<T>::NP;
-    if constexpr (BIAS && NP == 1)
-        if (a.rest && a.Nk <= FEW_KEYS) return launch(attn_fwd<T, DW, KT, BIAS, 2>, a.B * a.H * row_tiles(a.Nq), lds, stream, a);
-    return launch(attn_fwd<T, DW, KT, BIAS, NP>, a.B * a.H * row_tiles(a.Nq), lds, stream, a);
+    return launch(attn_fwd<T, DW, KT, BIAS>, a.B * a.H * row_tiles(a.Nq), lds, stream, a);
 }
 
 template <class T, int DW, int KW, bool BIAS>
@@ -1336,7 +1368,6 @@ int by_type(const hreg_tok_attn_t *p, const Args &a, void *stream) {
 int split_of(const hreg_tok_attn_t *p) {
     const int64_t R = (int64_t)p->Nq * (p->H / p->Hk), tiles = (int64_t)p->B * p->Hk * ((R + 31) / 32);
     const int64_t rows = (int64_t)p->B * p->H * row_tiles(p->Nq);
-    if (p->bias && p->out_rest && p->Nk <= FEW_KEYS) return 0;  // (fwd() has a form of its own for them)
     if (tiles == 0 || (R > 32 && (rows >= CUS || p->Nk <= 16 * rows))) return 0;
     int64_t s = (2 * CUS + tiles - 1) / tiles, most = (p->Nk + 255) / 256;
     s = s < most ? s : most;

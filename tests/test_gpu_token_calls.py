@@ -58,3 +58,40 @@ def test_a_query_that_is_nan_gives_nan(shape, train, dtype):
     with torch.no_grad():
         got = tokens.attention(q, k, one)
     assert torch.isnan(got[0]).all() and torch.isfinite(got[1]).all()
+
+
+@pytest.mark.parametrize("Nq", [237, 3])  # the row kernel, and the one that splits the keys
+@pytest.mark.parametrize("room", ["exact", "lengths", "mask", "both"])
+def test_bias_gradient_of_few_keys_is_the_same_with_padding(room, Nq):
+    """bf16 rows, nine keys, a float32 table: the gradient keeps 2^-11 whether the tensors hold nine keys or
+    five hundred of which lengths or a mask leave nine (p in 16 bits and out with its remainder leave 2^-15
+    of the terms of D = do . o, which the sums over rows bring down to no less than a sixteenth)"""
+    B, heads, key_heads, D, n, spec = 3, 32, 8, 72, 9, (64, 64, True)
+    N = n if room == "exact" else 500
+    q, do, k, v = (normal(i, B, m, h, D, dtype=H) for i, (m, h) in enumerate(((Nq, heads), (Nq, heads), (N, key_heads), (N, key_heads))))
+    bias = normal(9, spec[0], heads).requires_grad_(True)
+    kw = {}
+    if room in ("lengths", "both"):
+        kw["k_lengths"] = torch.full((B,), n if room == "lengths" else 300, device="cuda", dtype=torch.int32)
+    if room in ("mask", "both"):
+        kw["key_mask"] = torch.zeros(B, N, dtype=torch.bool, device="cuda")
+        kw["key_mask"][:, :n] = True
+        kw["key_mask"][:, 300:] = room == "both"  # (behind the lengths)
+    out = tokens.attention(q, k, v, bias=bias, buckets=tokens.Buckets(*spec), **kw)
+    got, = torch.autograd.grad(out, bias, do)
+    want = oracle.attention(q, k[:, :n], v[:, :n], do=do, bias=bias.detach(), spec=spec)["dbias"][0]
+    assert ((got.double() - want).norm() / want.norm()).item() < 2 ** -11
+
+
+def test_bias_gradient_of_a_causal_call_keeps_its_early_rows():
+    """bf16 rows: the first rows of a causal call see few keys and have the largest ds, so the table's gradient
+    (float32) follows theirs.  Rows that see more than 64 keys keep 8 bits of p, off by 2^-9 (root mean square
+    2^-9 / sqrt(3)) of single terms; over 64 keys or more out loses an eighth of that at most, 2^-12 / sqrt(3), and
+    D, a sum of D values like the others, no larger part: 2^-11 of the whole covers both."""
+    N, heads, D, spec = 300, 8, 64, (32, 128, False)
+    q, k, v, do = (normal(i, 2, N, heads, D, dtype=H) for i in range(4))
+    bias = normal(9, spec[0], heads).requires_grad_(True)
+    out = tokens.attention(q, k, v, causal=True, bias=bias, buckets=tokens.Buckets(*spec))
+    got, = torch.autograd.grad(out, bias, do)
+    want = oracle.attention(q, k, v, do=do, causal=True, bias=bias.detach(), spec=spec)["dbias"][0]
+    assert ((got.double() - want).norm() / want.norm()).item() < 2 ** -11
