@@ -16,6 +16,8 @@
 // each, as the tensors themselves are; to 16 bits where that costs nothing or few keys average too little
 // of it: attn_split, few_keys, prob_pieces), and cut into three exact pieces for f32 tensors.
 
+#include <float.h>
+
 #include "tokens.h"
 
 namespace {
@@ -88,9 +90,12 @@ __device__ __forceinline__ int bucket_of(const Buckets &bk, int o) {
     return b + (bk.both && o > 0 ? bk.n / 2 : 0);
 }
 
+// a bucket's bias in units of log2.  A finite one stays finite: the type's lowest value leaves a key visible
+// (a row that sees only such keys shares itself out among them), -infinity alone hides it.
 __device__ __forceinline__ float bias_at(const Args &a, int b, int h) {
     const size_t at = (size_t)b * a.H + h;
-    return a.bias_f32 ? static_cast<const float *>(a.bias)[at] : (float)static_cast<const __bf16 *>(a.bias)[at];
+    const float v = a.bias_f32 ? static_cast<const float *>(a.bias)[at] : (float)static_cast<const __bf16 *>(a.bias)[at];
+    return fabsf(v) < INFINITY ? fminf(fmaxf(v * LOG2E, -FLT_MAX), FLT_MAX) : v;
 }
 
 // This workgroup's batch entry, head and tile.  Workgroups go round the 8 XCDs: each XCD takes whole
@@ -260,7 +265,7 @@ __device__ __forceinline__ int table_size(int far) { return 2 * (far + PAD) + 1;
 __device__ __forceinline__ void fill_table(const Args &a, float *tab, int h) {
     const int far = a.bk.far;
     for (int o = threadIdx.x; o < table_size(far); o += NT)
-        tab[o] = bias_at(a, bucket_of(a.bk, min(max(o - far - PAD, -far), far)), h) * LOG2E;
+        tab[o] = bias_at(a, bucket_of(a.bk, min(max(o - far - PAD, -far), far)), h);
 }
 
 // Scores of 32 keys (rows) against the wave's 32 queries (columns) in units of log2: s = s * scale2 +
@@ -568,8 +573,8 @@ __global__ __launch_bounds__(NT, (Shape<T, DW>::SPLIT_WAVES)) void attn_split(Ar
             for (int g = 0; g < G; ++g) fill_table(a, at + g * W, w.h * G + g);
             tab = at + (hb - w.h * G) * W + a.bk.far + PAD;
         }
-        left = bias_at(a, bucket_of(a.bk, -a.bk.far), hb) * LOG2E;
-        right = bias_at(a, bucket_of(a.bk, a.bk.far), hb) * LOG2E;
+        left = bias_at(a, bucket_of(a.bk, -a.bk.far), hb);
+        right = bias_at(a, bucket_of(a.bk, a.bk.far), hb);
         __syncthreads();
     }
     bf16x8 qf[DW / 16][NP];
@@ -619,7 +624,7 @@ __global__ __launch_bounds__(NT, (Shape<T, DW>::SPLIT_WAVES)) void attn_split(Ar
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const int o = min(max(kpos + 8 * (e >> 2) + 4 * half + (e & 3), -a.bk.far), a.bk.far);
-                s[e] = __builtin_fmaf(s[e], scale2, bias_at(a, bucket_of(a.bk, o), r < R ? h : w.h * G) * LOG2E);
+                s[e] = __builtin_fmaf(s[e], scale2, bias_at(a, bucket_of(a.bk, o), r < R ? h : w.h * G));
             }
         }
         if (edge) keep_only(s, visible(a, kpos, seen_keys(j0, sp.nk, mask), half), -INFINITY);

@@ -263,7 +263,8 @@ def attention(q, k, v, *, scale=None, causal=False, align_end=None, q_lengths=No
     up to its own position.
 
     bias [num_buckets, H] (float32 or q's type) and ``Buckets`` add a learned bias by the offset of
-    key and query.  With bfloat16 rows its gradient has their accuracy (about 2^-8 of it)."""
+    key and query.  A finite entry hides no key, however low: rows that see nothing else share themselves out
+    among such keys.  With bfloat16 rows its gradient has their accuracy (about 2^-8 of it)."""
     _check_tensor("attention", "q", q)
     dev, dtype = q.device, q.dtype
     for name, t in (("k", k), ("v", v)):

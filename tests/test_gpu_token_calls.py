@@ -95,3 +95,45 @@ def test_bias_gradient_of_a_causal_call_keeps_its_early_rows():
     got, = torch.autograd.grad(out, bias, do)
     want = oracle.attention(q, k, v, do=do, causal=True, bias=bias.detach(), spec=spec)["dbias"][0]
     assert ((got.double() - want).norm() / want.norm()).item() < 2 ** -11
+
+
+@pytest.mark.parametrize("dtype,table", [(F, F)], ids=["fp32"])
+@pytest.mark.parametrize("shape", [(2, 70, 70, 4, 2, 32), (2, 1, 300, 4, 2, 64), (10, 130, 130, 8, 2, 64)],
+                         ids=["waves share rows", "keys split", "waves of their own"])
+@pytest.mark.parametrize("value", ["lowest", "-1e9", "largest"])
+def test_rows_whose_every_key_has_an_extreme_bias(value, shape, table, dtype):
+    """a finite bias hides no key: where all that a row sees have the type's lowest value (or -1e9, the largest) the
+    scores are absorbed and every key has the same share, forward and backward.  q is 0, so nothing but
+    shares of 1 / n is left; p is rounded once, out twice and ds, a product of both, not more often than four
+    times"""
+    B, Nq, Nk, heads, key_heads, D = shape
+    k, v, do = (normal(i, B, n, h, D, dtype=dtype) for i, (n, h) in enumerate(((Nk, key_heads), (Nk, key_heads), (Nq, heads))))
+    q = torch.zeros(B, Nq, heads, D, device="cuda", dtype=dtype)
+    low = {"lowest": torch.finfo(table).min, "-1e9": -1e9, "largest": torch.finfo(table).max}[value]
+    bias = torch.full((16, heads), low, device="cuda", dtype=table)
+    bias[:, 0] = 0  # (a head without)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v, bias)]
+    out = tokens.attention(*leaves[:3], causal=True, bias=leaves[3], buckets=tokens.Buckets(16, 30, False))
+    got = dict(zip(("out", "dq", "dk", "dv", "dbias"), (out.detach(), *torch.autograd.grad(out, leaves, do))))
+    want = oracle.attention(q, k, v, do=do, causal=True, bias=torch.zeros_like(bias), spec=(16, 30, False))
+    u = max(oracle.U[dtype], 2.0 ** -20)  # (float32: sums over some hundred keys)
+    for n in ("out", "dq", "dv", "dbias"):
+        a, b = got[n].double(), want[n][0]
+        assert ((a - b).norm() / b.norm()).item() < 4 * u, n
+    assert not got["dk"].any()  # (q is 0)
+
+
+@pytest.mark.parametrize("dtype", [F, H], ids=["fp32", "bf16"])
+def test_a_key_with_the_lowest_bias_that_stands_alone(dtype):
+    """the first row of a causal call sees its own key alone, whatever its bias; the others leave theirs out"""
+    N, D = 40, 32
+    q, k, v = (normal(i, 1, N, 2, D, dtype=dtype) for i in range(3))
+    bias = torch.zeros(8, 2, device="cuda", dtype=dtype)
+    bias[0] = torch.finfo(dtype).min
+    with torch.no_grad():
+        for rows in (N, 1):  # the row kernel's first row; a single token before a cache of one key
+            out = tokens.attention(q[:, :rows], k[:, :rows], v[:, :rows], causal=True, bias=bias, buckets=tokens.Buckets(8, 6, False))
+            assert torch.equal(out[:, 0], v[:, 0])
+    low = oracle.attention(q, k, v, causal=True, bias=bias, spec=(8, 6, False))["out"][0]
+    out = tokens.attention(q, k, v, causal=True, bias=bias, buckets=tokens.Buckets(8, 6, False))
+    assert ((out.double() - low).norm() / low.norm()).item() < 4 * max(oracle.U[dtype], 2.0 ** -20)
