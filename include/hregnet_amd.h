@@ -786,8 +786,9 @@ typedef struct {
     const void *q, *k, *v;
     void *out; /* read by the backward pass */
     int64_t qs[3], ks[3], vs[3], os[3];
-    /* written by fwd (or NULL), read by bwd: lse [2][B][H][Nq], for f32 rows the rows' largest score
-     * (in units of log2) and 1 / sum, for bf16 rows log2 of their sums and nothing; out_rest, like
+    /* written by fwd (or NULL), read by bwd: lse [2][B][H][Nq]: the rows' largest score (in
+     * units of log2) and 1 / sum; bf16 rows log2 of their sums and 1 (with a bias: where that score is
+     * below 4096; without: 1 is not written); out_rest, like
      * out but contiguous, bf16 only: what out lost in rounding */
     float *lse;
     void *out_rest;

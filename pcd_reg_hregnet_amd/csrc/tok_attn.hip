@@ -70,6 +70,7 @@ struct Args {
     void *out, *rest, *dq, *dk, *dv, *dbias;
     float *lse, *delta, *bins, *part, *sums;
     const int *q_len, *k_len;
+    int *own;  // [B][H][tiles][waves]: whether the wave has a row with a 1 / sum of its own (bf16 with a bias)
     const uint8_t *key_mask;
     const void *bias;
     int64_t qs[3], ks[3], vs[3], os[3], dos[3], mask_sb;
@@ -230,29 +231,29 @@ __device__ __forceinline__ void load_row(const T *row, bool ok, int D, int lane,
 // What the backward pass makes a row's probabilities from.  bf16: p = exp2(s - log2 of the sum).
 // f32: p = exp2(s - m) / sum with the forward pass's own m and 1 / sum, because the logarithm of a
 // sum near 2^10 is rounded by 2^-21 and that error would be common to a row: it does not cancel in
-// the bias gradient's sums (6 times their error).  A row without keys: p = exp2(s - inf) = 0.
+// the bias gradient's sums (6 times their error).  bf16 with a bias has them too in rows with |m| >= LARGE
+// (the others 1 for 1 / sum): m + log2(sum) is rounded by 2^-24 of m, and with a bias of -1e9 or the type's
+// lowest value on all that a row sees nothing of the sum is left.  A row without keys: p = exp2(s - inf) = 0.
+constexpr float LARGE = 4096.f;
 struct RowSum { float ref, inv; };
 template <class T>
 __device__ __forceinline__ void save_sum(const Args &a, size_t row, bool any, float m, float l, float inv) {
-    if constexpr (Elem<T>::NP == 1) {
-        a.lse[row] = any ? m + __builtin_amdgcn_logf(l) : INFINITY;
-    } else {
-        a.lse[row] = any ? m : INFINITY;
-        a.lse[(size_t)a.B * a.H * a.Nq + row] = inv;
-    }
+    const bool sum = Elem<T>::NP == 1 && !(a.bias && fabsf(m) >= LARGE);  // log2 of the sum, NaN among them
+    a.lse[row] = !any ? INFINITY : sum ? m + __builtin_amdgcn_logf(l) : m;
+    if (Elem<T>::NP > 1 || a.bias) a.lse[(size_t)a.B * a.H * a.Nq + row] = sum || !any ? 1.f : inv;
 }
-template <class T>
+template <class T, bool BIAS>
 __device__ __forceinline__ RowSum row_sum_of(const Args &a, size_t row, bool ok) {
-    RowSum r{INFINITY, 0.f};
+    RowSum r{INFINITY, 1.f};
     if (!ok) return r;
     r.ref = a.lse[row];
-    if constexpr (Elem<T>::NP > 1) r.inv = a.lse[(size_t)a.B * a.H * a.Nq + row];
+    if constexpr (Elem<T>::NP > 1 || BIAS) r.inv = a.lse[(size_t)a.B * a.H * a.Nq + row];
     return r;
 }
-template <class T>
+template <bool OWN>
 __device__ __forceinline__ float prob(float x, float inv) {  // x = s - ref
     const float p = __builtin_amdgcn_exp2f(x);
-    return Elem<T>::NP == 1 ? p : p * inv;
+    return OWN ? p * inv : p;
 }
 
 // ---------------------------------------------------------------------- forward --
@@ -785,8 +786,9 @@ constexpr int prob_pieces() { return Elem<T>::NP == 1 && KW > 1 ? 2 : Elem<T>::N
 // and ds are operands of the second products as they stand.  Bound by the matrix products and the
 // waits for their operands: 256 registers leave no room to read far ahead.  2 x 4096 x 16 heads x 128
 // bf16: 580 us (950 TFLOP/s); 64 columns 320 us (860); f32 2 x 2048 x 8 x 64: 215 us (160).
-template <class T, int DW, int QT, int KW, bool BIAS>
-__global__ __launch_bounds__(NT, (KW > 1 ? 1 : BIAS ? Shape<T, DW>::KV_BIAS_WAVES : Shape<T, DW>::KV_WAVES)) void attn_bwd_kv(Args a) {
+// OWN: probabilities are multiplied by the rows' 1 / sum.
+template <class T, int DW, int QT, int KW, bool BIAS, bool OWN>
+__device__ __forceinline__ void bwd_kv_rows(const Args &a) {
     constexpr int NP = Elem<T>::NP, PP = prob_pieces<T, KW>(), DP = pitch(DW), ND = blocks(DW), PLANE = QT * DP, ROWS = 128 / KW;
     static_assert(QT % (32 * KW) == 0, "tile");
     extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
@@ -823,12 +825,12 @@ __global__ __launch_bounds__(NT, (KW > 1 ? 1 : BIAS ? Shape<T, DW>::KV_BIAS_WAVE
             if (first < sp.nq) qd.issue(Q, a.qs[1], dO, a.dos[1], first, sp.nq, a.D, nullptr);
             // the rows' sums and dots go through registers into one of two buffers, a tile ahead: a
             // load that is waited for at each tile costs as much as the tile
-            RowSum rs{INFINITY, 0.f};
+            RowSum rs{INFINITY, 1.f};
             float dot = 0.f;
             const bool mine = threadIdx.x < QT;
             if (mine && first < sp.nq) {
                 const int i = first + threadIdx.x;
-                rs = row_sum_of<T>(a, row0 + i, i < sp.nq);
+                rs = row_sum_of<T, BIAS>(a, row0 + i, i < sp.nq);
                 lt[threadIdx.x] = -rs.ref;
                 it[threadIdx.x] = rs.inv;
                 et[threadIdx.x] = i < sp.nq ? a.delta[row0 + i] : 0.f;
@@ -840,7 +842,7 @@ __global__ __launch_bounds__(NT, (KW > 1 ? 1 : BIAS ? Shape<T, DW>::KV_BIAS_WAVE
                 if (i0 + QT < sp.nq) {
                     qd.issue(Q, a.qs[1], dO, a.dos[1], i0 + QT, sp.nq, a.D, nullptr);
                     const int i = i0 + QT + threadIdx.x;
-                    rs = row_sum_of<T>(a, row0 + i, mine && i < sp.nq);
+                    rs = row_sum_of<T, BIAS>(a, row0 + i, mine && i < sp.nq);
                     dot = mine && i < sp.nq ? a.delta[row0 + i] : 0.f;
                 }
 #pragma unroll
@@ -865,7 +867,7 @@ __global__ __launch_bounds__(NT, (KW > 1 ? 1 : BIAS ? Shape<T, DW>::KV_BIAS_WAVE
                         const int row = now + 32 * t + 2 * r0 + 4 * half;
                         const f32x4 ref = *reinterpret_cast<const f32x4_m *>(lt + row), dot4 = *reinterpret_cast<const f32x4_m *>(et + row);
                         f32x4 inv{1.f, 1.f, 1.f, 1.f};
-                        if constexpr (NP > 1) inv = *reinterpret_cast<const f32x4_m *>(it + row);
+                        if constexpr (OWN) inv = *reinterpret_cast<const f32x4_m *>(it + row);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int r = r0 + e;
@@ -876,7 +878,7 @@ __global__ __launch_bounds__(NT, (KW > 1 ? 1 : BIAS ? Shape<T, DW>::KV_BIAS_WAVE
                             } else {
                                 x = __builtin_fmaf(s[r], scale2, ref[e]);
                             }
-                            s[r] = prob<T>(x, inv[e]);
+                            s[r] = prob<OWN>(x, inv[e]);
                             dp[r] = s[r] * (dp[r] - dot4[e]);
                         }
                     }
@@ -982,6 +984,26 @@ __global__ __launch_bounds__(NT, (KW > 1 ? 1 : BIAS ? Shape<T, DW>::KV_BIAS_WAVE
     }
 }
 
+// bf16 with a bias: multiplied only where a row asks for it, which the query gradients' waves have noted (2 x
+// 2048 x 16 heads x 128, forward and backward: 348 us with the multiplication, 333 with the notes)
+template <class T, int DW, int QT, int KW, bool BIAS>
+__global__ __launch_bounds__(NT, (KW > 1 ? 1 : BIAS ? Shape<T, DW>::KV_BIAS_WAVES : Shape<T, DW>::KV_WAVES)) void attn_bwd_kv(Args a) {
+    constexpr bool F32 = Elem<T>::NP > 1;
+    if constexpr (!F32 && BIAS) {
+        const Where w = where(a.B, a.Hk * a.groups, (a.Nk + 128 / KW - 1) / (128 / KW));
+        const int64_t n = (int64_t)(a.H / a.Hk / a.groups) * ((a.Nq + a.tile_rows - 1) / a.tile_rows) * 4;  // its heads are neighbours
+        const int *own = a.own + ((int64_t)w.b * a.Hk * a.groups + w.h) * n;
+        int any = !a.own;  // (a call without query gradients has no notes)
+        if (a.own)
+            for (int64_t i = threadIdx.x & 63; i < n; i += 64) any |= own[i];
+        if (__any(any)) {  // (the same in every wave)
+            bwd_kv_rows<T, DW, QT, KW, BIAS, true>(a);
+            return;
+        }
+    }
+    bwd_kv_rows<T, DW, QT, KW, BIAS, F32>(a);
+}
+
 // dk and dv of a group from its parts, in order
 template <class T>
 __global__ __launch_bounds__(NT) void sum_group(Args a) {
@@ -1084,10 +1106,14 @@ __global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DW>::Q_WAVES : 1)) void att
                     a.D, lane, df, odd);
     const float sign = odd ? -1.f : 1.f;
     const size_t row = ((size_t)w.b * a.H + w.h) * a.Nq + i;
-    const RowSum rs = row_sum_of<T>(a, row, i < sp.nq);
+    const RowSum rs = row_sum_of<T, BIAS>(a, row, i < sp.nq);
     const float delta = row_dot<T, DW>(a, w.b, w.h, i, i < sp.nq, lane);
     if (half == 0 && share == 0 && i < a.Nq) a.delta[row] = delta;  // (the key gradients read it)
-    const float scale2 = a.scale * LOG2E;
+    if constexpr (BIAS && NP == 1) {
+        const bool own = __any(rs.inv != 1.f);
+        if (lane == 0) a.own[(((int64_t)w.b * a.H + w.h) * tiles + tile) * 4 + wave] = own;
+    }
+    const float scale2 = a.scale * LOG2E, delta_inv = delta * rs.inv;
     f32x16 acc[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) acc[d] = zero16();
@@ -1122,7 +1148,8 @@ __global__ __launch_bounds__(NT, (KW == 1 ? Shape<T, DW>::Q_WAVES : 1)) void att
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const float x = BIAS ? s[r] - rs.ref : __builtin_fmaf(s[r], scale2, -rs.ref);
-                s[r] = prob<T>(x, rs.inv) * (NP > 1 ? __builtin_fmaf(dp[r], sign, -delta) : dp[r] - delta);
+                if constexpr (NP > 1) s[r] = prob<true>(x, rs.inv) * __builtin_fmaf(dp[r], sign, -delta);
+                else s[r] = prob<false>(x, 1.f) * __builtin_fmaf(dp[r], rs.inv, -delta_inv);
             }
             if (edge) keep_only(s, visible(a, j - (i + sp.start), seen_keys(j, sp.nk, mask), half), 0.f);
             if (BIAS && a.dbias) dg.tile(s, j - qw, bins, a.bk.far, lane);
@@ -1411,6 +1438,11 @@ size_t bins_bytes(const hreg_tok_attn_t *p) {
     const size_t rows = bwd_plan(p).tile_rows, tiles = (p->Nq + rows - 1) / rows;
     return (p->B * p->H * tiles * (2 * (size_t)p->max_distance + 1) * 4 + 255) / 256 * 256;
 }
+size_t own_bytes(const hreg_tok_attn_t *p) {
+    if (!p->bias || p->dtype != HREG_TOK_BF16) return 0;
+    const size_t rows = bwd_plan(p).tile_rows;
+    return (p->B * p->H * ((p->Nq + rows - 1) / rows) * 16 + 255) / 256 * 256;
+}
 size_t delta_bytes(const hreg_tok_attn_t *p) { return ((size_t)p->B * p->H * p->Nq * 4 + 255) / 256 * 256; }
 
 }  // namespace
@@ -1420,7 +1452,7 @@ extern "C" {
 size_t hreg_tok_attn_ws_bytes(const hreg_tok_attn_t *p, int backward) {
     if (!p || p->B < 0 || p->Nq < 0 || p->Nk < 0 || p->H < 1 || p->Hk < 1 || p->H % p->Hk || p->D < 1) return 0;
     if (!backward) return part_floats(p, split_of(p)) * (p->D + 2) * 4;
-    return delta_bytes(p) + bins_bytes(p) + 2 * group_floats(p) * 4;
+    return delta_bytes(p) + bins_bytes(p) + own_bytes(p) + 2 * group_floats(p) * 4;
 }
 
 int hreg_tok_attn_fwd(const hreg_tok_attn_t *p, void *stream) {
@@ -1453,7 +1485,9 @@ int hreg_tok_attn_bwd(const hreg_tok_attn_t *p, void *stream) {
     a.delta = static_cast<float *>(p->ws);
     a.bins = reinterpret_cast<float *>(static_cast<char *>(p->ws) + delta_bytes(p));
     a.groups = plan.groups;
-    a.part = reinterpret_cast<float *>(static_cast<char *>(p->ws) + delta_bytes(p) + bins_bytes(p));
+    char *const own = static_cast<char *>(p->ws) + delta_bytes(p) + bins_bytes(p);
+    if (a.dq || a.dbias) a.own = reinterpret_cast<int *>(own);  // (else the kernel that writes it does not run)
+    a.part = reinterpret_cast<float *>(own + own_bytes(p));
     a.sums = a.part + group_floats(p);
     if (a.B > 0) {
         const int rc2 = by_type<true>(p, a, stream);

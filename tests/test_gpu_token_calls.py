@@ -97,7 +97,7 @@ def test_bias_gradient_of_a_causal_call_keeps_its_early_rows():
     assert ((got.double() - want).norm() / want.norm()).item() < 2 ** -11
 
 
-@pytest.mark.parametrize("dtype,table", [(F, F)], ids=["fp32"])
+@pytest.mark.parametrize("dtype,table", [(F, F), (H, F), (H, H)], ids=["fp32", "bf16, fp32 table", "bf16"])
 @pytest.mark.parametrize("shape", [(2, 70, 70, 4, 2, 32), (2, 1, 300, 4, 2, 64), (10, 130, 130, 8, 2, 64)],
                          ids=["waves share rows", "keys split", "waves of their own"])
 @pytest.mark.parametrize("value", ["lowest", "-1e9", "largest"])
@@ -137,3 +137,61 @@ def test_a_key_with_the_lowest_bias_that_stands_alone(dtype):
     low = oracle.attention(q, k, v, causal=True, bias=bias, spec=(8, 6, False))["out"][0]
     out = tokens.attention(q, k, v, causal=True, bias=bias, buckets=tokens.Buckets(8, 6, False))
     assert ((out.double() - low).norm() / low.norm()).item() < 4 * max(oracle.U[dtype], 2.0 ** -20)
+
+
+@pytest.mark.parametrize("dtype", [F, H], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("shape", [(2, 70, 70, 4, 2, 32), (2, 1, 300, 4, 2, 64), (10, 130, 130, 8, 2, 64)],
+                         ids=["waves share rows", "keys split", "waves of their own"])
+def test_a_bias_of_minus_infinity_hides_its_keys(shape, dtype):
+    """as a mask does: no share, no gradient; a row that sees nothing else is 0"""
+    B, Nq, Nk, heads, key_heads, D = shape
+    q, k, v, do = (normal(i, B, n, h, D, dtype=dtype) for i, (n, h) in enumerate(((Nq, heads), (Nk, key_heads), (Nk, key_heads),
+                                                                                  (Nq, heads))))
+    spec = (4, 3, False)  # the own key, the one before, two before, the others
+    bias = normal(7, 4, heads, dtype=dtype)
+    bias[:2] = -float("inf")
+    early = 2 if Nq == Nk else 0
+    do[:, :early] = 0
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v, bias)]
+    out = tokens.attention(*leaves[:3], causal=True, bias=leaves[3], buckets=tokens.Buckets(*spec))
+    got = dict(zip(("out", "dq", "dk", "dv", "dbias"), (out.detach(), *torch.autograd.grad(out, leaves, do))))
+    # (-1e4 leaves no share in 64 bits either, but to rows that see nothing else: no gradient goes there)
+    want = oracle.attention(q, k, v, do=do, causal=True, bias=bias.clamp(min=-1e4), spec=spec)
+    assert not got["out"][:, :early].any() and not got["dq"][:, :early].any() and not got["dbias"][:2].any()
+    assert not got["dk"][:, Nk - 2:].any() and not got["dv"][:, Nk - 2:].any()
+    # a table entry is a sum of ds that may cancel (one query: the entries add up to 0), and each ds is off by at
+    # most 4 u of itself: the sum by 4 u of their magnitudes, at most twice those of p dp as sum p = 1 and |D| <= max |dp|
+    Q, K, V, dO = (t.double().transpose(1, 2).contiguous() for t in (q, k.repeat_interleave(heads // key_heads, 2),
+                                                                     v.repeat_interleave(heads // key_heads, 2), do))
+    back = Nk - Nq + torch.arange(Nq, device="cuda")[:, None] - torch.arange(Nk, device="cuda")[None]
+    at = back.clamp(0, 3)
+    score = Q @ K.transpose(2, 3).contiguous() / D ** 0.5 + bias.double()[at].permute(2, 0, 1)
+    p = torch.softmax(score.masked_fill(back < 0, -float("inf")), -1).nan_to_num()
+    dp = dO @ V.transpose(2, 3).contiguous()
+    ds = (p * (dp - (p * dp).sum(-1, keepdim=True))).abs().sum(0)
+    size = torch.stack([(ds * (at == n)).sum((1, 2)) for n in range(4)])
+    u = max(oracle.U[dtype], 2.0 ** -20)
+    for n in want:
+        a, b = (t[:, early:] if n in ("out", "dq") else t for t in (got[n].double(), want[n][0]))
+        assert ((a - b).norm() / (size if n == "dbias" else b).norm()).item() < 4 * u, n
+
+
+@pytest.mark.parametrize("low", [0.0, -1e9])
+@pytest.mark.parametrize("shape", [(2, 70, 90, 4, 2, 32), (10, 130, 140, 8, 2, 64)], ids=["waves share rows", "waves of their own"])
+def test_bf16_gradients_that_are_asked_for_alone(shape, low):
+    """with a bias: each gradient alone has the bits that it has beside the others, although it then is made without
+    the query gradients' kernel"""
+    B, Nq, Nk, heads, key_heads, D = shape
+    t = [normal(i, B, n, h, D, dtype=H) for i, (n, h) in enumerate(((Nq, heads), (Nk, key_heads), (Nk, key_heads)))]
+    t.append(normal(5, 16, heads, dtype=H) + low)
+    do = normal(6, B, Nq, heads, D, dtype=H)
+
+    def grads(wanted):
+        leaves = [x.clone().requires_grad_(i in wanted) for i, x in enumerate(t)]
+        out = tokens.attention(*leaves[:3], causal=True, bias=leaves[3], buckets=tokens.Buckets(16, 30, False))
+        return torch.autograd.grad(out, [leaves[i] for i in wanted], do)
+
+    full = grads(range(4))
+    for wanted in ((0,), (1,), (2,), (3,), (1, 2)):
+        for i, g in zip(wanted, grads(wanted)):
+            assert torch.equal(g, full[i]), wanted
