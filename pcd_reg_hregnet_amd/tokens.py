@@ -264,7 +264,12 @@ def attention(q, k, v, *, scale=None, causal=False, align_end=None, q_lengths=No
 
     bias [num_buckets, H] (float32 or q's type) and ``Buckets`` add a learned bias by the offset of
     key and query.  A finite entry hides no key, however low: rows that see nothing else share themselves out
-    among such keys.  With bfloat16 rows its gradient has their accuracy (about 2^-8 of it)."""
+    among such keys.  With bfloat16 rows its gradient has their accuracy (about 2^-8 of it).
+
+    bfloat16: sums are float32; the probabilities and their gradients are rounded for the products with v, k and q,
+    to bfloat16 in large calls, to 16 bits in those that do not fill the card or read few rows against a cache.  So
+    out and gradients are between once and one and a half times as far off as their own rounding, and a row's last
+    bit may depend on the batch that it comes in."""
     _check_tensor("attention", "q", q)
     dev, dtype = q.device, q.dtype
     for name, t in (("k", k), ("v", v)):
