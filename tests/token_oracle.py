@@ -94,7 +94,8 @@ def attention(q, k, v, *, scale=None, causal=False, align_end=None, q_lengths=No
             if bias is not None:
                 N = (nq * len(keys) + 16) * F32
                 val["dbias"][:, h].index_add_(0, lut.reshape(-1), ds.reshape(-1))
-                # (the bias gradient sums ds before its rounding to bf16, but uses the rounded out)
+                # (the bias gradient sums ds before its rounding to bf16; the rounding of out that eds counts is
+                # more than the kernel's D = do . o feels, which keeps what out lost)
                 bound["dbias"][:, h].index_add_(0, lut.reshape(-1), (eds + N * ds.abs()).reshape(-1))
     for name in ("dk", "dv"):
         if name in val:
