@@ -795,9 +795,9 @@ typedef struct {
     const int32_t *q_len, *k_len;
     const uint8_t *key_mask;
     int64_t mask_sb;
-    /* bias[num_buckets][H] (or NULL) of bias_dtype.  An offset o = j - i - start has bucket n up to
-     * n < exact, then exact + #{t: n >= thresh[t]}; n = |o|, plus num_buckets / 2 where o > 0, with
-     * `both`, else max(-o, 0).  exact = half of a side's buckets, nthresh = side - exact - 1,
+    /* bias[num_buckets][H] (or NULL) of bias_dtype; a finite entry hides no key, -infinity does.  An
+     * offset o = j - i - start has bucket n up to n < exact, then exact + #{t: n >= thresh[t]}; n = |o|,
+     * plus num_buckets / 2 where o > 0, with `both`, else max(-o, 0).  exact = half of a side's buckets, nthresh = side - exact - 1,
      * ascending thresholds <= max_distance <= 1024. */
     const void *bias;
     int bias_dtype, num_buckets, max_distance, both, nthresh;

@@ -1436,12 +1436,12 @@ size_t group_floats(const hreg_tok_attn_t *p) {
 size_t bins_bytes(const hreg_tok_attn_t *p) {
     if (!p->bias) return 0;
     const size_t rows = bwd_plan(p).tile_rows, tiles = (p->Nq + rows - 1) / rows;
-    return (p->B * p->H * tiles * (2 * (size_t)p->max_distance + 1) * 4 + 255) / 256 * 256;
+    return ((size_t)p->B * p->H * tiles * (2 * (size_t)p->max_distance + 1) * 4 + 255) / 256 * 256;
 }
 size_t own_bytes(const hreg_tok_attn_t *p) {
     if (!p->bias || p->dtype != HREG_TOK_BF16) return 0;
     const size_t rows = bwd_plan(p).tile_rows;
-    return (p->B * p->H * ((p->Nq + rows - 1) / rows) * 16 + 255) / 256 * 256;
+    return ((size_t)p->B * p->H * ((p->Nq + rows - 1) / rows) * 16 + 255) / 256 * 256;
 }
 size_t delta_bytes(const hreg_tok_attn_t *p) { return ((size_t)p->B * p->H * p->Nq * 4 + 255) / 256 * 256; }
 

@@ -156,9 +156,11 @@ struct Block {
 template <int TPR> constexpr int threads() { return TPR > 64 ? TPR : NT; }
 
 // How a thread's elements are reached.  WHOLE: every thread of a row has eight, 16-byte aligned, and
-// the call is the usual one (both norms, both gradients in, the rows' gradients out): nothing is
+// the call has it all (both norms, both gradients in, the rows' gradients out): nothing is
 // asked per thread and little per call.  ALIGNED: eight or none.  SINGLE: one by one, any alignment.
-// (rows of 4096 bf16, backward: 900 vector instructions for eight elements without WHOLE)
+// (67 million elements bf16, a gate for each row, us: rows of 4096 with both norms 122 forward and 232 backward,
+// without the norm behind the block, so ALIGNED, 116 and 375; of 4088 with both 124 and 405, 768: 146 and 340,
+// 5120: 164 and 361.  ALIGNED takes 137 registers at 512 threads a row, which leaves three waves a SIMD.)
 enum { SINGLE, ALIGNED, WHOLE };
 
 // sum over the TPR threads of a row, in every one of them
