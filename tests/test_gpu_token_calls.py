@@ -195,3 +195,61 @@ def test_bf16_gradients_that_are_asked_for_alone(shape, low):
     for wanted in ((0,), (1,), (2,), (3,), (1, 2)):
         for i, g in zip(wanted, grads(wanted)):
             assert torch.equal(g, full[i]), wanted
+
+
+@pytest.mark.parametrize("dtype", [F, H], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("shape", [(3, 1, 300, 8, 2, 64), (3, 3, 2000, 4, 2, 32), (3, 70, 140, 4, 2, 64), (12, 130, 200, 8, 2, 48)],
+                         ids=["one run", "eight runs", "waves share rows", "waves of their own"])
+def test_hidden_values_have_no_influence(shape, dtype):
+    """what stands behind the lengths or under the mask reaches no bit of a result, however a call is divided"""
+    B, Nq, Nk, heads, key_heads, D = shape
+    s = {n: normal(i, B, m, h, D, dtype=dtype) for i, (n, m, h) in enumerate((("q", Nq, heads), ("k", Nk, key_heads),
+                                                                             ("v", Nk, key_heads), ("do", Nq, heads)))}
+    bias = normal(9, 8, heads, dtype=dtype)
+    kl = torch.tensor([Nk - 37, 0, 9] * (B // 3), device="cuda", dtype=torch.int32)
+    ql = torch.tensor([Nq, Nq - 1, (Nq + 1) // 2] * (B // 3), device="cuda", dtype=torch.int32)
+    mask = torch.ones(B, Nk, dtype=torch.bool, device="cuda")
+    mask[:, 3:7] = False
+    dirty = {n: t.clone() for n, t in s.items()}
+    for b in range(B):
+        for n, bad in (("k", float("nan")), ("v", -float("inf"))):
+            dirty[n][b, kl[b].item():] = bad
+            dirty[n][b, 3:7] = bad
+        for n in ("q", "do"):
+            dirty[n][b, ql[b].item():] = float("nan")
+    results = []
+    for t in (s, dirty):
+        leaves = [x.clone().requires_grad_(True) for x in (t["q"], t["k"], t["v"], bias)]
+        out = tokens.attention(*leaves[:3], causal=True, k_lengths=kl, q_lengths=ql, key_mask=mask, bias=leaves[3],
+                               buckets=tokens.Buckets(8, 6, True))
+        results.append([out.detach(), *torch.autograd.grad(out, leaves, t["do"])])
+    for a, b in zip(*results):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
+def test_calls_on_two_streams_at_once():
+    """each call has buffers of its own: two programs' steps that overlap give the bits of a step alone"""
+    def inputs(seed, dtype):
+        t = [normal(seed + i, 4, 300, 8, 64, dtype=dtype).requires_grad_(True) for i in range(3)]
+        return t, normal(seed + 7, 4, 300, 8, 64, dtype=dtype), normal(seed + 8, 16, 8, dtype=dtype).requires_grad_(True)
+
+    def step(t, do, bias):
+        out = tokens.attention(*t, causal=True, bias=bias, buckets=tokens.Buckets(16, 30, False))
+        _, h = tokens.gated_residual_norm(out.flatten(2), t[0].flatten(2), post_norm="rms", p=0.1, seed=5)
+        with torch.no_grad():
+            one = tokens.attention(t[0][:, -1:], t[1], t[2], causal=True)
+        return [h.detach(), one, *torch.autograd.grad(h, [*t, bias], do.flatten(2))]
+
+    sets = [inputs(20, F), inputs(40, H)]
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(6):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(step(*sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(g, want[i]))
